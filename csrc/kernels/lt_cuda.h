@@ -278,6 +278,19 @@ int lt_paged_decode_window(const void* q, const void* k_cache, const void* v_cac
 int lt_kv_append(const void* k_new, const void* v_new, void* k_cache, void* v_cache, const int* slots, long long n_tok,
                  int Hkv, int D, int block_size, int kv_fp8, float k_scale, float v_scale, void* stream);
 
+// ---- token_embedding.cu: rows of a table times a scale, gradient by sorted tokens; type 0 fp32, 1 bf16, 2 fp16
+int lt_token_embedding_fwd(int type, const void* idx, int idx32, const void* table, void* out, long long n, int D, int V, float scale, void* stream);
+int lt_token_embedding_bwd(int type, const void* idx, int idx32, const void* dout, long long ldd, void* grad, long long n, int D, int V, float scale, long long pad,
+                           void* order, float* part, int tile, void* stream);
+
+// ---- distill.cu: loss and gradient against a teacher's top logits
+int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t, const long long* idx, int N, int V, int K, float temperature, unsigned char* flags,
+               int fill_flags, const float* up, int up_rows, int skip_one, float* stats, int have_stats, float* loss, float* out, void* grad, void* stream);
+
+// ---- sample.cu: tokens by temperature, top-k, top-p and min-p from given random numbers
+int lt_sample_tokens(int type, const void* z, long long ldz, const void* u, int u64bit, const float* tau, const int* top_k, const float* top_p, const float* min_p,
+                     double tau1, int top_k1, double top_p1, double min_p1, int rows, int V, long long* tokens, float* logprobs, void* stream);
+
 // ---- pointwise.cu: RoPE, SwiGLU, GELU, embedding, casts, axpby
 int lt_rope(void* x, const float* cos_t, const float* sin_t, const int* pos, long long rows, int T, int heads, int hd,
             long long row_stride, int backward, void* stream);

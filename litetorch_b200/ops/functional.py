@@ -9,6 +9,7 @@ missing: loading it raises.
 from __future__ import annotations
 
 import math
+from operator import index
 from typing import Optional
 
 import torch
@@ -489,6 +490,205 @@ def embedding(idx, table):
     if _native(table) and table.shape[1] % 8 == 0 and idx.is_cuda:
         return _Embedding.apply(idx, table)
     return F.embedding(idx.to(torch.int64), table)
+
+
+class _TokenEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, idx, table, scale, pad):
+        idx = K._dense_index(idx, torch.int64, torch.int32)
+        ctx.save_for_backward(idx)
+        ctx.vocab, ctx.scale, ctx.pad = table.shape[0], scale, pad
+        return K.token_embedding(idx, table.contiguous(), scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        (idx,) = ctx.saved_tensors
+        return None, K.token_embedding_grad(idx, dout, ctx.vocab, ctx.scale, ctx.pad), None, None
+
+
+_KERNEL_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _whole(name: str, t: torch.Tensor) -> None:
+    if not torch.is_tensor(t) or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise TypeError("%s: whole numbers are expected" % name)
+
+
+def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """scale * table[idx] for tokens idx [...] and a table [V, D]: [..., D], rounded once from fp32.  A token outside [0, V) gives a row of zeros and no
+    gradient; `padding_idx` (negative: from the end) gives its row and no gradient.  The table's gradient is summed over the sorted tokens in fp32 and in their
+    order, then rounded once, where `embedding` adds bf16 numbers with atomics: it is the same from run to run."""
+    _whole("token_embedding", idx)
+    if table.dim() != 2 or not table.is_floating_point():
+        raise TypeError("token_embedding: the table is a matrix of floating-point numbers")
+    V, D = table.shape
+    if idx.device != table.device:
+        raise ValueError("token_embedding: tokens on %s, table on %s" % (idx.device, table.device))
+    if V < 1 or V >= (1 << 31) - 1 or idx.numel() > (1 << 31) - 4097:
+        raise ValueError("token_embedding: a table of 1 to 2^31 - 2 rows and fewer than 2^31 - 4096 tokens are expected")
+    pad = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError("token_embedding: padding_idx %d is not among %d rows" % (padding_idx, V))
+        pad = int(padding_idx) % V
+    if table.is_cuda and table.dtype in _KERNEL_TYPES:
+        return _TokenEmbedding.apply(idx.reshape(-1), table, float(scale), pad).view(*idx.shape, D)
+    flat = idx.reshape(-1).to(torch.int64)
+    inside = ((flat >= 0) & (flat < V))[:, None]
+    wide = table if table.dtype == torch.float64 else table.float()
+    rows = wide[flat.clamp(0, V - 1)]
+    if pad >= 0:
+        rows = torch.where((flat == pad)[:, None], rows.detach(), rows)
+    return torch.where(inside, rows * scale, torch.zeros_like(rows)).to(table.dtype).view(*idx.shape, D)
+
+
+# ---------------------------------------------------------------------------------------------- distillation
+class _Distillation(torch.autograd.Function):
+    """The loss is one pass over the logits.  Where one number comes back for all rows, the same pass leaves the gradient for an upstream gradient of 1, which
+    backward only forms again if it is another one: [N, V] is then read and written once for both.  With a number for every row, and while a graph is
+    recorded (whose backward may be replayed by itself), backward forms it from the logits and their kept maxima and sums."""
+
+    @staticmethod
+    def forward(ctx, z, t, idx, temperature, reduction):
+        rows = K.DistillRows(z, t, idx, temperature, reduction == "mean")
+        ahead = ctx.needs_input_grad[0] and reduction != "none" and not torch.cuda.is_current_stream_capturing()
+        loss, ctx.grad, kept = rows.loss(reduction != "none", ahead)
+        ctx.save_for_backward(z, rows.t, rows.idx, *kept)
+        ctx.temperature, ctx.mean = temperature, reduction == "mean"
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        z, t, idx, *kept = ctx.saved_tensors
+        ahead, ctx.grad = ctx.grad, None                       # handed out once
+        if ahead is not None and torch.cuda.is_current_stream_capturing():
+            ahead = None
+        rows = K.DistillRows(z, t, idx, ctx.temperature, ctx.mean)
+        return rows.grad(kept, up.contiguous(), ahead), None, None, None, None
+
+
+def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_idx: torch.Tensor, temperature: float = 1.0,
+                      reduction: str = "mean") -> torch.Tensor:
+    """Distance of a student, logits [..., V], from a teacher of whom the top K logits are known, teacher_logits [..., K] at the classes teacher_idx [..., K]:
+
+        T^2 sum_k p_k (log p_k - log q[idx_k]),   p = softmax(teacher_logits / T) over the K entries,   q = softmax(logits / T) over all V classes
+
+    An entry whose class is outside [0, V) (-1 for padding) or whose logit is -inf is not there; a row without any has loss 0 and no gradient.
+    reduction: "mean" over the rows that have a teacher, "sum", or "none" (a loss for every row, fp32).  The teacher gets no gradient."""
+    if not logits.is_floating_point() or not teacher_logits.is_floating_point():
+        raise TypeError("distillation_loss: logits are floating-point numbers")
+    _whole("distillation_loss", teacher_idx)
+    if logits.dim() < 1 or teacher_logits.shape != teacher_idx.shape or teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_logits.dim() != logits.dim():
+        raise ValueError("distillation_loss: logits %s, teacher's logits %s at %s" % (list(logits.shape), list(teacher_logits.shape), list(teacher_idx.shape)))
+    if not logits.device == teacher_logits.device == teacher_idx.device:
+        raise ValueError("distillation_loss: student and teacher are on different devices")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("distillation_loss: reduction %r" % (reduction,))
+    if not (0.0 < temperature < math.inf):
+        raise ValueError("distillation_loss: a temperature above 0 is expected, not %r" % (temperature,))
+    V, top = logits.shape[-1], teacher_idx.shape[-1]
+    if not 1 <= top <= 1024 or V < 1:
+        raise ValueError("distillation_loss: 1 to 1024 of the teacher's logits and at least one class are expected")
+    lead = logits.shape[:-1]
+    z, t, idx = logits.reshape(-1, V), teacher_logits.detach().reshape(-1, top), teacher_idx.reshape(-1, top)
+    if z.shape[0] >= 1 << 31 or V >= 1 << 30:
+        raise ValueError("distillation_loss: too many rows or classes")
+    if z.is_cuda and z.dtype in _KERNEL_TYPES and z.shape[0] > 0:
+        loss = _Distillation.apply(z, t if t.dtype in _KERNEL_TYPES else t.float(), idx, float(temperature), reduction)
+    else:
+        wide = torch.promote_types(z.dtype, torch.float32)
+        there = (idx >= 0) & (idx < V) & (t != -math.inf)
+        has = there.any(1)
+        log_p = torch.log_softmax((t.to(wide) / temperature).masked_fill(~there, -math.inf).masked_fill(~has[:, None], 0.0), -1)
+        log_q = torch.log_softmax(z.to(wide) / temperature, -1).gather(1, idx.to(torch.int64).clamp(0, V - 1))
+        p = log_p.exp().masked_fill(~there, 0.0)
+        counts = p != 0
+        loss = (p * (torch.where(counts, log_p, 0.0) - torch.where(counts, log_q, 0.0))).sum(1) * temperature ** 2
+        if reduction != "none":
+            loss = loss.sum() / (has.sum().clamp(min=1) if reduction == "mean" else 1)
+        loss = loss if wide == torch.float64 else loss.float()
+    return loss.view(lead) if reduction == "none" else loss
+
+
+# ---------------------------------------------------------------------------------------------- sampling
+def _sample_plain(z, u, tau, k, p, low):
+    """(tokens, log probabilities) in 64 bits; parameters as columns."""
+    V = z.shape[1]
+    z = torch.where(torch.isnan(z), -math.inf, z.double())
+    top = z.amax(1, keepdim=True)
+    greedy = ~(tau > 0)
+    tau = torch.where(greedy, 1.0, tau)
+    k = torch.where(greedy, 1.0, k)
+    x = torch.where(z == top, 0.0, torch.where(z == -math.inf, -math.inf, (z - top) / tau))
+    e = torch.exp(x)
+    order = torch.sort(z, dim=1, descending=True, stable=True).indices
+    first = (torch.arange(V, device=z.device) < k) | (k <= 0)
+    ranked = e.gather(1, order) * first
+    before = ranked.cumsum(1) - ranked
+    first &= (before < p * ranked.sum(1, keepdim=True)) | (p >= 1.0) | (torch.arange(V, device=z.device) == 0)
+    keep = torch.zeros_like(first).scatter_(1, order, first) & (e >= low.clamp(max=1.0))
+    e = e * keep
+    total = e.sum(1, keepdim=True)
+    cum = e.cumsum(1)
+    u = torch.where(u > 0, u, 0.0)[:, None]
+    last = torch.where(e > 0, torch.arange(V, device=z.device), 0).amax(1)
+    tokens = torch.minimum((cum <= u * total).sum(1), last)
+    logprobs = x.gather(1, tokens[:, None])[:, 0] - torch.log(total[:, 0])
+    empty = top[:, 0] == -math.inf
+    return torch.where(empty, -1, tokens), torch.where(empty, -math.inf, logprobs).float()
+
+
+@torch.no_grad()
+def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(tokens, log probabilities) for logits [..., V], drawn with the given random numbers uniform [...] in [0, 1).  With w = e^((z - max z) / temperature)
+    and the tokens in order of their logit, of equals the lowest index first:
+
+        top_k > 0    the first k stay
+        top_p < 1    those stay whose predecessors' mass is below top_p times the mass of what stayed (the first always does)
+        min_p > 0    those stay with w >= min_p
+
+    and the token is the first, by index, at which the cumulated mass of what stays exceeds `uniform` times all of it; its log probability is that among what
+    stays.  temperature <= 0 takes the largest logit.  Every parameter is a number or a tensor with one for every row.  NaN counts as -inf; a row of nothing
+    else gives token -1.  The choice is that of exact sums: it does not change with the batch, the device or the run."""
+    if not logits.is_floating_point() or logits.dim() < 1:
+        raise TypeError("sample_tokens: logits [..., V] of floating-point numbers are expected")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if not 1 <= V <= 1 << 19:
+        raise ValueError("sample_tokens: 1 to 524288 tokens are expected, not %d" % V)
+    if not torch.is_tensor(uniform) or not uniform.is_floating_point() or uniform.shape != lead or uniform.device != logits.device:
+        raise ValueError("sample_tokens: a random number for every row, on the logits' device, is expected")
+    z = logits.detach().reshape(-1, V)
+    rows = z.shape[0]
+    u = uniform.detach().reshape(-1)
+    u = (u if u.dtype == torch.float64 else u.float()).contiguous()
+    if rows >= 1 << 28:
+        raise ValueError("sample_tokens: too many rows")
+    given = []
+    for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if torch.is_tensor(v):
+            if v.device != logits.device or v.shape not in (lead, torch.Size(())):
+                raise ValueError("sample_tokens: %s has one number, or one for every row on the logits' device" % name)
+            if dtype == torch.int32:
+                _whole("sample_tokens: top_k", v)
+                v = v.clamp(0, V)
+            v = v.detach().expand(lead).reshape(-1).to(dtype).contiguous()
+        elif dtype == torch.int32:
+            v = index(v)
+        else:
+            v = float(v)
+            if v != v:
+                raise ValueError("sample_tokens: %s is NaN" % name)
+        given.append(v)
+    if rows == 0:
+        tokens, logprobs = torch.empty(0, dtype=torch.int64, device=z.device), torch.empty(0, dtype=torch.float32, device=z.device)
+    elif z.is_cuda and z.dtype in _KERNEL_TYPES:
+        tokens, logprobs = K.sample_tokens(z if z.stride(1) == 1 else z.contiguous(), u, *given)
+    else:
+        tokens, logprobs = _sample_plain(z, u.double(), *(v.double()[:, None] if torch.is_tensor(v) else torch.full((rows, 1), float(v), dtype=torch.float64, device=z.device)
+                                                          for v in given))
+    return tokens.view(lead), logprobs.view(lead)
 
 
 # ------------------------------------------------------------------------------------------------ softmax / dropout / router

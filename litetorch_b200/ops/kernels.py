@@ -6,6 +6,7 @@ tensors.  No autograd here: `litetorch_b200.ops.functional` wraps these into aut
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 from ctypes import c_void_p, c_int, c_longlong, c_float
@@ -14,9 +15,13 @@ import torch
 
 from .._native import cuda_lib
 
-_vp, _i, _ll, _f = c_void_p, c_int, c_longlong, c_float
+_vp, _i, _ll, _f, _d = c_void_p, c_int, c_longlong, c_float, ctypes.c_double
 
 _SIGS = {
+    "lt_token_embedding_fwd": [_i, _vp, _i, _vp, _vp, _ll, _i, _i, _f, _vp],
+    "lt_token_embedding_bwd": [_i, _vp, _i, _vp, _ll, _vp, _ll, _i, _i, _f, _ll, _vp, _vp, _i, _vp],
+    "lt_distill": [_i, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _f, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _vp],
+    "lt_sample_tokens": [_i, _vp, _ll, _vp, _i] + [_vp] * 4 + [_d, _i, _d, _d, _i, _i, _vp, _vp, _vp],
     "lt_residual_norm": [_i, _vp, _vp, _vp, _vp, _ll, _vp, _vp, _vp, _i, _vp, _f, _vp, _f, _vp, _vp, _i, _i, _i, _vp],
     "lt_latent_rope": [_i, _vp, _ll] + [_i] * 8 + [_vp, _f, _vp, _vp, _vp, _f, _vp, _i, _i, _vp, _vp, _vp],
     "lt_latent_decode": [_vp] * 7 + [_i] * 9 + [_f, _vp],
@@ -141,7 +146,7 @@ class LlamaLayer(ctypes.Structure):
 _bound = {}
 
 # Kernels launched per native call; `launch_count()` is what bench.py reports as "gpu_launches".
-_LAUNCHES_PER_CALL = {"lt_gemm_num_tiles": 0, "lt_gemm_skinny_set_target": 0, "lt_adam_q8": 3, "lt_set_wait_budget_cycles": 0, "lt_norm_bwd": 2, "lt_paged_decode": 2, "lt_paged_decode_window": 2, "lt_mlstm_prefill": 4, "lt_rglru_scan": 3, "lt_rglru_step": 2, "lt_flash_bwd": 3, "lt_flash_bwd_rope": 3, "lt_llama_layer_fwd": 8, "lt_llama_layer_bwd": 16, "lt_status_fetch": 0, "lt_sm_count": 0, "lt_gemm_set_tail_split": 0, "lt_reduce_parts": 0, "lt_reduce_all": 2, "lt_gemm_set_pair_mode": 0, "lt_flash_bwd_set_trace": 0, "lt_flash_fwd_set_trace": 0, "lt_norm_bwd_ctas": 0, "lt_paged_decode_places": 0,
+_LAUNCHES_PER_CALL = {"lt_gemm_num_tiles": 0, "lt_token_embedding_bwd": 3, "lt_gemm_skinny_set_target": 0, "lt_adam_q8": 3, "lt_set_wait_budget_cycles": 0, "lt_norm_bwd": 2, "lt_paged_decode": 2, "lt_paged_decode_window": 2, "lt_mlstm_prefill": 4, "lt_rglru_scan": 3, "lt_rglru_step": 2, "lt_flash_bwd": 3, "lt_flash_bwd_rope": 3, "lt_llama_layer_fwd": 8, "lt_llama_layer_bwd": 16, "lt_status_fetch": 0, "lt_sm_count": 0, "lt_gemm_set_tail_split": 0, "lt_reduce_parts": 0, "lt_reduce_all": 2, "lt_gemm_set_pair_mode": 0, "lt_flash_bwd_set_trace": 0, "lt_flash_fwd_set_trace": 0, "lt_norm_bwd_ctas": 0, "lt_paged_decode_places": 0,
                       "lt_adam_chunk_elems": 0}
 _launches = [0]
 
@@ -1616,3 +1621,105 @@ def moe_expert_bwd(gu, dh_u, w, slot_src):
                                   hw.data_ptr(), dw.data_ptr(), S, F, _stream())
     _check(rc, "lt_moe_expert_bwd")
     return dgu, hw, dw
+
+
+# ------------------------------------------------------------------------------------------------ vocabulary: embedding, distillation, sampling
+_ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _on(t: torch.Tensor):
+    """The tensor's device as the current one."""
+    return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[idx] as [tokens, D] (fp32, bf16 or fp16, rounded once); a token outside the table gives zeros."""
+    assert table.dim() == 2 and table.is_contiguous() and table.dtype in _ELEM and idx.device == table.device
+    idx = _dense_index(idx, torch.int64, torch.int32)
+    V, D = table.shape
+    out = torch.empty((idx.numel(), D), dtype=table.dtype, device=table.device)
+    with _on(table):
+        _check(_fn("lt_token_embedding_fwd")(_ELEM[table.dtype], idx.data_ptr(), 1 if idx.dtype == torch.int32 else 0, table.data_ptr(), out.data_ptr(),
+                                             idx.numel(), D, V, float(scale), _stream()), "lt_token_embedding_fwd")
+    return out
+
+
+def token_embedding_grad(idx: torch.Tensor, dout: torch.Tensor, vocab: int, scale: float = 1.0, padding_idx: int = -1) -> torch.Tensor:
+    """The gradient [vocab, D] of `token_embedding`'s table from dout [tokens, D]: sums in fp32 in the order of the tokens, rounded once, the same from run
+    to run.  Tokens outside the table and `padding_idx` give nothing."""
+    assert dout.dim() == 2 and dout.dtype in _ELEM and idx.numel() == dout.shape[0] and idx.device == dout.device
+    idx = _dense_index(idx, torch.int64, torch.int32)
+    if dout.stride(1) != 1:
+        dout = dout.contiguous()
+    n, D = dout.shape
+    grad = torch.empty((vocab, D), dtype=dout.dtype, device=dout.device)
+    tile = 32
+    order = torch.empty((2, max(n, 1)), dtype=torch.int64, device=dout.device)
+    part = torch.empty(((n + tile - 1) // tile, 2, D), dtype=torch.float32, device=dout.device)
+    with _on(dout):
+        _check(_fn("lt_token_embedding_bwd")(_ELEM[dout.dtype], idx.data_ptr(), 1 if idx.dtype == torch.int32 else 0, dout.data_ptr(), dout.stride(0), grad.data_ptr(),
+                                             n, D, int(vocab), float(scale), int(padding_idx), order.data_ptr(), part.data_ptr(), tile, _stream()),
+               "lt_token_embedding_bwd")
+    return grad
+
+
+class DistillRows:
+    """Rows of student logits z [N, V] (rows may be strided) against a teacher's top logits t [N, K] at classes idx [N, K] (`functional.distillation_loss` has
+    the formulas).  `loss` may form the gradient for an upstream gradient of 1 on the way; `grad` forms it from the kept statistics."""
+
+    def __init__(self, z, t, idx, temperature: float, mean: bool):
+        assert z.dim() == 2 and t.shape == idx.shape and t.dim() == 2 and t.shape[0] == z.shape[0] and z.dtype in _ELEM and t.dtype in _ELEM
+        assert z.device == t.device == idx.device and 1 <= t.shape[1] <= 1024 and temperature > 0 and z.shape[0] < 1 << 31
+        self.z = z if z.stride(1) == 1 else z.contiguous()
+        self.t, self.idx = t.contiguous(), idx.to(torch.int64).contiguous()
+        self.temperature, self.mean = float(temperature), mean
+
+    def _run(self, flags, fill, up, skip_one, stats, have, loss, out, grad):
+        z = self.z
+        with _on(z):
+            _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), _ELEM[self.t.dtype], self.t.data_ptr(), self.idx.data_ptr(), z.shape[0], z.shape[1],
+                                     self.t.shape[1], self.temperature, _p(flags), fill, _p(up), 1 if up is not None and up.dim() else 0, skip_one, _p(stats), have,
+                                     _p(loss), _p(out), _p(grad), _stream()), "lt_distill")
+        _launches[0] += (fill and flags is not None) + (out is not None)
+
+    def loss(self, reduce: bool, with_grad: bool):
+        """(loss: the mean or sum, or [N] without `reduce`; gradient or None; what `grad` needs)."""
+        N, dev = self.z.shape[0], self.z.device
+        rows = torch.empty(N, dtype=torch.float32, device=dev)
+        stats = torch.empty((N, 2), dtype=torch.float32, device=dev)
+        flags = torch.empty(N, dtype=torch.uint8, device=dev) if self.mean else None
+        out = torch.empty((), dtype=torch.float32, device=dev) if reduce else None
+        grad = torch.empty(self.z.shape, dtype=self.z.dtype, device=dev) if with_grad else None
+        self._run(flags, 1, None, 0, stats, 0, rows, out, grad)
+        return (out if reduce else rows), grad, (stats, flags)
+
+    def grad(self, kept, up, grad=None):
+        """The gradient for the upstream gradient `up` (one number on the device, or one a row).  With `grad`, which holds it for 1: nothing is done where `up` is 1."""
+        stats, flags = kept
+        assert up.dtype == torch.float32 and up.is_contiguous()
+        there = grad is not None
+        if not there:
+            grad = torch.empty(self.z.shape, dtype=self.z.dtype, device=self.z.device)
+        self._run(flags, 0, up, 1 if there else 0, stats, 1, None, None, grad)
+        return grad
+
+
+def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(tokens int64 [rows], their log probabilities fp32 [rows]) of logits [rows, V] by one random number a row; every parameter a number or a tensor [rows]
+    (`functional.sample_tokens` says what they do)."""
+    rows, V = logits.shape
+    assert logits.dtype in _ELEM and (V == 1 or logits.stride(1) == 1) and 1 <= V <= 1 << 19 and uniform.dtype in (torch.float32, torch.float64)
+    assert uniform.shape == (rows,) and uniform.is_contiguous() and uniform.device == logits.device
+    ptrs, nums = [], []
+    for v, off, dtype in ((temperature, 1.0, torch.float32), (top_k, 0, torch.int32), (top_p, 1.0, torch.float32), (min_p, 0.0, torch.float32)):
+        own = torch.is_tensor(v)
+        assert not own or (v.shape == (rows,) and v.dtype == dtype and v.is_contiguous() and v.device == logits.device)
+        ptrs.append(v.data_ptr() if own else None)
+        nums.append(off if own else v)
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    with _on(logits):
+        _check(_fn("lt_sample_tokens")(_ELEM[logits.dtype], logits.data_ptr(), logits.stride(0), uniform.data_ptr(), 1 if uniform.dtype == torch.float64 else 0, *ptrs,
+                                       float(nums[0]), max(0, min(int(nums[1]), V)), float(nums[2]), float(nums[3]), rows, V, tokens.data_ptr(), logprobs.data_ptr(), _stream()),
+               "lt_sample_tokens")
+    return tokens, logprobs
