@@ -8,6 +8,7 @@
 #include "lt_cuda.h"
 
 #include <algorithm>
+#include <atomic>
 
 #include "common/elem.cuh"
 #include "common/host.h"
@@ -15,25 +16,27 @@
 
 namespace lt {
 
-constexpr int kDistillThreads = 512, kDistillWarps = kDistillThreads / 32, kDistillTop = 1024;
+constexpr int kDistillThreads = 1024, kDistillWarps = kDistillThreads / 32, kDistillTop = 1024, kDistillCluster = 8;
+constexpr int kLongThreads = 512, kLongWarps = kLongThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct DistillArgs {
   const void* z;
   long long ldz;
-  const void* t;                 // [N, K] of type t_type
-  int t_type;
-  const long long* idx;          // [N, K]
+  float2* entries;               // [N, K]: log2 p of the teacher's entries and their class (its bits); -1: not there, -2: none of the row is
   int N, V, K;
-  float temperature;
+  float temperature, c;          // c: log2(e) / temperature
   const unsigned char* flags;    // which rows have a teacher, for a mean; else null
   const float* up;               // upstream gradient: one (up_rows 0) or one for every row; null: 1
   int up_rows;
   int skip_one;                  // with one upstream gradient: return where it is 1 (the gradient is there)
-  float2* stats;                 // [N] maximum of z, and sum of e^((z - maximum) / T)
+  float2* stats;                 // [N] reference (the maximum of z log2(e) / T) and sum of 2^(z log2(e) / T - reference)
   int have_stats;
   float* loss;                   // [N] or null
-  void* grad;                    // [N, V] or null
+  void* grad;                    // [N, V] (pitch ldg, rows where those of z lie within 16 bytes) or null
+  long long ldg;
+  int cluster_log;               // log2 of the CTAs of a cluster
+  int* status;
 };
 
 __device__ __forceinline__ float load_as(int type, const void* p, long long i) {
@@ -42,15 +45,43 @@ __device__ __forceinline__ float load_as(int type, const void* p, long long i) {
 }
 __device__ __forceinline__ bool entry_there(float t, long long i, int V) { return i >= 0 && i < V && t != -INFINITY; }
 
-__global__ void __launch_bounds__(256) distill_flags_kernel(const void* t, int t_type, const long long* idx, int N, int V, int K, unsigned char* flags) {
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The teacher's side, a warp to a row: log2 of its probabilities, and whether it is there at all.
+__global__ void __launch_bounds__(256) distill_teacher_kernel(const void* t, int t_type, const long long* idx, int N, int V, int K, float c, float2* entries,
+                                                              unsigned char* flags) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
   for (long long r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < N; r += gridDim.x * 8ll) {
+    float m = -INFINITY, s = 0.f;
     bool any = false;
-    for (int k = lane; k < K && !any; k += 32) any = entry_there(load_as(t_type, t, r * K + k), idx[r * K + k], V);
+    for (int k = lane; k < K; k += 32) {
+      const float x = load_as(t_type, t, r * K + k);
+      if (!entry_there(x, idx[r * K + k], V)) continue;
+      any = true;
+      m = fmaxf(m, x);
+    }
     any = __any_sync(0xffffffffu, any);
-    if (lane == 0) flags[r] = any;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int k = lane; k < K; k += 32) {
+      const float x = load_as(t_type, t, r * K + k);
+      if (entry_there(x, idx[r * K + k], V)) s += ex2((x - m) * c);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float ls = log2f(s);
+    for (int k = lane; k < K; k += 32) {
+      const float x = load_as(t_type, t, r * K + k);
+      const long long i = idx[r * K + k];
+      entries[r * K + k] = make_float2((x - m) * c - ls, __int_as_float(entry_there(x, i, V) ? int(i) : any ? -1 : -2));
+    }
+    if (flags && lane == 0) flags[r] = any;
   }
 }
 
@@ -66,143 +97,429 @@ __device__ __forceinline__ int count_flags(const unsigned char* flags, int N, in
   return n;
 }
 
-// (maximum, sum of 2^(c (. - maximum))) of two parts.  Differences are taken before the factor: next to the maximum they are exact.
-__device__ __forceinline__ void join_max_sum(float& m, float& s, float om, float os, float c) {
-  const float nm = fmaxf(m, om);
-  s = (m == -INFINITY ? s : s * exp2f((m - nm) * c)) + (om == -INFINITY ? os : os * exp2f((om - nm) * c));
-  m = nm;
+// (reference, sum of 2^(. - reference)) over the warp.  Logits enter as fma(z, c, -reference), so that the reference is exact whatever its own rounding.
+__device__ __forceinline__ void warp_max_sum(float& m, float& s) {
+  const float own = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (own != -INFINITY) s *= ex2(own - m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
 }
-__device__ __forceinline__ void block_max_sum(float& m, float& s, float c, float2* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
-    join_max_sum(m, s, om, os, c);
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+// The first `bytes` of 16 (all that is read); the rest becomes zero.
+__device__ __forceinline__ void copy_async16_part(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_async8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
+// p[i] (bytes or 16-bit numbers) becomes v; returns what it was.
+template <typename LINK>
+__device__ __forceinline__ uint32_t exchange_small(LINK* p, int i, uint32_t v) {
+  constexpr int BITS = 8 * sizeof(LINK), PER = 4 / sizeof(LINK);
+  uint32_t* word = reinterpret_cast<uint32_t*>(p) + i / PER;
+  const int sh = i % PER * BITS;
+  const uint32_t mask = ((1u << BITS) - 1u) << sh;
+  uint32_t old = *reinterpret_cast<volatile uint32_t*>(word);
+  for (;;) {
+    const uint32_t seen = atomicCAS(word, old, (old & ~mask) | v << sh);
+    if (seen == old) return (old & mask) >> sh;
+    old = seen;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncthreads();
-  if (lane == 0) red[warp] = make_float2(m, s);
-  __syncthreads();
-  const float2 v = lane < kDistillWarps ? red[lane] : make_float2(-INFINITY, 0.f);
-  m = v.x;
-  s = v.y;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o);
-    join_max_sum(m, s, om, os, c);
+}
+// The teacher's probability of entry e's class (p by that entry alone) with those of the entries chained behind it that have the same.  Their sum is taken in
+// whole numbers of 2^-62: it must not depend on the chain's order.
+template <typename LINK>
+__device__ __noinline__ float chained_p(const float2* entries, const LINK* link, int e, float p) {
+  const int i = __float_as_int(entries[e - 1].y);
+  unsigned long long sum = 0;
+  int n = 0;
+  for (int o = e; o; o = link[o - 1])
+    if (__float_as_int(entries[o - 1].y) == i) {
+      const float x = ex2(entries[o - 1].x);
+      if (x != x) return x;
+      sum += (unsigned long long)(x * 4611686018427387904.f);
+      ++n;
+    }
+  return n > 1 ? float(double(sum) * (1.0 / 4611686018427387904.0)) : p;
+}
+// -inf in every element, and the largest element of 16 bytes (NaN only if there is nothing else).
+template <typename T> __device__ __forceinline__ uint32_t minus_inf() { return 0xff800000u; }
+template <> __device__ __forceinline__ uint32_t minus_inf<__nv_bfloat16>() { return 0xff80ff80u; }
+template <> __device__ __forceinline__ uint32_t minus_inf<__half>() { return 0xfc00fc00u; }
+template <typename T> __device__ __forceinline__ float max16(uint4 u) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else if constexpr (__is_same(T, __nv_bfloat16)) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
   }
+}
+// An 8-byte store to the place `dst` of CTA `cta`'s shared memory that is counted on the barrier `bar` there.
+__device__ __forceinline__ void send8(uint32_t dst, uint32_t bar, uint32_t cta, float2 v) {
+  asm volatile(
+      "{\n\t.reg .b32 rd, rb;\n\t.reg .b64 v;\n\t"
+      "mapa.shared::cluster.u32 rd, %0, %2;\n\tmapa.shared::cluster.u32 rb, %1, %2;\n\t"
+      "mov.b64 v, {%3, %4};\n\t"
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [rd], v, [rb];\n\t}"
+      ::"r"(dst), "r"(bar), "r"(cta), "f"(v.x), "f"(v.y)
+      : "memory");
 }
 
-template <typename T>
+// Shared memory of a CTA of so many threads, a multiple of 32.
+template <typename LINK, int VPT>
+struct DistillSmem {
+  static constexpr int kTop = sizeof(LINK) == 1 ? 255 : kDistillTop;      // entries that a LINK numbers
+  static constexpr int kVectors = 3, kEntries = 4, kChains = 3, kPeers = 4;           // rows in turn
+  static __host__ __device__ int entries(int nt) { return kVectors * VPT * nt * 16; }
+  static __host__ __device__ int peers(int nt, int K) { return entries(nt) + kEntries * K * 8; }
+  static __host__ __device__ int heads(int nt, int K) { return peers(nt, K) + kPeers * kDistillCluster * (nt / 32) * 8; }
+  static __host__ __device__ int links(int nt, int K) { return heads(nt, K) + kChains * nt * 4 * int(sizeof(LINK)); }
+  static __host__ __device__ int bytes(int nt, int K) { return links(nt, K) + kChains * K * int(sizeof(LINK)); }
+};
+
+// A cluster of CTAs holds a row, every thread up to VPT vectors of 16 bytes: a row is read from global memory once.  The threads go over their vectors twice, first
+// for the warps' maxima and sums, which go to all warps of the cluster, and then for the gradient; between the two they do the first pass over the
+// next row, so that nobody waits for the exchange, and the rows after that are on their way into shared memory.  There is no barrier of all threads:
+// a thread reads the vectors that it fetched itself, and one mbarrier a row counts the pairs that arrive and the warps that are through with the row before.
+// The teacher's classes are chained by the vector they lie in; the thread that writes the vector writes them again, from the 32-bit values.
+// EVEN: all rows begin and end with a vector.  LINK: the type that numbers entries.
+template <typename T, bool EVEN, typename LINK, int VPT>
 __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a) {
+  constexpr int VEC = kVec<T>;
+  typedef DistillSmem<LINK, VPT> S;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ __align__(8) uint64_t bars[S::kPeers];
+  __shared__ uint4 cut[2];                                    // the row's first and last vector, if they are cut
+  __shared__ int isum[kDistillWarps];
+  __shared__ int abort_flag;
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int VEC = kVec<T>;
-  __shared__ float2 red[32];
-  __shared__ float top_p[kDistillTop];
-  __shared__ int top_i[kDistillTop];
-  __shared__ float fsum[32];
-  __shared__ int isum[32];
   if (a.skip_one && a.up && a.up[0] == 1.f) return;
-  float mean = 1.f;
-  if (a.flags) mean = 1.f / float(max(1, count_flags(a.flags, a.N, isum)));
-  const float c = kLog2e / a.temperature;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int row = blockIdx.x; row < a.N; row += gridDim.x) {
-    const T* z = static_cast<const T*>(a.z) + row * a.ldz;
-    T* g = a.grad ? static_cast<T*>(a.grad) + (long long)row * a.V : nullptr;
-    // teacher: entries to shared memory, p over those that are there
-    float tm = -INFINITY, ts = 0.f;
-    for (int k = threadIdx.x; k < a.K; k += kDistillThreads) {
-      const float t = load_as(a.t_type, a.t, (long long)row * a.K + k);
-      const long long i = a.idx[(long long)row * a.K + k];
-      const bool there = entry_there(t, i, a.V);
-      top_i[k] = there ? int(i) : -1;
-      top_p[k] = t;
-      if (there) join_max_sum(tm, ts, t, 1.f, c);
+  float weight = a.temperature;
+  if (a.flags) weight /= float(max(1, count_flags(a.flags, a.N, isum)));
+  if (a.up && !a.up_rows) weight *= a.up[0];
+  const float c = a.c;
+  const int tid = threadIdx.x, lane = tid & 31, nt = blockDim.x, nw = nt >> 5;
+  const int clog = a.cluster_log, rank = clog ? int(cluster_ctarank()) : 0;
+  uint4* vectors = reinterpret_cast<uint4*>(smem) + tid;      // [3][VPT][nt], from this thread's
+  float2* entry_buf = reinterpret_cast<float2*>(smem + S::entries(nt));   // [4][K]
+  float2* peers = reinterpret_cast<float2*>(smem + S::peers(nt, a.K));    // [4][CTAs][warps]: (reference, sum)
+  LINK* heads = reinterpret_cast<LINK*>(smem + S::heads(nt, a.K));        // [3][nt][4]: number of a vector's first entry + 1
+  LINK* links = reinterpret_cast<LINK*>(smem + S::links(nt, a.K));        // [3][K]: that of an entry's next
+  const int pairs = nw << clog;
+  const uint32_t bar0 = smem_u32(bars);
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < S::kPeers; ++i) mbar_init(bar0 + 8 * i, nw);
+    fence_barrier_init();
+  }
+  for (int i = tid; i < S::kChains * nt * int(sizeof(LINK)); i += nt) reinterpret_cast<uint32_t*>(heads)[i] = 0u;
+#pragma unroll
+  for (int k = 0; k < S::kVectors * VPT; ++k) vectors[k * nt] = make_uint4(minus_inf<T>(), minus_inf<T>(), minus_inf<T>(), minus_inf<T>());
+
+  // Vector v of a row holds its elements [v VEC - shift, v VEC - shift + VEC): vectors are aligned, the first and the last may be cut.
+  struct Row {
+    const T* z;
+    int shift, lo, end, vecs;                                 // vectors [lo, end) are this CTA's
+  };
+  auto row_of = [&](int row) {
+    Row r;
+    r.z = static_cast<const T*>(a.z) + (long long)row * a.ldz;
+    r.shift = EVEN ? 0 : int(reinterpret_cast<uintptr_t>(r.z) & 15) / int(sizeof(T));
+    r.vecs = (a.V + r.shift + VEC - 1) / VEC;
+    const int part = (r.vecs + (1 << clog) - 1) >> clog;
+    r.lo = min(r.vecs, rank * part);
+    r.end = min(r.vecs, r.lo + part);
+    return r;
+  };
+  // (what lies in front of the row in its first 16 bytes belongs to the same tensor's memory; behind its last element nothing is read)
+  auto fetch = [&](int row, int it) {
+    if (row < a.N) {
+      const Row r = row_of(row);
+      uint4* mine = vectors + it % S::kVectors * VPT * nt;
+      const T* from = r.z - r.shift + (r.lo + tid) * VEC;
+      const uint32_t to = smem_u32(mine);
+      const int end = r.end - r.lo - tid, last = r.vecs - 1 - r.lo - tid;
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        if (k * nt < end) {
+          if (EVEN || k * nt != last) copy_async16(to + k * nt * 16, from + k * nt * VEC);
+          else copy_async16_part(to + k * nt * 16, from + k * nt * VEC, (a.V + r.shift - (r.vecs - 1) * VEC) * int(sizeof(T)));
+        } else if (!EVEN) {                                   // (rows may differ by a vector)
+          mine[k * nt] = make_uint4(minus_inf<T>(), minus_inf<T>(), minus_inf<T>(), minus_inf<T>());
+        }
+      }
+      float2* entries = entry_buf + it % S::kEntries * a.K;
+      for (int k = tid; k < a.K; k += nt) copy_async8(smem_u32(entries + k), a.entries + (long long)row * a.K + k);
     }
-    block_max_sum(tm, ts, c, red);
-    const bool empty = tm == -INFINITY && ts == 0.f;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int stride = gridDim.x >> clog, row0 = blockIdx.x >> clog;
+  __syncthreads();
+  for (int i = 0; i < S::kVectors; ++i) fetch(row0 + i * stride, i);
+  if (clog) cluster_sync_all();                               // every CTA is there to be written to
+  int row = row0;
+  for (int it = 0; row - stride < a.N; row += stride, ++it) {
+    if (row < a.N) {
+      // ---- first pass over this row
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      const Row r = row_of(row);
+      const int turn = it % S::kPeers, chain = it % S::kChains;
+      uint4* mine = vectors + it % S::kVectors * VPT * nt;
+      if (a.grad) {
+        const int elo = r.lo * VEC - r.shift, ehi = r.end * VEC - r.shift;
+        const float2* entries = entry_buf + it % S::kEntries * a.K;
+        for (int k = tid; k < a.K; k += nt) {
+          const int i = __float_as_int(entries[k].y);
+          if (i >= max(elo, 0) && i < ehi) {
+            const int v = (i - elo) / VEC;
+            links[chain * a.K + k] = LINK(exchange_small(heads, (chain * nt + v % nt) * 4 + v / nt, uint32_t(k + 1)));
+          }
+        }
+      }
+      if (!EVEN) {                                            // what a cut vector holds of others
+        if (rank == 0 && tid == 0)
+          for (int j = 0; j < r.shift; ++j) reinterpret_cast<T*>(mine)[j] = from_f32<T>(-INFINITY);
+        const int last = r.vecs - 1 - r.lo - tid;
+        if (r.vecs == r.end && last >= 0 && last % nt == 0)
+          for (int j = a.V + r.shift - (r.vecs - 1) * VEC; j < VEC; ++j) reinterpret_cast<T*>(mine + last)[j] = from_f32<T>(-INFINITY);
+      }
+      if (!a.have_stats) {
+        uint4 u[VPT];
+        float m = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+          u[k] = mine[k * nt];
+          m = fmaxf(m, max16<T>(u[k]));
+        }
+        m *= c;
+        const float from = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+          float f[VEC], part = 0.f;
+          unpack16<T>(u[k], f);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) part += ex2(fmaf(f[j], c, from));
+          s += part;
+        }
+        warp_max_sum(m, s);
+        const int at = turn * kDistillCluster * nw + rank * nw + (tid >> 5);
+        if (clog) {
+          if (lane >> clog == 0) send8(smem_u32(peers + at), bar0 + 8 * turn, lane, make_float2(m, s));
+        } else if (lane == 0) {
+          peers[at] = make_float2(m, s);
+        }
+      }
+    }
+    if (it > 0) {
+      // ---- second pass over the row before
+      const int was = it - 1, old = row - stride, turn = was % S::kPeers, chain = was % S::kChains;
+      const Row r = row_of(old);
+      uint4* mine = vectors + was % S::kVectors * VPT * nt;
+      const float2* entries = entry_buf + was % S::kEntries * a.K;
+      mbar_wait(bar0 + 8 * turn, (was / S::kPeers) & 1, &abort_flag, a.status, kStatusTimeoutLocalFlag);
+      const bool empty = __float_as_int(entries[0].y) == -2;
+      float m, s;
+      if (a.have_stats) {
+        const float2 q = a.stats[old];
+        m = q.x;
+        s = q.y;
+      } else {
+        m = -INFINITY;
+        s = 0.f;
+        const float2* all = peers + turn * kDistillCluster * nw;
+        for (int i = lane; i < pairs; i += 32) {
+          const float2 q = all[i];
+          const float nm = fmaxf(m, q.x);
+          s = (m == -INFINITY ? s : s * ex2(m - nm)) + (q.x == -INFINITY ? q.y : q.y * ex2(q.x - nm));
+          m = nm;
+        }
+        warp_max_sum(m, s);
+        if (a.stats && rank == 0 && tid == 0) a.stats[old] = make_float2(m, s);
+      }
+      if (a.grad) {
+        T* g = static_cast<T*>(a.grad) + (long long)old * a.ldg;
+        const float w = a.up_rows ? weight * a.up[old] : weight, scale = w / s;
+        T* to = g - r.shift + (r.lo + tid) * VEC;
+        const int end = r.end - r.lo - tid;
+        const bool cuts = !EVEN && (r.shift != 0 || r.vecs * VEC != a.V);
+        const int head = cuts ? -r.lo - tid : -1, last = cuts ? r.vecs - 1 - r.lo - tid : -1;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+          if (k * nt < end) {
+            float f[VEC];
+            unpack16<T>(mine[k * nt], f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = empty ? 0.f : ex2(fmaf(f[j], c, -m)) * scale;
+            const uint4 u = pack16<T>(f);
+            if (!EVEN && k * nt == head) cut[0] = u;
+            else if (!EVEN && k * nt == last) cut[1] = u;
+            else *reinterpret_cast<uint4*>(to + k * nt * VEC) = u;
+          }
+        }
+        if (cuts) {                                           // cut vectors by their elements
+          if (head == 0 && end > 0)
+            for (int j = r.shift; j < min(VEC, a.V + r.shift); ++j) g[j - r.shift] = reinterpret_cast<const T*>(cut)[j];
+          if (r.vecs > 1 && r.vecs == r.end && last >= 0 && last % nt == 0)
+            for (int j = 0; j < a.V + r.shift - (r.vecs - 1) * VEC; ++j) g[(r.vecs - 1) * VEC - r.shift + j] = reinterpret_cast<const T*>(cut + 1)[j];
+        }
+        // chains of this thread's vectors
+        uint32_t* words = reinterpret_cast<uint32_t*>(heads + (chain * nt + tid) * 4);
+        uint32_t any = words[0];
+        if (sizeof(LINK) == 2) any |= words[1];
+        if (any) {
+          if (!empty) {
+            const LINK* link = links + chain * a.K;
+#pragma unroll 1
+            for (int v = 0; v < VPT; ++v) {
+              uint32_t done = 0;
+#pragma unroll 1
+              for (int e = heads[(chain * nt + tid) * 4 + v]; e; e = link[e - 1]) {
+                const int i = __float_as_int(entries[e - 1].y), j = (i + r.shift) & (VEC - 1);
+                if (done >> j & 1u) continue;
+                done |= 1u << j;
+                float p = ex2(entries[e - 1].x);
+                if (link[e - 1]) p = chained_p(entries, link, e, p);
+                const float z = to_f32(reinterpret_cast<const T*>(mine + v * nt)[j]);
+                g[i] = from_f32<T>((ex2(fmaf(z, c, -m)) / s - p) * w);
+              }
+            }
+          }
+          words[0] = 0u;
+          if (sizeof(LINK) == 2) words[1] = 0u;
+        }
+      }
+      if (a.loss && rank == 0 && tid >> 5 == was % nw) {      // (the warps take the rows' losses in turn)
+        const float ls = log2f(s);
+        float part = 0.f;
+#pragma unroll 4
+        for (int k = lane; k < a.K; k += 32) {
+          const int i = __float_as_int(entries[k].y);
+          const float lp = entries[k].x, z = i >= 0 ? to_f32(r.z[i]) : 0.f, p = ex2(lp);
+          if (i >= 0 && !(p == 0.f)) part += p * (lp - (fmaf(z, c, -m) - ls));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+        if (lane == 0) a.loss[old] = empty ? 0.f : part * 0.6931471805599453f * a.temperature * a.temperature;
+      }
+      fetch(old + S::kVectors * stride, was + S::kVectors);
+    }
+    if (row < a.N) {
+      // this warp's part of the first pass is written, and it is through with the row before
+      __syncwarp();
+      if (lane == 0) {
+        const uint32_t bar = bar0 + 8 * (it % S::kPeers);
+        if (tid == 0 && clog && !a.have_stats) mbar_expect_tx(bar, pairs * 8);
+        else mbar_arrive(bar);
+      }
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (clog) cluster_sync_all();                               // a CTA's shared memory is written until here
+}
+
+// Rows that no cluster holds: a CTA goes over a row twice.
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs a) {
+  constexpr int VEC = kVec<T>;
+  __shared__ float2 red[kLongWarps];
+  __shared__ float fsum[kLongWarps];
+  __shared__ int isum[kLongWarps];
+  pdl_launch_dependents();
+  pdl_wait();
+  if (a.skip_one && a.up && a.up[0] == 1.f) return;
+  float weight = a.temperature;
+  if (a.flags) weight /= float(max(1, count_flags(a.flags, a.N, isum)));
+  if (a.up && !a.up_rows) weight *= a.up[0];
+  const float c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  for (int row = blockIdx.x; row < a.N; row += gridDim.x) {
+    const T* z = static_cast<const T*>(a.z) + (long long)row * a.ldz;
+    T* g = a.grad ? static_cast<T*>(a.grad) + (long long)row * a.ldg : nullptr;
+    const float2* entries = a.entries + (long long)row * a.K;
+    bool there = false;
+    for (int k = tid; k < a.K; k += kLongThreads) there = there || __float_as_int(entries[k].y) >= 0;
+    const bool empty = __syncthreads_or(there) == 0;
     const int head = min(a.V, int((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / int(sizeof(T)));
-    const int vecs = (a.V - head) / VEC, tail = head + vecs * VEC;
+    const int vecs = (a.V - head) / VEC, tail = head + vecs * VEC, rest = head + (a.V - tail);
+    auto edge = [&](int i) { return i < head ? i : tail + i - head; };
     float m = -INFINITY, s = 0.f;
     if (a.have_stats) {
       m = a.stats[row].x;
       s = a.stats[row].y;
-    } else if (!empty) {
-      for (int i = threadIdx.x; i < vecs; i += kDistillThreads) {
+    } else {
+      for (int i = tid; i < vecs; i += kLongThreads) {
         float f[VEC];
         unpack16<T>(*reinterpret_cast<const uint4*>(z + head + i * VEC), f);
-        float vm = f[0];
+        float vm = -INFINITY;
 #pragma unroll
-        for (int j = 1; j < VEC; ++j) vm = fmaxf(vm, f[j]);
-        float vs = 0.f;
+        for (int j = 0; j < VEC; ++j) vm = fmaxf(vm, f[j]);
+        vm = fmaxf(m, vm * c);
+        const float from = vm == -INFINITY ? 0.f : vm;
+        s = m == -INFINITY ? s : s * ex2(m - vm);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) vs += f[j] == -INFINITY ? 0.f : exp2f((f[j] - vm) * c);
-        join_max_sum(m, s, vm, vs, c);
+        for (int j = 0; j < VEC; ++j) s += ex2(fmaf(f[j], c, -from));
+        m = vm;
       }
-      for (int i = threadIdx.x; i < head + (a.V - tail); i += kDistillThreads) {
-        const float f = to_f32(z[i < head ? i : tail + i - head]);
-        if (f != -INFINITY) join_max_sum(m, s, f, 1.f, c);
+      for (int i = tid; i < rest; i += kLongThreads) {
+        const float f = to_f32(z[edge(i)]), vm = fmaxf(m, f * c);
+        s = (m == -INFINITY ? s : s * ex2(m - vm)) + ex2(fmaf(f, c, vm == -INFINITY ? 0.f : -vm));
+        m = vm;
       }
-      block_max_sum(m, s, c, red);
-      if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(m, s);
+      warp_max_sum(m, s);
+      if (lane == 0) red[warp] = make_float2(m, s);
+      __syncthreads();
+      m = lane < kLongWarps ? red[lane].x : -INFINITY;
+      s = lane < kLongWarps ? red[lane].y : 0.f;
+      warp_max_sum(m, s);
+      if (a.stats && tid == 0) a.stats[row] = make_float2(m, s);
     }
-    const float ln2 = 0.6931471805599453f;
     if (a.loss) {
+      const float ls = log2f(s);
       float part = 0.f;
-      if (!empty)
-        for (int k = threadIdx.x; k < a.K; k += kDistillThreads) {
-          if (top_i[k] < 0) continue;
-          const float lp = (top_p[k] - tm) * c - log2f(ts), p = exp2f(lp);
-          const float lq = (to_f32(z[top_i[k]]) - m) * c - log2f(s);
-          if (p > 0.f || p != p) part += p * (lp - lq);
-        }
+      for (int k = tid; k < a.K; k += kLongThreads) {
+        const int i = __float_as_int(entries[k].y);
+        const float lp = entries[k].x, p = ex2(lp);
+        if (i >= 0 && !(p == 0.f)) part += p * (lp - (fmaf(to_f32(z[i]), c, -m) - ls));
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
       if (lane == 0) fsum[warp] = part;
       __syncthreads();
-      if (threadIdx.x == 0) {
+      if (tid == 0) {
         part = 0.f;
-        for (int w = 0; w < kDistillWarps; ++w) part += fsum[w];
-        a.loss[row] = part * ln2 * a.temperature * a.temperature;
+        for (int q = 0; q < kLongWarps; ++q) part += fsum[q];
+        a.loss[row] = empty ? 0.f : part * 0.6931471805599453f * a.temperature * a.temperature;
       }
     }
     if (g) {
-      const float w = a.temperature * mean * (a.up ? a.up[a.up_rows ? row : 0] : 1.f);
-      if (empty) {
-        for (int i = threadIdx.x; i < a.V; i += kDistillThreads) g[i] = from_f32<T>(0.f);
-      } else {
-        const float k = w / s;
-        const bool side = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(z)) & 15) == 0;
-        for (int i = threadIdx.x; i < vecs; i += kDistillThreads) {
-          float f[VEC];
-          unpack16<T>(*reinterpret_cast<const uint4*>(z + head + i * VEC), f);
+      const float w = a.up_rows ? weight * a.up[row] : weight;
+      const float scale = w / s;
+      for (int i = tid; i < vecs; i += kLongThreads) {
+        float f[VEC];
+        unpack16<T>(*reinterpret_cast<const uint4*>(z + head + i * VEC), f);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) f[j] = exp2f((f[j] - m) * c) * k;
-          if (side) *reinterpret_cast<uint4*>(g + head + i * VEC) = pack16<T>(f);
-          else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) g[head + i * VEC + j] = from_f32<T>(f[j]);
+        for (int j = 0; j < VEC; ++j) f[j] = empty ? 0.f : ex2(fmaf(f[j], c, -m)) * scale;
+        *reinterpret_cast<uint4*>(g + head + i * VEC) = pack16<T>(f);
+      }
+      for (int i = tid; i < rest; i += kLongThreads) g[edge(i)] = from_f32<T>(empty ? 0.f : ex2(fmaf(to_f32(z[edge(i)]), c, -m)) * scale);
+      __syncthreads();
+      for (int k = tid; k < a.K; k += kLongThreads) {
+        const int i = __float_as_int(entries[k].y);
+        if (i < 0) continue;
+        float p = 0.f;
+        bool first = true;
+        for (int o = 0; o < a.K; ++o)
+          if (__float_as_int(entries[o].y) == i) {
+            first = first && o >= k;
+            p += ex2(entries[o].x);
           }
-        }
-        for (int i = threadIdx.x; i < head + (a.V - tail); i += kDistillThreads) {
-          const int at = i < head ? i : tail + i - head;
-          g[at] = from_f32<T>(exp2f((to_f32(z[at]) - m) * c) * k);
-        }
-        __syncthreads();
-        // the teacher's classes again, from the 32-bit values; a class that comes several times is written by its first entry
-        for (int e = threadIdx.x; e < a.K; e += kDistillThreads) {
-          const int at = top_i[e];
-          if (at < 0) continue;
-          float p = 0.f;
-          bool first = true;
-          for (int o = 0; o < a.K; ++o)
-            if (top_i[o] == at) {
-              if (o < e) first = false;
-              p += exp2f((top_p[o] - tm) * c - log2f(ts));
-            }
-          if (first) g[at] = from_f32<T>((exp2f((to_f32(z[at]) - m) * c) / s - p) * w);
-        }
+        if (first) g[i] = from_f32<T>((ex2(fmaf(to_f32(z[i]), c, -m)) / s - p) * w);
       }
     }
     __syncthreads();
@@ -229,16 +546,75 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* rows,
   }
 }
 
-template <typename T>
-int distill(DistillArgs a, unsigned char* flags, int fill_flags, float* out, cudaStream_t st) {
-  if (flags && fill_flags) {
-    const int grid = int(std::min<long long>((a.N + 7) / 8, 8ll * sm_count()));
-    LT_RETURN_IF_CUDA(launch_chained(distill_flags_kernel, grid, 256, 0, st, a.t, a.t_type, a.idx, a.N, a.V, a.K, flags));
+// How many clusters of 2^cluster_log CTAs of nt threads the GPU holds at once.
+template <typename T, bool EVEN, typename LINK, int VPT>
+cudaError_t cluster_places(int cluster_log, int nt, int* places) {
+  auto kernel = distill_kernel<T, EVEN, LINK, VPT>;
+  typedef DistillSmem<LINK, VPT> S;
+  static std::atomic<int> known[64][4][6];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  int size = 0;
+  while (32 << size < nt) ++size;
+  *places = dev < 64 ? known[dev][cluster_log][size].load(std::memory_order_acquire) : 0;
+  if (*places > 0) return cudaSuccess;
+  if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(kDistillThreads, S::kTop))) != cudaSuccess) return e;
+  const int smem = S::bytes(nt, std::min(S::kTop, 64));       // (more entries than that: some clusters may follow the others)
+  if (cluster_log == 0) {
+    int per_sm = 0;
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, nt, smem)) != cudaSuccess) return e;
+    *places = per_sm * sm_count();
+  } else {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1 << cluster_log;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = 1 << cluster_log;
+    cfg.blockDim = nt;
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if ((e = cudaOccupancyMaxActiveClusters(places, kernel, &cfg)) != cudaSuccess) return e;
   }
-  a.flags = flags;
-  const int grid = std::min(a.N, 4 * sm_count());
-  LT_RETURN_IF_CUDA(launch_chained(distill_kernel<T>, grid, kDistillThreads, 0, st, a));
-  if (out) LT_RETURN_IF_CUDA(launch_chained(distill_reduce_kernel, 1, 1024, 0, st, static_cast<const float*>(a.loss), static_cast<const unsigned char*>(flags), a.N, out));
+  if (*places < 1) return cudaErrorInvalidConfiguration;
+  if (dev < 64) known[dev][cluster_log][size].store(*places, std::memory_order_release);
+  return cudaSuccess;
+}
+
+template <typename T, bool EVEN, typename LINK, int VPT>
+int distill_clusters(const DistillArgs& a, int nt, cudaStream_t st) {
+  int places = 0;
+  LT_RETURN_IF_CUDA((cluster_places<T, EVEN, LINK, VPT>(a.cluster_log, nt, &places)));
+  const int ctas = 1 << a.cluster_log, clusters = std::min(a.N, places), smem = DistillSmem<LINK, VPT>::bytes(nt, a.K);
+  auto kernel = distill_kernel<T, EVEN, LINK, VPT>;
+  if (ctas > 1) LT_RETURN_IF_CUDA(launch_chained_clusters(kernel, clusters * ctas, nt, smem, ctas, st, a));
+  else LT_RETURN_IF_CUDA(launch_chained(kernel, clusters, nt, smem, st, a));
+  return 0;
+}
+
+template <typename T>
+int distill(DistillArgs a, float* out, cudaStream_t st) {
+  const bool even = a.V % kVec<T> == 0 && (a.N == 1 || a.ldz % kVec<T> == 0) && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0;
+  const int vecs = even ? a.V / kVec<T> : a.V / kVec<T> + 2;  // (a row may begin and end inside a vector)
+  const bool few = a.K <= DistillSmem<uint8_t, 4>::kTop;
+  const int per = few ? 4 : 3;
+  a.cluster_log = 0;
+  while ((1 << a.cluster_log) < kDistillCluster && vecs > (per * kDistillThreads) << a.cluster_log) ++a.cluster_log;
+  if (vecs <= (per * kDistillThreads) << a.cluster_log) {
+    // few rows: more CTAs for each
+    while ((1 << a.cluster_log) < kDistillCluster && (long long)a.N << (a.cluster_log + 1) <= sm_count() && vecs >> a.cluster_log >= 512) ++a.cluster_log;
+    int nt = 32;
+    while (nt < kDistillThreads && vecs > (per * nt) << a.cluster_log) nt *= 2;
+    int rc;
+    if (few) rc = even ? distill_clusters<T, true, uint8_t, 4>(a, nt, st) : distill_clusters<T, false, uint8_t, 4>(a, nt, st);
+    else rc = even ? distill_clusters<T, true, uint16_t, 3>(a, nt, st) : distill_clusters<T, false, uint16_t, 3>(a, nt, st);
+    if (rc) return rc;
+  } else {
+    LT_RETURN_IF_CUDA(launch_chained(distill_long_kernel<T>, std::min(a.N, 4 * sm_count()), kLongThreads, 0, st, a));
+  }
+  if (out) LT_RETURN_IF_CUDA(launch_chained(distill_reduce_kernel, 1, 1024, 0, st, static_cast<const float*>(a.loss), a.flags, a.N, out));
   return 0;
 }
 
@@ -247,19 +623,30 @@ int distill(DistillArgs a, unsigned char* flags, int fill_flags, float* out, cud
 extern "C" {
 
 // Distillation of student logits z [N, V] (pitch ldz; fp32, bf16 or fp16: type 0, 1, 2) from teacher logits t [N, K] (type t_type) at classes idx [N, K].
-//   flags [N] bytes: the loss is a mean over the rows that have a teacher (fill_flags: find them first); null: no mean
+//   entries [N, K, 2] floats: written from t and idx; read if t is null
+//   flags [N] bytes: the loss is a mean over the rows that have a teacher (written or read likewise); null: no mean
 //   loss [N] or null; out: their sum or mean, or null; stats [N, 2]: written, or read (have_stats: z is not searched for its maximum again)
-//   grad [N, V] or null: times up, which is null (1), one number, or (up_rows) one for every row; skip_one: nothing is done where up is one number and it is 1
-int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t, const long long* idx, int N, int V, int K, float temperature, unsigned char* flags, int fill_flags,
-               const float* up, int up_rows, int skip_one, float* stats, int have_stats, float* loss, float* out, void* grad, void* stream) {
+//   grad [N, V] (pitch ldg; every row as far behind a multiple of 16 bytes as z's) or null: times up, which is null (1), one number, or (up_rows) one for every row; skip_one: nothing is done where up is one number and it is 1
+int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t, const long long* idx, float* entries, int N, int V, int K, float temperature,
+               unsigned char* flags, const float* up, int up_rows, int skip_one, float* stats, int have_stats, float* loss, float* out, void* grad, long long ldg,
+               void* stream) {
   using namespace lt;
-  if (type < 0 || type > 2 || t_type < 0 || t_type > 2 || N < 0 || V < 1 || K < 1 || K > kDistillTop || !(temperature > 0.f) || (out && !loss)) return -int(kStatusBadArgument);
+  if (type < 0 || type > 2 || t_type < 0 || t_type > 2 || N < 0 || V < 1 || K < 1 || K > kDistillTop || !(temperature > 0.f) || (out && !loss) ||
+      (reinterpret_cast<uintptr_t>(entries) & 7) != 0)
+    return -int(kStatusBadArgument);
   if (N == 0) return 0;
-  DistillArgs a{z, ldz, t, t_type, idx, N, V, K, temperature, nullptr, up, up_rows, skip_one, reinterpret_cast<float2*>(stats), have_stats, loss, grad};
+  const int bytes = type == kElemF32 ? 4 : 2;
+  if (grad && (((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(z)) & 15) != 0 || (N > 1 && (ldg - ldz) * bytes % 16 != 0))) return -int(kStatusBadArgument);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (type == kElemF32) return distill<float>(a, flags, fill_flags, out, st);
-  if (type == kElemBf16) return distill<__nv_bfloat16>(a, flags, fill_flags, out, st);
-  return distill<__half>(a, flags, fill_flags, out, st);
+  float2* pairs = reinterpret_cast<float2*>(entries);
+  if (t) {
+    const int grid = int(std::min<long long>((N + 7) / 8, 8ll * sm_count()));
+    LT_RETURN_IF_CUDA(launch_chained(distill_teacher_kernel, grid, 256, 0, st, t, t_type, idx, N, V, K, kLog2e / temperature, pairs, flags));
+  }
+  DistillArgs a{z, ldz, pairs, N, V, K, temperature, kLog2e / temperature, flags, up, up_rows, skip_one, reinterpret_cast<float2*>(stats), have_stats, loss, grad, ldg, 0, device_status_word()};
+  if (type == kElemF32) return distill<float>(a, out, st);
+  if (type == kElemBf16) return distill<__nv_bfloat16>(a, out, st);
+  return distill<__half>(a, out, st);
 }
 
 }  // extern "C"

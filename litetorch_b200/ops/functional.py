@@ -551,22 +551,20 @@ class _Distillation(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, z, t, idx, temperature, reduction):
-        rows = K.DistillRows(z, t, idx, temperature, reduction == "mean")
         ahead = ctx.needs_input_grad[0] and reduction != "none" and not torch.cuda.is_current_stream_capturing()
-        loss, ctx.grad, kept = rows.loss(reduction != "none", ahead)
-        ctx.save_for_backward(z, rows.t, rows.idx, *kept)
-        ctx.temperature, ctx.mean = temperature, reduction == "mean"
+        loss, ctx.ahead, room = K.distill_loss(z, t, idx, temperature, reduction, ahead)
+        ctx.save_for_backward(z, room)
+        ctx.rest = t.shape[1], temperature, reduction == "mean"
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
-        z, t, idx, *kept = ctx.saved_tensors
-        ahead, ctx.grad = ctx.grad, None                       # handed out once
+        z, room = ctx.saved_tensors
+        ahead, ctx.ahead = ctx.ahead, None                     # handed out once
         if ahead is not None and torch.cuda.is_current_stream_capturing():
             ahead = None
-        rows = K.DistillRows(z, t, idx, ctx.temperature, ctx.mean)
-        return rows.grad(kept, up.contiguous(), ahead), None, None, None, None
+        return K.distill_grad(z, room, *ctx.rest, up.contiguous(), ahead), None, None, None, None
 
 
 def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_idx: torch.Tensor, temperature: float = 1.0,

@@ -20,7 +20,7 @@ _vp, _i, _ll, _f, _d = c_void_p, c_int, c_longlong, c_float, ctypes.c_double
 _SIGS = {
     "lt_token_embedding_fwd": [_i, _vp, _i, _vp, _vp, _ll, _i, _i, _f, _vp],
     "lt_token_embedding_bwd": [_i, _vp, _i, _vp, _ll, _vp, _ll, _i, _i, _f, _ll, _vp, _vp, _i, _vp],
-    "lt_distill": [_i, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _f, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _vp],
+    "lt_distill": [_i, _vp, _ll, _i, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _ll, _vp],
     "lt_sample_tokens": [_i, _vp, _ll, _vp, _i] + [_vp] * 4 + [_d, _i, _d, _d, _i, _i, _vp, _vp, _vp],
     "lt_residual_norm": [_i, _vp, _vp, _vp, _vp, _ll, _vp, _vp, _vp, _i, _vp, _f, _vp, _f, _vp, _vp, _i, _i, _i, _vp],
     "lt_latent_rope": [_i, _vp, _ll] + [_i] * 8 + [_vp, _f, _vp, _vp, _vp, _f, _vp, _i, _i, _vp, _vp, _vp],
@@ -1663,45 +1663,53 @@ def token_embedding_grad(idx: torch.Tensor, dout: torch.Tensor, vocab: int, scal
     return grad
 
 
-class DistillRows:
-    """Rows of student logits z [N, V] (rows may be strided) against a teacher's top logits t [N, K] at classes idx [N, K] (`functional.distillation_loss` has
-    the formulas).  `loss` may form the gradient for an upstream gradient of 1 on the way; `grad` forms it from the kept statistics."""
+def _like_rows(z):
+    """A tensor like z [N, V] whose rows lie as far behind multiples of 16 bytes as those of z."""
+    (N, V), ld, each = z.shape, z.stride(0), 16 // z.element_size()
+    shift = z.data_ptr() % 16 // z.element_size()
+    if shift == 0 and (ld == V or N <= 1):
+        return torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    if ld < V:                                              # one row for several
+        ld = V + (ld - V) % each
+    return torch.empty(shift + N * ld, dtype=z.dtype, device=z.device).as_strided((N, V), (ld, 1), shift)
 
-    def __init__(self, z, t, idx, temperature: float, mean: bool):
-        assert z.dim() == 2 and t.shape == idx.shape and t.dim() == 2 and t.shape[0] == z.shape[0] and z.dtype in _ELEM and t.dtype in _ELEM
-        assert z.device == t.device == idx.device and 1 <= t.shape[1] <= 1024 and temperature > 0 and z.shape[0] < 1 << 31
-        self.z = z if z.stride(1) == 1 else z.contiguous()
-        self.t, self.idx = t.contiguous(), idx.to(torch.int64).contiguous()
-        self.temperature, self.mean = float(temperature), mean
 
-    def _run(self, flags, fill, up, skip_one, stats, have, loss, out, grad):
-        z = self.z
-        with _on(z):
-            _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), _ELEM[self.t.dtype], self.t.data_ptr(), self.idx.data_ptr(), z.shape[0], z.shape[1],
-                                     self.t.shape[1], self.temperature, _p(flags), fill, _p(up), 1 if up is not None and up.dim() else 0, skip_one, _p(stats), have,
-                                     _p(loss), _p(out), _p(grad), _stream()), "lt_distill")
-        _launches[0] += (fill and flags is not None) + (out is not None)
+def distill_loss(z, t, idx, temperature: float, reduction: str, with_grad: bool):
+    """(loss, gradient for an upstream gradient of 1 or None, what `distill_grad` needs) of student logits z [N, V] (rows may be strided) against a teacher's top
+    logits t [N, K] at classes idx [N, K] (`functional.distillation_loss` has the formulas)."""
+    (N, V), top = z.shape, t.shape[1]
+    assert t.shape == idx.shape == (N, top) and z.dtype in _ELEM and t.dtype in _ELEM and z.device == t.device == idx.device and 1 <= top <= 1024
+    z = z if z.stride(1) == 1 else z.contiguous()
+    t, idx = t.contiguous(), idx.to(torch.int64).contiguous()
+    mean = reduction == "mean"
+    # [N, K, 2] entries, [N, 2] maxima and sums, [N] losses, [N] bytes
+    room = z.new_empty(N * (2 * top + 3) + (N + 3) // 4, dtype=torch.float32)
+    at = room.data_ptr()
+    stats, loss, flags = at + 8 * N * top, at + 8 * N * (top + 1), at + 4 * N * (2 * top + 3)
+    out = None if reduction == "none" else z.new_empty((), dtype=torch.float32)
+    grad = _like_rows(z) if with_grad else None
+    with _on(z):
+        _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), _ELEM[t.dtype], t.data_ptr(), idx.data_ptr(), at, N, V, top, temperature,
+                                 flags if mean else None, None, 0, 0, stats, 0, loss, _p(out), _p(grad), 0 if grad is None else grad.stride(0), _stream()), "lt_distill")
+    _launches[0] += 1 if out is None else 2
+    return room[2 * N * (top + 1):][:N] if out is None else out, grad, room
 
-    def loss(self, reduce: bool, with_grad: bool):
-        """(loss: the mean or sum, or [N] without `reduce`; gradient or None; what `grad` needs)."""
-        N, dev = self.z.shape[0], self.z.device
-        rows = torch.empty(N, dtype=torch.float32, device=dev)
-        stats = torch.empty((N, 2), dtype=torch.float32, device=dev)
-        flags = torch.empty(N, dtype=torch.uint8, device=dev) if self.mean else None
-        out = torch.empty((), dtype=torch.float32, device=dev) if reduce else None
-        grad = torch.empty(self.z.shape, dtype=self.z.dtype, device=dev) if with_grad else None
-        self._run(flags, 1, None, 0, stats, 0, rows, out, grad)
-        return (out if reduce else rows), grad, (stats, flags)
 
-    def grad(self, kept, up, grad=None):
-        """The gradient for the upstream gradient `up` (one number on the device, or one a row).  With `grad`, which holds it for 1: nothing is done where `up` is 1."""
-        stats, flags = kept
-        assert up.dtype == torch.float32 and up.is_contiguous()
-        there = grad is not None
-        if not there:
-            grad = torch.empty(self.z.shape, dtype=self.z.dtype, device=self.z.device)
-        self._run(flags, 0, up, 1 if there else 0, stats, 1, None, None, grad)
-        return grad
+def distill_grad(z, room, top: int, temperature: float, mean: bool, up, grad=None):
+    """The gradient of `distill_loss` for the upstream gradient `up` (one number on the device, or one a row).  With `grad`, which holds it for 1: nothing is
+    done where `up` is 1."""
+    N, V = z.shape
+    z = z if z.stride(1) == 1 else z.contiguous()
+    assert up.dtype == torch.float32 and up.is_contiguous() and up.shape in ((), (N,))
+    there = grad is not None
+    if not there:
+        grad = _like_rows(z)
+    at = room.data_ptr()
+    with _on(z):
+        _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), 0, None, None, at, N, V, top, temperature, at + 4 * N * (2 * top + 3) if mean else None,
+                                 up.data_ptr(), up.dim(), 1 if there else 0, at + 8 * N * top, 1, None, None, grad.data_ptr(), grad.stride(0),
+                                 _stream()), "lt_distill")
+    return grad
 
 
 def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
