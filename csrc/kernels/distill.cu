@@ -16,7 +16,7 @@
 
 namespace lt {
 
-constexpr int kDistillThreads = 1024, kDistillWarps = kDistillThreads / 32, kDistillTop = 1024, kDistillCluster = 8;
+constexpr int kDistillThreads = 512, kDistillWarps = kDistillThreads / 32, kDistillTop = 1024, kDistillCluster = 8;
 constexpr int kLongThreads = 512, kLongWarps = kLongThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -35,7 +35,7 @@ struct DistillArgs {
   float* loss;                   // [N] or null
   void* grad;                    // [N, V] (pitch ldg, rows where those of z lie within 16 bytes) or null
   long long ldg;
-  int cluster_log;               // log2 of the CTAs of a cluster
+  int cluster_log, vpt;          // log2 of the CTAs of a cluster, vectors of a thread
   int* status;
 };
 
@@ -126,6 +126,14 @@ __device__ __forceinline__ uint32_t exchange_small(LINK* p, int i, uint32_t v) {
     old = seen;
   }
 }
+// The chains of a thread's eight vectors at once.
+template <typename LINK> struct Heads;
+template <> struct Heads<uint8_t> { typedef uint2 type; };
+template <> struct Heads<uint16_t> { typedef uint4 type; };
+__device__ __forceinline__ bool any(const uint2& h) { return (h.x | h.y) != 0u; }
+__device__ __forceinline__ bool any(const uint4& h) { return (h.x | h.y | h.z | h.w) != 0u; }
+__device__ __forceinline__ void clear(uint2& h) { h = make_uint2(0u, 0u); }
+__device__ __forceinline__ void clear(uint4& h) { h = make_uint4(0u, 0u, 0u, 0u); }
 // The teacher's probability of entry e's class (p by that entry alone) with those of the entries chained behind it that have the same.  Their sum is taken in
 // whole numbers of 2^-62: it must not depend on the chain's order.
 template <typename LINK>
@@ -170,16 +178,17 @@ __device__ __forceinline__ void send8(uint32_t dst, uint32_t bar, uint32_t cta, 
       : "memory");
 }
 
-// Shared memory of a CTA of so many threads, a multiple of 32.
-template <typename LINK, int VPT>
+// Shared memory of a CTA of so many threads, 32 times a power of two.
+template <typename LINK>
 struct DistillSmem {
   static constexpr int kTop = sizeof(LINK) == 1 ? 255 : kDistillTop;      // entries that a LINK numbers
   static constexpr int kVectors = 3, kEntries = 4, kChains = 3, kPeers = 4;           // rows in turn
-  static __host__ __device__ int entries(int nt) { return kVectors * VPT * nt * 16; }
-  static __host__ __device__ int peers(int nt, int K) { return entries(nt) + kEntries * K * 8; }
-  static __host__ __device__ int heads(int nt, int K) { return peers(nt, K) + kPeers * kDistillCluster * (nt / 32) * 8; }
-  static __host__ __device__ int links(int nt, int K) { return heads(nt, K) + kChains * nt * 4 * int(sizeof(LINK)); }
-  static __host__ __device__ int bytes(int nt, int K) { return links(nt, K) + kChains * K * int(sizeof(LINK)); }
+  // vpt: vectors of a thread
+  static __host__ __device__ int entries(int nt, int vpt) { return kVectors * vpt * nt * 16; }
+  static __host__ __device__ int peers(int nt, int vpt, int K) { return entries(nt, vpt) + kEntries * K * 8; }
+  static __host__ __device__ int heads(int nt, int vpt, int K) { return peers(nt, vpt, K) + kPeers * kDistillCluster * (nt / 32) * 8; }
+  static __host__ __device__ int links(int nt, int vpt, int K) { return heads(nt, vpt, K) + kChains * nt * 8 * int(sizeof(LINK)); }
+  static __host__ __device__ int bytes(int nt, int vpt, int K) { return links(nt, vpt, K) + kChains * K * int(sizeof(LINK)); }
 };
 
 // A cluster of CTAs holds a row, every thread up to VPT vectors of 16 bytes: a row is read from global memory once.  The threads go over their vectors twice, first
@@ -191,7 +200,7 @@ struct DistillSmem {
 template <typename T, bool EVEN, typename LINK, int VPT>
 __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a) {
   constexpr int VEC = kVec<T>;
-  typedef DistillSmem<LINK, VPT> S;
+  typedef DistillSmem<LINK> S;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[S::kPeers];
   __shared__ uint4 cut[2];                                    // the row's first and last vector, if they are cut
@@ -206,11 +215,13 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
   const float c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, nt = blockDim.x, nw = nt >> 5;
   const int clog = a.cluster_log, rank = clog ? int(cluster_ctarank()) : 0;
-  uint4* vectors = reinterpret_cast<uint4*>(smem) + tid;      // [3][VPT][nt], from this thread's
-  float2* entry_buf = reinterpret_cast<float2*>(smem + S::entries(nt));   // [4][K]
-  float2* peers = reinterpret_cast<float2*>(smem + S::peers(nt, a.K));    // [4][CTAs][warps]: (reference, sum)
-  LINK* heads = reinterpret_cast<LINK*>(smem + S::heads(nt, a.K));        // [3][nt][4]: number of a vector's first entry + 1
-  LINK* links = reinterpret_cast<LINK*>(smem + S::links(nt, a.K));        // [3][K]: that of an entry's next
+  const int vpt = a.vpt, room = vpt * nt;
+  const int first = (tid >> 5) * vpt * 32 + lane;             // this thread's vectors: first, first + 32, ... of the CTA's
+  uint4* vectors = reinterpret_cast<uint4*>(smem) + first;    // [3][vpt nt]
+  float2* entry_buf = reinterpret_cast<float2*>(smem + S::entries(nt, vpt));   // [4][K]
+  float2* peers = reinterpret_cast<float2*>(smem + S::peers(nt, vpt, a.K));    // [4][CTAs][warps]: (reference, sum)
+  LINK* heads = reinterpret_cast<LINK*>(smem + S::heads(nt, vpt, a.K));        // [3][nt][8]: number of a vector's first entry + 1
+  LINK* links = reinterpret_cast<LINK*>(smem + S::links(nt, vpt, a.K));        // [3][K]: that of an entry's next
   const int pairs = nw << clog;
   const uint32_t bar0 = smem_u32(bars);
   if (tid == 0) {
@@ -218,75 +229,84 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
     for (int i = 0; i < S::kPeers; ++i) mbar_init(bar0 + 8 * i, nw);
     fence_barrier_init();
   }
-  for (int i = tid; i < S::kChains * nt * int(sizeof(LINK)); i += nt) reinterpret_cast<uint32_t*>(heads)[i] = 0u;
+  for (int i = tid; i < S::kChains * nt * 2 * int(sizeof(LINK)); i += nt) reinterpret_cast<uint32_t*>(heads)[i] = 0u;
+  const uint4 none = make_uint4(minus_inf<T>(), minus_inf<T>(), minus_inf<T>(), minus_inf<T>());
 #pragma unroll
-  for (int k = 0; k < S::kVectors * VPT; ++k) vectors[k * nt] = make_uint4(minus_inf<T>(), minus_inf<T>(), minus_inf<T>(), minus_inf<T>());
+  for (int i = 0; i < S::kVectors; ++i)
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+      if (k < vpt) vectors[i * room + k * 32] = none;
 
   // Vector v of a row holds its elements [v VEC - shift, v VEC - shift + VEC): vectors are aligned, the first and the last may be cut.
   struct Row {
-    const T* z;
     int shift, lo, end, vecs;                                 // vectors [lo, end) are this CTA's
   };
-  auto row_of = [&](int row) {
+  auto row_of = [&](const T* z) {
     Row r;
-    r.z = static_cast<const T*>(a.z) + (long long)row * a.ldz;
-    r.shift = EVEN ? 0 : int(reinterpret_cast<uintptr_t>(r.z) & 15) / int(sizeof(T));
+    r.shift = EVEN ? 0 : int(reinterpret_cast<uintptr_t>(z) & 15) / int(sizeof(T));
     r.vecs = (a.V + r.shift + VEC - 1) / VEC;
     const int part = (r.vecs + (1 << clog) - 1) >> clog;
     r.lo = min(r.vecs, rank * part);
     r.end = min(r.vecs, r.lo + part);
     return r;
   };
+  const int stride = gridDim.x >> clog;
+  int row = blockIdx.x >> clog;
+  const long long step = (long long)stride * a.ldz;
+  const T* z = static_cast<const T*>(a.z) + (long long)row * a.ldz;      // the row of the first pass
+  int to_fetch = row;
+  const T* z_fetch = z;
   // (what lies in front of the row in its first 16 bytes belongs to the same tensor's memory; behind its last element nothing is read)
-  auto fetch = [&](int row, int it) {
-    if (row < a.N) {
-      const Row r = row_of(row);
-      uint4* mine = vectors + it % S::kVectors * VPT * nt;
-      const T* from = r.z - r.shift + (r.lo + tid) * VEC;
+  auto fetch = [&](int buf, int entry_turn) {
+    if (to_fetch < a.N) {
+      const Row r = row_of(z_fetch);
+      uint4* mine = vectors + buf * room;
+      const T* from = z_fetch - r.shift + (r.lo + first) * VEC;
       const uint32_t to = smem_u32(mine);
-      const int end = r.end - r.lo - tid, last = r.vecs - 1 - r.lo - tid;
+      const int end = r.end - r.lo - first, last = r.vecs - 1 - r.lo - first;
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
-        if (k * nt < end) {
-          if (EVEN || k * nt != last) copy_async16(to + k * nt * 16, from + k * nt * VEC);
-          else copy_async16_part(to + k * nt * 16, from + k * nt * VEC, (a.V + r.shift - (r.vecs - 1) * VEC) * int(sizeof(T)));
+        if (k >= vpt) break;
+        if (k * 32 < end) {
+          if (EVEN || k * 32 != last) copy_async16(to + k * 512, from + k * 32 * VEC);
+          else copy_async16_part(to + k * 512, from + k * 32 * VEC, (a.V + r.shift - (r.vecs - 1) * VEC) * int(sizeof(T)));
         } else if (!EVEN) {                                   // (rows may differ by a vector)
-          mine[k * nt] = make_uint4(minus_inf<T>(), minus_inf<T>(), minus_inf<T>(), minus_inf<T>());
+          mine[k * 32] = none;
         }
       }
-      float2* entries = entry_buf + it % S::kEntries * a.K;
-      for (int k = tid; k < a.K; k += nt) copy_async8(smem_u32(entries + k), a.entries + (long long)row * a.K + k);
+      for (int k = tid; k < a.K; k += nt) copy_async8(smem_u32(entry_buf + entry_turn * a.K + k), a.entries + (long long)to_fetch * a.K + k);
     }
+    to_fetch += stride;
+    z_fetch += step;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  const int stride = gridDim.x >> clog, row0 = blockIdx.x >> clog;
   __syncthreads();
-  for (int i = 0; i < S::kVectors; ++i) fetch(row0 + i * stride, i);
+  for (int i = 0; i < S::kVectors; ++i) fetch(i, i);
   if (clog) cluster_sync_all();                               // every CTA is there to be written to
-  int row = row0;
-  for (int it = 0; row - stride < a.N; row += stride, ++it) {
+  int cur = 0, prev = 2;                                      // the first pass's place among three, and the second's
+  for (int it = 0; row - stride < a.N; row += stride, z += step, ++it) {
     if (row < a.N) {
       // ---- first pass over this row
       asm volatile("cp.async.wait_group 1;" ::: "memory");
-      const Row r = row_of(row);
-      const int turn = it % S::kPeers, chain = it % S::kChains;
-      uint4* mine = vectors + it % S::kVectors * VPT * nt;
+      const Row r = row_of(z);
+      const int turn = it % S::kPeers;
+      uint4* mine = vectors + cur * room;
       if (a.grad) {
         const int elo = r.lo * VEC - r.shift, ehi = r.end * VEC - r.shift;
         const float2* entries = entry_buf + it % S::kEntries * a.K;
         for (int k = tid; k < a.K; k += nt) {
           const int i = __float_as_int(entries[k].y);
           if (i >= max(elo, 0) && i < ehi) {
-            const int v = (i - elo) / VEC;
-            links[chain * a.K + k] = LINK(exchange_small(heads, (chain * nt + v % nt) * 4 + v / nt, uint32_t(k + 1)));
+            const int v = (i - elo) / VEC, w = v / (32 * vpt), owner = w * 32 + v % 32;
+            links[cur * a.K + k] = LINK(exchange_small(heads, (cur * nt + owner) * 8 + (v / 32 - w * vpt), uint32_t(k + 1)));
           }
         }
       }
       if (!EVEN) {                                            // what a cut vector holds of others
         if (rank == 0 && tid == 0)
           for (int j = 0; j < r.shift; ++j) reinterpret_cast<T*>(mine)[j] = from_f32<T>(-INFINITY);
-        const int last = r.vecs - 1 - r.lo - tid;
-        if (r.vecs == r.end && last >= 0 && last % nt == 0)
+        const int last = r.vecs - 1 - r.lo - first;
+        if (r.vecs == r.end && last >= 0 && last < 32 * vpt && last % 32 == 0)
           for (int j = a.V + r.shift - (r.vecs - 1) * VEC; j < VEC; ++j) reinterpret_cast<T*>(mine + last)[j] = from_f32<T>(-INFINITY);
       }
       if (!a.have_stats) {
@@ -294,7 +314,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
         float m = -INFINITY, s = 0.f;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-          u[k] = mine[k * nt];
+          u[k] = k < vpt ? mine[k * 32] : none;
           m = fmaxf(m, max16<T>(u[k]));
         }
         m *= c;
@@ -308,7 +328,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
           s += part;
         }
         warp_max_sum(m, s);
-        const int at = turn * kDistillCluster * nw + rank * nw + (tid >> 5);
+        const int at = (turn * kDistillCluster + rank) * nw + (tid >> 5);
         if (clog) {
           if (lane >> clog == 0) send8(smem_u32(peers + at), bar0 + 8 * turn, lane, make_float2(m, s));
         } else if (lane == 0) {
@@ -318,9 +338,10 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
     }
     if (it > 0) {
       // ---- second pass over the row before
-      const int was = it - 1, old = row - stride, turn = was % S::kPeers, chain = was % S::kChains;
-      const Row r = row_of(old);
-      uint4* mine = vectors + was % S::kVectors * VPT * nt;
+      const int was = it - 1, old = row - stride, turn = was % S::kPeers;
+      const T* z_old = z - step;
+      const Row r = row_of(z_old);
+      uint4* mine = vectors + prev * room;
       const float2* entries = entry_buf + was % S::kEntries * a.K;
       mbar_wait(bar0 + 8 * turn, (was / S::kPeers) & 1, &abort_flag, a.status, kStatusTimeoutLocalFlag);
       const bool empty = __float_as_int(entries[0].y) == -2;
@@ -333,81 +354,89 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
         m = -INFINITY;
         s = 0.f;
         const float2* all = peers + turn * kDistillCluster * nw;
+        for (int i = lane; i < pairs; i += 32) m = fmaxf(m, all[i].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         for (int i = lane; i < pairs; i += 32) {
           const float2 q = all[i];
-          const float nm = fmaxf(m, q.x);
-          s = (m == -INFINITY ? s : s * ex2(m - nm)) + (q.x == -INFINITY ? q.y : q.y * ex2(q.x - nm));
-          m = nm;
+          s += q.x == -INFINITY ? q.y : q.y * ex2(q.x - m);
         }
-        warp_max_sum(m, s);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (a.stats && rank == 0 && tid == 0) a.stats[old] = make_float2(m, s);
       }
       if (a.grad) {
         T* g = static_cast<T*>(a.grad) + (long long)old * a.ldg;
-        const float w = a.up_rows ? weight * a.up[old] : weight, scale = w / s;
-        T* to = g - r.shift + (r.lo + tid) * VEC;
-        const int end = r.end - r.lo - tid;
+        const float w = a.up_rows ? weight * a.up[old] : weight, scale = __fdividef(w, s);
+        T* to = g - r.shift + (r.lo + first) * VEC;
+        const int end = r.end - r.lo - first;
         const bool cuts = !EVEN && (r.shift != 0 || r.vecs * VEC != a.V);
-        const int head = cuts ? -r.lo - tid : -1, last = cuts ? r.vecs - 1 - r.lo - tid : -1;
+        const int head = cuts ? -r.lo - first : -1, last = cuts ? r.vecs - 1 - r.lo - first : -1;
+        auto store = [&](int k, uint4 u) {
+          if (!EVEN && k * 32 == head) cut[0] = u;
+          else if (!EVEN && k * 32 == last) cut[1] = u;
+          else *reinterpret_cast<uint4*>(to + k * 32 * VEC) = u;
+        };
+        if (!empty) {
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-          if (k * nt < end) {
-            float f[VEC];
-            unpack16<T>(mine[k * nt], f);
+          for (int k = 0; k < VPT; ++k) {
+            if (k < vpt && k * 32 < end) {
+              float f[VEC];
+              unpack16<T>(mine[k * 32], f);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) f[j] = empty ? 0.f : ex2(fmaf(f[j], c, -m)) * scale;
-            const uint4 u = pack16<T>(f);
-            if (!EVEN && k * nt == head) cut[0] = u;
-            else if (!EVEN && k * nt == last) cut[1] = u;
-            else *reinterpret_cast<uint4*>(to + k * nt * VEC) = u;
+              for (int j = 0; j < VEC; ++j) f[j] = ex2(fmaf(f[j], c, -m)) * scale;
+              store(k, pack16<T>(f));
+            }
           }
+        } else {
+#pragma unroll
+          for (int k = 0; k < VPT; ++k)
+            if (k < vpt && k * 32 < end) store(k, make_uint4(0u, 0u, 0u, 0u));
         }
         if (cuts) {                                           // cut vectors by their elements
           if (head == 0 && end > 0)
             for (int j = r.shift; j < min(VEC, a.V + r.shift); ++j) g[j - r.shift] = reinterpret_cast<const T*>(cut)[j];
-          if (r.vecs > 1 && r.vecs == r.end && last >= 0 && last % nt == 0)
+          if (r.vecs > 1 && r.vecs == r.end && last >= 0 && last < 32 * vpt && last % 32 == 0)
             for (int j = 0; j < a.V + r.shift - (r.vecs - 1) * VEC; ++j) g[(r.vecs - 1) * VEC - r.shift + j] = reinterpret_cast<const T*>(cut + 1)[j];
         }
         // chains of this thread's vectors
-        uint32_t* words = reinterpret_cast<uint32_t*>(heads + (chain * nt + tid) * 4);
-        uint32_t any = words[0];
-        if (sizeof(LINK) == 2) any |= words[1];
-        if (any) {
+        typedef typename Heads<LINK>::type heads_t;
+        heads_t& chains = *reinterpret_cast<heads_t*>(heads + (prev * nt + tid) * 8);
+        if (any(chains)) {
           if (!empty) {
-            const LINK* link = links + chain * a.K;
+            const LINK* link = links + prev * a.K;
 #pragma unroll 1
-            for (int v = 0; v < VPT; ++v) {
+            for (int v = 0; v < vpt; ++v) {
               uint32_t done = 0;
 #pragma unroll 1
-              for (int e = heads[(chain * nt + tid) * 4 + v]; e; e = link[e - 1]) {
+              for (int e = heads[(prev * nt + tid) * 8 + v]; e; e = link[e - 1]) {
                 const int i = __float_as_int(entries[e - 1].y), j = (i + r.shift) & (VEC - 1);
                 if (done >> j & 1u) continue;
                 done |= 1u << j;
                 float p = ex2(entries[e - 1].x);
                 if (link[e - 1]) p = chained_p(entries, link, e, p);
-                const float z = to_f32(reinterpret_cast<const T*>(mine + v * nt)[j]);
-                g[i] = from_f32<T>((ex2(fmaf(z, c, -m)) / s - p) * w);
+                const float x = to_f32(reinterpret_cast<const T*>(mine + v * 32)[j]);
+                g[i] = from_f32<T>((ex2(fmaf(x, c, -m)) / s - p) * w);
               }
             }
           }
-          words[0] = 0u;
-          if (sizeof(LINK) == 2) words[1] = 0u;
+          clear(chains);
         }
       }
-      if (a.loss && rank == 0 && tid >> 5 == was % nw) {      // (the warps take the rows' losses in turn)
+      if (a.loss && rank == 0 && tid >> 5 == (was & (nw - 1))) {         // (the warps take the rows' losses in turn)
         const float ls = log2f(s);
         float part = 0.f;
 #pragma unroll 4
         for (int k = lane; k < a.K; k += 32) {
           const int i = __float_as_int(entries[k].y);
-          const float lp = entries[k].x, z = i >= 0 ? to_f32(r.z[i]) : 0.f, p = ex2(lp);
-          if (i >= 0 && !(p == 0.f)) part += p * (lp - (fmaf(z, c, -m) - ls));
+          const float lp = entries[k].x, x = i >= 0 ? to_f32(z_old[i]) : 0.f, p = ex2(lp);
+          if (i >= 0 && !(p == 0.f)) part += p * (lp - (fmaf(x, c, -m) - ls));
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
         if (lane == 0) a.loss[old] = empty ? 0.f : part * 0.6931471805599453f * a.temperature * a.temperature;
       }
-      fetch(old + S::kVectors * stride, was + S::kVectors);
+      fetch(prev, (was + S::kVectors) % S::kEntries);
     }
     if (row < a.N) {
       // this warp's part of the first pass is written, and it is through with the row before
@@ -418,6 +447,8 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
         else mbar_arrive(bar);
       }
     }
+    prev = cur;
+    cur = cur == 2 ? 0 : cur + 1;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (clog) cluster_sync_all();                               // a CTA's shared memory is written until here
@@ -548,19 +579,21 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* rows,
 
 // How many clusters of 2^cluster_log CTAs of nt threads the GPU holds at once.
 template <typename T, bool EVEN, typename LINK, int VPT>
-cudaError_t cluster_places(int cluster_log, int nt, int* places) {
+cudaError_t cluster_places(int cluster_log, int nt, int vpt, int K, int* places) {
   auto kernel = distill_kernel<T, EVEN, LINK, VPT>;
-  typedef DistillSmem<LINK, VPT> S;
-  static std::atomic<int> known[64][4][6];
+  typedef DistillSmem<LINK> S;
+  static std::atomic<int> known[64][4][5][VPT + 1][3];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   int size = 0;
   while (32 << size < nt) ++size;
-  *places = dev < 64 ? known[dev][cluster_log][size].load(std::memory_order_acquire) : 0;
+  const int many = K > 128 ? 2 : K > 32 ? 1 : 0;              // (as if there were as many entries as that takes)
+  std::atomic<int>& slot = known[dev & 63][cluster_log][size][vpt][many];
+  *places = dev < 64 ? slot.load(std::memory_order_acquire) : 0;
   if (*places > 0) return cudaSuccess;
-  if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(kDistillThreads, S::kTop))) != cudaSuccess) return e;
-  const int smem = S::bytes(nt, std::min(S::kTop, 64));       // (more entries than that: some clusters may follow the others)
+  if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(kDistillThreads, VPT, S::kTop))) != cudaSuccess) return e;
+  const int smem = S::bytes(nt, vpt, std::min(S::kTop, many == 2 ? kDistillTop : many == 1 ? 128 : 32));
   if (cluster_log == 0) {
     int per_sm = 0;
     if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, nt, smem)) != cudaSuccess) return e;
@@ -579,15 +612,15 @@ cudaError_t cluster_places(int cluster_log, int nt, int* places) {
     if ((e = cudaOccupancyMaxActiveClusters(places, kernel, &cfg)) != cudaSuccess) return e;
   }
   if (*places < 1) return cudaErrorInvalidConfiguration;
-  if (dev < 64) known[dev][cluster_log][size].store(*places, std::memory_order_release);
+  if (dev < 64) slot.store(*places, std::memory_order_release);
   return cudaSuccess;
 }
 
 template <typename T, bool EVEN, typename LINK, int VPT>
 int distill_clusters(const DistillArgs& a, int nt, cudaStream_t st) {
   int places = 0;
-  LT_RETURN_IF_CUDA((cluster_places<T, EVEN, LINK, VPT>(a.cluster_log, nt, &places)));
-  const int ctas = 1 << a.cluster_log, clusters = std::min(a.N, places), smem = DistillSmem<LINK, VPT>::bytes(nt, a.K);
+  LT_RETURN_IF_CUDA((cluster_places<T, EVEN, LINK, VPT>(a.cluster_log, nt, a.vpt, a.K, &places)));
+  const int ctas = 1 << a.cluster_log, clusters = std::min(a.N, places), smem = DistillSmem<LINK>::bytes(nt, a.vpt, a.K);
   auto kernel = distill_kernel<T, EVEN, LINK, VPT>;
   if (ctas > 1) LT_RETURN_IF_CUDA(launch_chained_clusters(kernel, clusters * ctas, nt, smem, ctas, st, a));
   else LT_RETURN_IF_CUDA(launch_chained(kernel, clusters, nt, smem, st, a));
@@ -598,18 +631,20 @@ template <typename T>
 int distill(DistillArgs a, float* out, cudaStream_t st) {
   const bool even = a.V % kVec<T> == 0 && (a.N == 1 || a.ldz % kVec<T> == 0) && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0;
   const int vecs = even ? a.V / kVec<T> : a.V / kVec<T> + 2;  // (a row may begin and end inside a vector)
-  const bool few = a.K <= DistillSmem<uint8_t, 4>::kTop;
-  const int per = few ? 4 : 3;
+  const bool few = a.K <= DistillSmem<uint8_t>::kTop;
+  const int per = few ? 8 : 6;
   a.cluster_log = 0;
   while ((1 << a.cluster_log) < kDistillCluster && vecs > (per * kDistillThreads) << a.cluster_log) ++a.cluster_log;
   if (vecs <= (per * kDistillThreads) << a.cluster_log) {
     // few rows: more CTAs for each
     while ((1 << a.cluster_log) < kDistillCluster && (long long)a.N << (a.cluster_log + 1) <= sm_count() && vecs >> a.cluster_log >= 512) ++a.cluster_log;
+    const int own = (vecs + (1 << a.cluster_log) - 1) >> a.cluster_log;
     int nt = 32;
-    while (nt < kDistillThreads && vecs > (per * nt) << a.cluster_log) nt *= 2;
+    while (nt < kDistillThreads && own > per * nt) nt *= 2;
+    a.vpt = (own + nt - 1) / nt;
     int rc;
-    if (few) rc = even ? distill_clusters<T, true, uint8_t, 4>(a, nt, st) : distill_clusters<T, false, uint8_t, 4>(a, nt, st);
-    else rc = even ? distill_clusters<T, true, uint16_t, 3>(a, nt, st) : distill_clusters<T, false, uint16_t, 3>(a, nt, st);
+    if (few) rc = even ? distill_clusters<T, true, uint8_t, 8>(a, nt, st) : distill_clusters<T, false, uint8_t, 8>(a, nt, st);
+    else rc = even ? distill_clusters<T, true, uint16_t, 6>(a, nt, st) : distill_clusters<T, false, uint16_t, 6>(a, nt, st);
     if (rc) return rc;
   } else {
     LT_RETURN_IF_CUDA(launch_chained(distill_long_kernel<T>, std::min(a.N, 4 * sm_count()), kLongThreads, 0, st, a));
@@ -643,7 +678,7 @@ int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t
     const int grid = int(std::min<long long>((N + 7) / 8, 8ll * sm_count()));
     LT_RETURN_IF_CUDA(launch_chained(distill_teacher_kernel, grid, 256, 0, st, t, t_type, idx, N, V, K, kLog2e / temperature, pairs, flags));
   }
-  DistillArgs a{z, ldz, pairs, N, V, K, temperature, kLog2e / temperature, flags, up, up_rows, skip_one, reinterpret_cast<float2*>(stats), have_stats, loss, grad, ldg, 0, device_status_word()};
+  DistillArgs a{z, ldz, pairs, N, V, K, temperature, kLog2e / temperature, flags, up, up_rows, skip_one, reinterpret_cast<float2*>(stats), have_stats, loss, grad, ldg, 0, 0, device_status_word()};
   if (type == kElemF32) return distill<float>(a, out, st);
   if (type == kElemBf16) return distill<__nv_bfloat16>(a, out, st);
   return distill<__half>(a, out, st);
