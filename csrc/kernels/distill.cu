@@ -53,10 +53,11 @@ __device__ __forceinline__ float ex2(float x) {
 
 // The teacher's side, a warp to a row: log2 of its probabilities, and whether it is there at all.
 __global__ void __launch_bounds__(256) distill_teacher_kernel(const void* t, int t_type, const long long* idx, int N, int V, int K, float c, float2* entries,
-                                                              unsigned char* flags) {
+                                                              unsigned char* flags, unsigned* finished) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *finished = 0u;
   for (long long r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < N; r += gridDim.x * 8ll) {
     float m = -INFINITY, s = 0.f;
     bool any = false;
@@ -134,6 +135,17 @@ __device__ __forceinline__ bool any(const uint2& h) { return (h.x | h.y) != 0u; 
 __device__ __forceinline__ bool any(const uint4& h) { return (h.x | h.y | h.z | h.w) != 0u; }
 __device__ __forceinline__ void clear(uint2& h) { h = make_uint2(0u, 0u); }
 __device__ __forceinline__ void clear(uint4& h) { h = make_uint4(0u, 0u, 0u, 0u); }
+// The number of the first chain from v on (8: there is none), and its first entry + 1.
+__device__ __forceinline__ int first_head(const uint2& h, int v) {
+  const unsigned long long x = v < 8 ? ((unsigned long long)h.y << 32 | h.x) >> (8 * v) : 0ull;
+  return x ? v + (__ffsll(x) - 1) / 8 : 8;
+}
+__device__ __forceinline__ int head_of(const uint2& h, int v) { return ((v < 4 ? h.x : h.y) >> (8 * (v & 3))) & 0xff; }
+__device__ __forceinline__ int head_of(const uint4& h, int v) { return ((v < 4 ? v < 2 ? h.x : h.y : v < 6 ? h.z : h.w) >> (16 * (v & 1))) & 0xffff; }
+__device__ __forceinline__ int first_head(const uint4& h, int v) {
+  while (v < 8 && head_of(h, v) == 0) ++v;
+  return v;
+}
 // The teacher's probability of entry e's class (p by that entry alone) with those of the entries chained behind it that have the same.  Their sum is taken in
 // whole numbers of 2^-62: it must not depend on the chain's order.
 template <typename LINK>
@@ -182,7 +194,7 @@ __device__ __forceinline__ void send8(uint32_t dst, uint32_t bar, uint32_t cta, 
 template <typename LINK>
 struct DistillSmem {
   static constexpr int kTop = sizeof(LINK) == 1 ? 255 : kDistillTop;      // entries that a LINK numbers
-  static constexpr int kVectors = 3, kEntries = 4, kChains = 3, kPeers = 4;           // rows in turn
+  static constexpr int kVectors = 3, kEntries = 5, kChains = 4, kPeers = 4;           // rows in turn
   // vpt: vectors of a thread
   static __host__ __device__ int entries(int nt, int vpt) { return kVectors * vpt * nt * 16; }
   static __host__ __device__ int peers(int nt, int vpt, int K) { return entries(nt, vpt) + kEntries * K * 8; }
@@ -194,11 +206,12 @@ struct DistillSmem {
 // A cluster of CTAs holds a row, every thread up to VPT vectors of 16 bytes: a row is read from global memory once.  The threads go over their vectors twice, first
 // for the warps' maxima and sums, which go to all warps of the cluster, and then for the gradient; between the two they do the first pass over the
 // next row, so that nobody waits for the exchange, and the rows after that are on their way into shared memory.  There is no barrier of all threads:
-// a thread reads the vectors that it fetched itself, and one mbarrier a row counts the pairs that arrive and the warps that are through with the row before.
+// a thread reads the vectors that it fetched itself, and one mbarrier a row counts the pairs that arrive and this CTA's warps.  A warp that has passed the one of
+// row i - 2 knows that all have begun row i - 1 and are through with row i - 4: what rows share lies in as many places as that takes.
 // The teacher's classes are chained by the vector they lie in; the thread that writes the vector writes them again, from the 32-bit values.
 // EVEN: all rows begin and end with a vector.  LINK: the type that numbers entries.
 template <typename T, bool EVEN, typename LINK, int VPT>
-__global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a) {
+__global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs a) {
   constexpr int VEC = kVec<T>;
   typedef DistillSmem<LINK> S;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -250,6 +263,8 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
     r.end = min(r.vecs, r.lo + part);
     return r;
   };
+  // every thread of the warp has VPT vectors, none of which is cut
+  auto full = [&](const Row& r) { return vpt == VPT && r.lo + first - lane + 32 * VPT <= r.end && (EVEN || (r.lo + first - lane > 0 && r.lo + first - lane + 32 * VPT < r.vecs)); };
   const int stride = gridDim.x >> clog;
   int row = blockIdx.x >> clog;
   const long long step = (long long)stride * a.ldz;
@@ -264,6 +279,10 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
       const T* from = z_fetch - r.shift + (r.lo + first) * VEC;
       const uint32_t to = smem_u32(mine);
       const int end = r.end - r.lo - first, last = r.vecs - 1 - r.lo - first;
+      if (full(r)) {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) copy_async16(to + k * 512, from + k * 32 * VEC);
+      } else
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         if (k >= vpt) break;
@@ -283,7 +302,8 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
   __syncthreads();
   for (int i = 0; i < S::kVectors; ++i) fetch(i, i);
   if (clog) cluster_sync_all();                               // every CTA is there to be written to
-  int cur = 0, prev = 2;                                      // the first pass's place among three, and the second's
+  int cur = 0, prev = 2;                                      // places of the first pass's vectors and of the second's
+  int entry_cur = 0;                                          // place of the first pass's entries
   for (int it = 0; row - stride < a.N; row += stride, z += step, ++it) {
     if (row < a.N) {
       // ---- first pass over this row
@@ -292,13 +312,13 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
       const int turn = it % S::kPeers;
       uint4* mine = vectors + cur * room;
       if (a.grad) {
+        const float2* entries = entry_buf + entry_cur * a.K;
         const int elo = r.lo * VEC - r.shift, ehi = r.end * VEC - r.shift;
-        const float2* entries = entry_buf + it % S::kEntries * a.K;
-        for (int k = tid; k < a.K; k += nt) {
+            for (int k = tid; k < a.K; k += nt) {
           const int i = __float_as_int(entries[k].y);
           if (i >= max(elo, 0) && i < ehi) {
             const int v = (i - elo) / VEC, w = v / (32 * vpt), owner = w * 32 + v % 32;
-            links[cur * a.K + k] = LINK(exchange_small(heads, (cur * nt + owner) * 8 + (v / 32 - w * vpt), uint32_t(k + 1)));
+            links[turn * a.K + k] = LINK(exchange_small(heads, (turn * nt + owner) * 8 + (v / 32 - w * vpt), uint32_t(k + 1)));
           }
         }
       }
@@ -311,22 +331,33 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
       }
       if (!a.have_stats) {
         uint4 u[VPT];
-        float m = -INFINITY, s = 0.f;
+        if (full(r)) {
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-          u[k] = k < vpt ? mine[k * 32] : none;
-          m = fmaxf(m, max16<T>(u[k]));
+          for (int k = 0; k < VPT; ++k) u[k] = mine[k * 32];
+        } else {
+#pragma unroll
+          for (int k = 0; k < VPT; ++k) u[k] = k < vpt ? mine[k * 32] : none;
         }
+        float m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) m = fmaxf(m, max16<T>(u[k]));
         m *= c;
         const float from = m == -INFINITY ? 0.f : -m;
+        float part[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) part[j] = 0.f;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-          float f[VEC], part = 0.f;
+          float f[VEC];
           unpack16<T>(u[k], f);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) part += ex2(fmaf(f[j], c, from));
-          s += part;
+          for (int j = 0; j < VEC; ++j) part[j] += ex2(fmaf(f[j], c, from));
         }
+#pragma unroll
+        for (int j = VEC / 2; j > 0; j /= 2)
+#pragma unroll
+          for (int i = 0; i < j; ++i) part[i] += part[i + j];
+        float s = part[0];
         warp_max_sum(m, s);
         const int at = (turn * kDistillCluster + rank) * nw + (tid >> 5);
         if (clog) {
@@ -335,14 +366,18 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
           peers[at] = make_float2(m, s);
         }
       }
+      __syncwarp();
+      if (lane == 0) {
+        if (tid == 0 && clog && !a.have_stats) mbar_expect_tx(bar0 + 8 * turn, pairs * 8);
+        else mbar_arrive(bar0 + 8 * turn);
+      }
     }
     if (it > 0) {
       // ---- second pass over the row before
       const int was = it - 1, old = row - stride, turn = was % S::kPeers;
-      const T* z_old = z - step;
-      const Row r = row_of(z_old);
+      const Row r = row_of(z - step);
       uint4* mine = vectors + prev * room;
-      const float2* entries = entry_buf + was % S::kEntries * a.K;
+      const float2* entries = entry_buf + (entry_cur == 0 ? S::kEntries - 1 : entry_cur - 1) * a.K;
       mbar_wait(bar0 + 8 * turn, (was / S::kPeers) & 1, &abort_flag, a.status, kStatusTimeoutLocalFlag);
       const bool empty = __float_as_int(entries[0].y) == -2;
       float m, s;
@@ -354,13 +389,20 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
         m = -INFINITY;
         s = 0.f;
         const float2* all = peers + turn * kDistillCluster * nw;
-        for (int i = lane; i < pairs; i += 32) m = fmaxf(m, all[i].x);
+        float2 q[kDistillCluster * kDistillWarps / 32];
+#pragma unroll
+        for (int i = 0; i < kDistillCluster * kDistillWarps / 32; ++i) {
+          q[i] = make_float2(-INFINITY, 0.f);
+          if (i * 32 < pairs) {
+            if (i * 32 + lane < pairs) q[i] = all[i * 32 + lane];
+            m = fmaxf(m, q[i].x);
+          }
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        for (int i = lane; i < pairs; i += 32) {
-          const float2 q = all[i];
-          s += q.x == -INFINITY ? q.y : q.y * ex2(q.x - m);
-        }
+#pragma unroll
+        for (int i = 0; i < kDistillCluster * kDistillWarps / 32; ++i)
+          if (i * 32 < pairs) s += q[i].x == -INFINITY ? q[i].y : q[i].y * ex2(q[i].x - m);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (a.stats && rank == 0 && tid == 0) a.stats[old] = make_float2(m, s);
@@ -377,21 +419,30 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
           else if (!EVEN && k * 32 == last) cut[1] = u;
           else *reinterpret_cast<uint4*>(to + k * 32 * VEC) = u;
         };
-        if (!empty) {
+        auto gradient = [&](uint4 u) {
+          float f[VEC];
+          unpack16<T>(u, f);
 #pragma unroll
-          for (int k = 0; k < VPT; ++k) {
-            if (k < vpt && k * 32 < end) {
-              float f[VEC];
-              unpack16<T>(mine[k * 32], f);
+          for (int j = 0; j < VEC; ++j) f[j] = ex2(fmaf(f[j], c, -m)) * scale;
+          return pack16<T>(f);
+        };
+        if (!empty && full(r)) {
+          uint4 u[VPT];
 #pragma unroll
-              for (int j = 0; j < VEC; ++j) f[j] = ex2(fmaf(f[j], c, -m)) * scale;
-              store(k, pack16<T>(f));
+          for (int k = 0; k < VPT; ++k) u[k] = mine[k * 32];
+#pragma unroll
+          for (int k = 0; k < VPT; ++k) *reinterpret_cast<uint4*>(to + k * 32 * VEC) = gradient(u[k]);
+        } else if (!empty) {
+#pragma unroll 1
+          for (int k = 0; k < vpt; ++k) {
+            if (k * 32 < end) {
+              store(k, gradient(mine[k * 32]));
             }
           }
         } else {
-#pragma unroll
-          for (int k = 0; k < VPT; ++k)
-            if (k < vpt && k * 32 < end) store(k, make_uint4(0u, 0u, 0u, 0u));
+#pragma unroll 1
+          for (int k = 0; k < vpt; ++k)
+            if (k * 32 < end) store(k, make_uint4(0u, 0u, 0u, 0u));
         }
         if (cuts) {                                           // cut vectors by their elements
           if (head == 0 && end > 0)
@@ -401,54 +452,32 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(DistillArgs a)
         }
         // chains of this thread's vectors
         typedef typename Heads<LINK>::type heads_t;
-        heads_t& chains = *reinterpret_cast<heads_t*>(heads + (prev * nt + tid) * 8);
+        heads_t& chains = *reinterpret_cast<heads_t*>(heads + (turn * nt + tid) * 8);
         if (any(chains)) {
           if (!empty) {
-            const LINK* link = links + prev * a.K;
-#pragma unroll 1
-            for (int v = 0; v < vpt; ++v) {
+            const LINK* link = links + turn * a.K;
+            const heads_t h = chains;
+            for (int v = first_head(h, 0); v < 8; v = first_head(h, v + 1)) {
               uint32_t done = 0;
-#pragma unroll 1
-              for (int e = heads[(prev * nt + tid) * 8 + v]; e; e = link[e - 1]) {
+              for (int e = head_of(h, v); e; e = link[e - 1]) {
                 const int i = __float_as_int(entries[e - 1].y), j = (i + r.shift) & (VEC - 1);
                 if (done >> j & 1u) continue;
                 done |= 1u << j;
                 float p = ex2(entries[e - 1].x);
                 if (link[e - 1]) p = chained_p(entries, link, e, p);
                 const float x = to_f32(reinterpret_cast<const T*>(mine + v * 32)[j]);
-                g[i] = from_f32<T>((ex2(fmaf(x, c, -m)) / s - p) * w);
+                g[i] = from_f32<T>((__fdividef(ex2(fmaf(x, c, -m)), s) - p) * w);
               }
             }
           }
           clear(chains);
         }
       }
-      if (a.loss && rank == 0 && tid >> 5 == (was & (nw - 1))) {         // (the warps take the rows' losses in turn)
-        const float ls = log2f(s);
-        float part = 0.f;
-#pragma unroll 4
-        for (int k = lane; k < a.K; k += 32) {
-          const int i = __float_as_int(entries[k].y);
-          const float lp = entries[k].x, x = i >= 0 ? to_f32(z_old[i]) : 0.f, p = ex2(lp);
-          if (i >= 0 && !(p == 0.f)) part += p * (lp - (fmaf(x, c, -m) - ls));
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-        if (lane == 0) a.loss[old] = empty ? 0.f : part * 0.6931471805599453f * a.temperature * a.temperature;
-      }
-      fetch(prev, (was + S::kVectors) % S::kEntries);
-    }
-    if (row < a.N) {
-      // this warp's part of the first pass is written, and it is through with the row before
-      __syncwarp();
-      if (lane == 0) {
-        const uint32_t bar = bar0 + 8 * (it % S::kPeers);
-        if (tid == 0 && clog && !a.have_stats) mbar_expect_tx(bar, pairs * 8);
-        else mbar_arrive(bar);
-      }
+      fetch(prev, entry_cur < S::kEntries - 2 ? entry_cur + 2 : entry_cur + 2 - S::kEntries);
     }
     prev = cur;
-    cur = cur == 2 ? 0 : cur + 1;
+    cur = cur == S::kVectors - 1 ? 0 : cur + 1;
+    entry_cur = entry_cur == S::kEntries - 1 ? 0 : entry_cur + 1;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (clog) cluster_sync_all();                               // a CTA's shared memory is written until here
@@ -459,7 +488,6 @@ template <typename T>
 __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs a) {
   constexpr int VEC = kVec<T>;
   __shared__ float2 red[kLongWarps];
-  __shared__ float fsum[kLongWarps];
   __shared__ int isum[kLongWarps];
   pdl_launch_dependents();
   pdl_wait();
@@ -510,24 +538,6 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
       warp_max_sum(m, s);
       if (a.stats && tid == 0) a.stats[row] = make_float2(m, s);
     }
-    if (a.loss) {
-      const float ls = log2f(s);
-      float part = 0.f;
-      for (int k = tid; k < a.K; k += kLongThreads) {
-        const int i = __float_as_int(entries[k].y);
-        const float lp = entries[k].x, p = ex2(lp);
-        if (i >= 0 && !(p == 0.f)) part += p * (lp - (fmaf(to_f32(z[i]), c, -m) - ls));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      if (lane == 0) fsum[warp] = part;
-      __syncthreads();
-      if (tid == 0) {
-        part = 0.f;
-        for (int q = 0; q < kLongWarps; ++q) part += fsum[q];
-        a.loss[row] = empty ? 0.f : part * 0.6931471805599453f * a.temperature * a.temperature;
-      }
-    }
     if (g) {
       const float w = a.up_rows ? weight * a.up[row] : weight;
       const float scale = w / s;
@@ -557,22 +567,49 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
   }
 }
 
-// The mean over the rows that have a teacher, or the sum.
-__global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* rows, const unsigned char* flags, int N, float* out) {
+// The losses, a warp to a row, from the rows' references and sums; the last CTA to finish makes their mean over the rows that have a teacher, or their sum.
+template <typename T>
+__global__ void __launch_bounds__(256) distill_loss_kernel(DistillArgs a, float* out, unsigned* finished) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ double red[32];
-  __shared__ int isum[32];
+  __shared__ double red[8];
+  __shared__ int isum[8];
+  __shared__ bool last;
+  const int lane = threadIdx.x & 31;
+  for (int row = blockIdx.x * 8 + (threadIdx.x >> 5); row < a.N; row += gridDim.x * 8) {
+    const T* z = static_cast<const T*>(a.z) + (long long)row * a.ldz;
+    const float2* entries = a.entries + (long long)row * a.K;
+    const float2 q = a.stats[row];
+    const float ls = log2f(q.y);
+    float part = 0.f;
+#pragma unroll 4
+    for (int k = lane; k < a.K; k += 32) {
+      const float2 e = entries[k];
+      const int i = __float_as_int(e.y);
+      const float x = i >= 0 ? to_f32(z[i]) : 0.f, p = ex2(e.x);
+      if (i >= 0 && !(p == 0.f)) part += p * (e.x - (fmaf(x, a.c, -q.x) - ls));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    if (lane == 0) a.loss[row] = part * 0.6931471805599453f * a.temperature * a.temperature;
+  }
+  if (!out) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(finished, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   double v = 0.0;
-  for (int i = threadIdx.x; i < N; i += 1024) v += rows[i];
+  for (int i = threadIdx.x; i < a.N; i += 256) v += __ldcg(a.loss + i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  const int n = flags ? max(1, count_flags(flags, N, isum)) : 1;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
+  const int n = a.flags ? max(1, count_flags(a.flags, a.N, isum)) : 1;
   __syncthreads();
   if (threadIdx.x == 0) {
     v = 0.0;
-    for (int w = 0; w < 32; ++w) v += red[w];
+    for (int w = 0; w < 8; ++w) v += red[w];
     *out = float(v / n);
   }
 }
@@ -628,11 +665,11 @@ int distill_clusters(const DistillArgs& a, int nt, cudaStream_t st) {
 }
 
 template <typename T>
-int distill(DistillArgs a, float* out, cudaStream_t st) {
+int distill(DistillArgs a, float* out, unsigned* finished, cudaStream_t st) {
   const bool even = a.V % kVec<T> == 0 && (a.N == 1 || a.ldz % kVec<T> == 0) && (reinterpret_cast<uintptr_t>(a.z) & 15) == 0;
   const int vecs = even ? a.V / kVec<T> : a.V / kVec<T> + 2;  // (a row may begin and end inside a vector)
   const bool few = a.K <= DistillSmem<uint8_t>::kTop;
-  const int per = few ? 8 : 6;
+  const int per = few ? 8 : 5;
   a.cluster_log = 0;
   while ((1 << a.cluster_log) < kDistillCluster && vecs > (per * kDistillThreads) << a.cluster_log) ++a.cluster_log;
   if (vecs <= (per * kDistillThreads) << a.cluster_log) {
@@ -644,12 +681,12 @@ int distill(DistillArgs a, float* out, cudaStream_t st) {
     a.vpt = (own + nt - 1) / nt;
     int rc;
     if (few) rc = even ? distill_clusters<T, true, uint8_t, 8>(a, nt, st) : distill_clusters<T, false, uint8_t, 8>(a, nt, st);
-    else rc = even ? distill_clusters<T, true, uint16_t, 6>(a, nt, st) : distill_clusters<T, false, uint16_t, 6>(a, nt, st);
+    else rc = even ? distill_clusters<T, true, uint16_t, 5>(a, nt, st) : distill_clusters<T, false, uint16_t, 5>(a, nt, st);
     if (rc) return rc;
   } else {
     LT_RETURN_IF_CUDA(launch_chained(distill_long_kernel<T>, std::min(a.N, 4 * sm_count()), kLongThreads, 0, st, a));
   }
-  if (out) LT_RETURN_IF_CUDA(launch_chained(distill_reduce_kernel, 1, 1024, 0, st, static_cast<const float*>(a.loss), a.flags, a.N, out));
+  if (a.loss) LT_RETURN_IF_CUDA(launch_chained(distill_loss_kernel<T>, std::min((a.N + 7) / 8, 8 * sm_count()), 256, 0, st, a, out, finished));
   return 0;
 }
 
@@ -658,7 +695,7 @@ int distill(DistillArgs a, float* out, cudaStream_t st) {
 extern "C" {
 
 // Distillation of student logits z [N, V] (pitch ldz; fp32, bf16 or fp16: type 0, 1, 2) from teacher logits t [N, K] (type t_type) at classes idx [N, K].
-//   entries [N, K, 2] floats: written from t and idx; read if t is null
+//   entries [N, K, 2] floats and one more: written from t and idx; read if t is null
 //   flags [N] bytes: the loss is a mean over the rows that have a teacher (written or read likewise); null: no mean
 //   loss [N] or null; out: their sum or mean, or null; stats [N, 2]: written, or read (have_stats: z is not searched for its maximum again)
 //   grad [N, V] (pitch ldg; every row as far behind a multiple of 16 bytes as z's) or null: times up, which is null (1), one number, or (up_rows) one for every row; skip_one: nothing is done where up is one number and it is 1
@@ -666,7 +703,7 @@ int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t
                unsigned char* flags, const float* up, int up_rows, int skip_one, float* stats, int have_stats, float* loss, float* out, void* grad, long long ldg,
                void* stream) {
   using namespace lt;
-  if (type < 0 || type > 2 || t_type < 0 || t_type > 2 || N < 0 || V < 1 || K < 1 || K > kDistillTop || !(temperature > 0.f) || (out && !loss) ||
+  if (type < 0 || type > 2 || t_type < 0 || t_type > 2 || N < 0 || V < 1 || K < 1 || K > kDistillTop || !(temperature > 0.f) || (out && !loss) || (loss && (!stats || !t)) ||
       (reinterpret_cast<uintptr_t>(entries) & 7) != 0)
     return -int(kStatusBadArgument);
   if (N == 0) return 0;
@@ -674,14 +711,15 @@ int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t
   if (grad && (((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(z)) & 15) != 0 || (N > 1 && (ldg - ldz) * bytes % 16 != 0))) return -int(kStatusBadArgument);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float2* pairs = reinterpret_cast<float2*>(entries);
+  unsigned* finished = reinterpret_cast<unsigned*>(entries + 2ll * N * K);
   if (t) {
     const int grid = int(std::min<long long>((N + 7) / 8, 8ll * sm_count()));
-    LT_RETURN_IF_CUDA(launch_chained(distill_teacher_kernel, grid, 256, 0, st, t, t_type, idx, N, V, K, kLog2e / temperature, pairs, flags));
+    LT_RETURN_IF_CUDA(launch_chained(distill_teacher_kernel, grid, 256, 0, st, t, t_type, idx, N, V, K, kLog2e / temperature, pairs, flags, finished));
   }
   DistillArgs a{z, ldz, pairs, N, V, K, temperature, kLog2e / temperature, flags, up, up_rows, skip_one, reinterpret_cast<float2*>(stats), have_stats, loss, grad, ldg, 0, 0, device_status_word()};
-  if (type == kElemF32) return distill<float>(a, out, st);
-  if (type == kElemBf16) return distill<__nv_bfloat16>(a, out, st);
-  return distill<__half>(a, out, st);
+  if (type == kElemF32) return distill<float>(a, out, finished, st);
+  if (type == kElemBf16) return distill<__nv_bfloat16>(a, out, finished, st);
+  return distill<__half>(a, out, finished, st);
 }
 
 }  // extern "C"

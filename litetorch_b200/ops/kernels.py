@@ -1682,17 +1682,18 @@ def distill_loss(z, t, idx, temperature: float, reduction: str, with_grad: bool)
     z = z if z.stride(1) == 1 else z.contiguous()
     t, idx = t.contiguous(), idx.to(torch.int64).contiguous()
     mean = reduction == "mean"
-    # [N, K, 2] entries, [N, 2] maxima and sums, [N] losses, [N] bytes
-    room = z.new_empty(N * (2 * top + 3) + (N + 3) // 4, dtype=torch.float32)
+    # [N, K, 2] entries and a counter, [N, 2] references and sums, [N] losses, [N] bytes
+    room = z.new_empty(N * (2 * top + 3) + 2 + (N + 3) // 4, dtype=torch.float32)
     at = room.data_ptr()
-    stats, loss, flags = at + 8 * N * top, at + 8 * N * (top + 1), at + 4 * N * (2 * top + 3)
+    stats = at + 8 * (N * top + 1)
+    loss, flags = stats + 8 * N, stats + 12 * N
     out = None if reduction == "none" else z.new_empty((), dtype=torch.float32)
     grad = _like_rows(z) if with_grad else None
     with _on(z):
         _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), _ELEM[t.dtype], t.data_ptr(), idx.data_ptr(), at, N, V, top, temperature,
                                  flags if mean else None, None, 0, 0, stats, 0, loss, _p(out), _p(grad), 0 if grad is None else grad.stride(0), _stream()), "lt_distill")
-    _launches[0] += 1 if out is None else 2
-    return room[2 * N * (top + 1):][:N] if out is None else out, grad, room
+    _launches[0] += 2
+    return room[2 * (N * (top + 1) + 1):][:N] if out is None else out, grad, room
 
 
 def distill_grad(z, room, top: int, temperature: float, mean: bool, up, grad=None):
@@ -1706,8 +1707,8 @@ def distill_grad(z, room, top: int, temperature: float, mean: bool, up, grad=Non
         grad = _like_rows(z)
     at = room.data_ptr()
     with _on(z):
-        _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), 0, None, None, at, N, V, top, temperature, at + 4 * N * (2 * top + 3) if mean else None,
-                                 up.data_ptr(), up.dim(), 1 if there else 0, at + 8 * N * top, 1, None, None, grad.data_ptr(), grad.stride(0),
+        _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), 0, None, None, at, N, V, top, temperature, at + 4 * (N * (2 * top + 3) + 2) if mean else None,
+                                 up.data_ptr(), up.dim(), 1 if there else 0, at + 8 * (N * top + 1), 1, None, None, grad.data_ptr(), grad.stride(0),
                                  _stream()), "lt_distill")
     return grad
 
