@@ -98,11 +98,15 @@ __device__ __forceinline__ int count_flags(const unsigned char* flags, int N, in
   return n;
 }
 
+__device__ __forceinline__ float warp_max(float v) {
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
+  return y;
+}
 // (reference, sum of 2^(. - reference)) over the warp.  Logits enter as fma(z, c, -reference), so that the reference is exact whatever its own rounding.
 __device__ __forceinline__ void warp_max_sum(float& m, float& s) {
   const float own = m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  m = warp_max(m);
   if (own != -INFINITY) s *= ex2(own - m);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -226,6 +230,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
   if (a.flags) weight /= float(max(1, count_flags(a.flags, a.N, isum)));
   if (a.up && !a.up_rows) weight *= a.up[0];
   const float c = a.c;
+  const uint64_t c2 = pack_f32x2(c, c);
   const int tid = threadIdx.x, lane = tid & 31, nt = blockDim.x, nw = nt >> 5;
   const int clog = a.cluster_log, rank = clog ? int(cluster_ctarank()) : 0;
   const int vpt = a.vpt, room = vpt * nt;
@@ -343,21 +348,28 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
         for (int k = 0; k < VPT; ++k) m = fmaxf(m, max16<T>(u[k]));
         m *= c;
         const float from = m == -INFINITY ? 0.f : -m;
-        float part[VEC];
+        uint64_t part[VEC / 2];
+        const uint64_t from2 = pack_f32x2(from, from);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) part[j] = 0.f;
+        for (int j = 0; j < VEC / 2; ++j) part[j] = 0ull;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
           float f[VEC];
           unpack16<T>(u[k], f);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) part[j] += ex2(fmaf(f[j], c, from));
+          for (int j = 0; j < VEC / 2; ++j) {
+            float x, y;
+            unpack_f32x2(fma_f32x2(pack_f32x2(f[2 * j], f[2 * j + 1]), c2, from2), x, y);
+            part[j] = add_f32x2(part[j], pack_f32x2(ex2(x), ex2(y)));
+          }
         }
 #pragma unroll
-        for (int j = VEC / 2; j > 0; j /= 2)
+        for (int j = VEC / 4; j > 0; j /= 2)
 #pragma unroll
-          for (int i = 0; i < j; ++i) part[i] += part[i + j];
-        float s = part[0];
+          for (int i = 0; i < j; ++i) part[i] = add_f32x2(part[i], part[i + j]);
+        float s, s1;
+        unpack_f32x2(part[0], s, s1);
+        s += s1;
         warp_max_sum(m, s);
         const int at = (turn * kDistillCluster + rank) * nw + (tid >> 5);
         if (clog) {
@@ -398,8 +410,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
             m = fmaxf(m, q[i].x);
           }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        m = warp_max(m);
 #pragma unroll
         for (int i = 0; i < kDistillCluster * kDistillWarps / 32; ++i)
           if (i * 32 < pairs) s += q[i].x == -INFINITY ? q[i].y : q[i].y * ex2(q[i].x - m);
@@ -423,7 +434,11 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
           float f[VEC];
           unpack16<T>(u, f);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) f[j] = ex2(fmaf(f[j], c, -m)) * scale;
+          for (int j = 0; j < VEC / 2; ++j) {
+            float x, y;
+            unpack_f32x2(fma_f32x2(pack_f32x2(f[2 * j], f[2 * j + 1]), c2, pack_f32x2(-m, -m)), x, y);
+            unpack_f32x2(mul_f32x2(pack_f32x2(ex2(x), ex2(y)), pack_f32x2(scale, scale)), f[2 * j], f[2 * j + 1]);
+          }
           return pack16<T>(f);
         };
         if (!empty && full(r)) {
