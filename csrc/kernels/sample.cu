@@ -18,6 +18,10 @@
 namespace lt {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32, kSampleBins = 2048, kSampleCluster = 8;
+constexpr int kSampleHold = 192 * 1024;                       // bytes of a row that a CTA holds at most, and such that two CTAs share an SM
+constexpr int kSampleHoldTwo = 80 * 1024;
+constexpr int kSampleFew = 256;                               // tokens that are compared each with each
+constexpr int kSampleGroups = 512;                            // maxima of groups of tokens
 constexpr double kMassOne = 17592186044416.0;                 // 2^44
 
 struct SampleArgs {
@@ -29,7 +33,7 @@ struct SampleArgs {
   const int* top_k;
   double tau1, top_p1, min_p1;
   int top_k1;
-  int rows, V, ctas;
+  int rows, V, ctas, held;
   long long* tokens;
   float* logprobs;              // or null
 };
@@ -62,289 +66,353 @@ template <> struct Key<__half> {
 
 typedef unsigned long long u64;
 
-__device__ __forceinline__ u64 mass_of(float z, float m, double inv_tau) {
-  if (!(z > -INFINITY)) return 0ull;
-  if (z == m) return u64(kMassOne);
-  const double x = (double(z) - double(m)) * inv_tau;
-  return x > -31.5 ? u64(rint(exp(x) * kMassOne)) : 0ull;     // (e^-31.5 is below half of 2^-44)
+// What the weights of a row go by.
+struct Weigh {
+  float m;                      // the largest logit
+  double md, k;                 // the same, and log2(e) / tau
+};
+// 2^44 times the weight of a logit, to the nearest whole number: 2^y with y = 16ths + r, |r| <= 1/32, the 16ths from a table, 2^r by the exponential series up to the
+// fifth power (the next term is below 2^-42).  Adding 256 to the weight leaves the whole number in the low bits of the sum.
+__device__ __forceinline__ u64 mass_of(float z, const Weigh& q, const double* table) {
+  // (no branches: the compiler works at several at once, each of which is a long chain)
+  const double y = (double(z) - q.md) * q.k;
+  const double shifted = fma(y, 16.0, 6755399441055744.0);    // (1.5 2^52: the sum's low bits are 16 y rounded)
+  const int n = __double2loint(shifted);
+  const double r = fma(shifted - 6755399441055744.0, -0.0625, y);
+  constexpr double L = 0.693147180559945309417232121458;
+  double p = fma(r, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
+  p = fma(p, r, L * L * L / 6.0);
+  p = fma(p, r, L * L / 2.0);
+  p = fma(p, r, L);
+  p = fma(p, r, 1.0) * table[n & 15];
+  p = __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p)) + 256.0;
+  const u64 w = y > -45.5 ? u64(__double_as_longlong(p)) & 0xfffffffffffffull : 0ull;
+  return z == q.m ? u64(kMassOne) : w;                        // (an infinite one too)
 }
 __device__ __forceinline__ u64 warp_add64(u64 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ u64 warp_scan64(u64 v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+// Logits with -inf in the place of NaN.
+template <typename T> __device__ __forceinline__ uint4 no_nan(uint4 u) {
+  if constexpr (sizeof(T) == 4) {
+    return make_uint4(__float_as_uint(fmaxf(__uint_as_float(u.x), -INFINITY)), __float_as_uint(fmaxf(__uint_as_float(u.y), -INFINITY)),
+                      __float_as_uint(fmaxf(__uint_as_float(u.z), -INFINITY)), __float_as_uint(fmaxf(__uint_as_float(u.w), -INFINITY)));
+  } else {
+    uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (__is_same(T, __nv_bfloat16)) {
+        const __nv_bfloat162 h = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), __floats2bfloat162_rn(-INFINITY, -INFINITY));
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&w[i]), __floats2half2_rn(-INFINITY, -INFINITY));
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
 
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+
+struct SampleShared {
+  uint32_t hist[kSampleBins];
+  u64 mass[kSampleBins];        // histograms of the general way; the short list's tokens and weights lie in the same place
+  u64 part[2];                  // what the other CTAs of the cluster read
+  u64 wsum[kSampleWarps];
+  uint32_t wcnt[kSampleWarps];
+  u64 found[2];
+  double table[16];
+  uint32_t groups[kSampleGroups];
+  uint32_t count;               // of the short list (the first CTA's)
+};
+
+// A row of a cluster of CTAs: where its vectors lie.  [vlo, vhi) are this warp's, and of all warps of all CTAs in index order.
 template <typename T>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
+struct SampleRow {
+  static constexpr int VEC = kVec<T>;
+  const T* z;
+  const uint4* held;            // vector 0 of the row, if it were in this CTA's shared memory as the CTA's own vectors are; null: they are read from z again
+  int shift, V, vlo, vhi;
+  __device__ __forceinline__ bool whole(int v) const { return v * VEC >= shift && v * VEC - shift + VEC <= V; }
+  __device__ __forceinline__ uint4 fetch(int v) const {
+    const int lo = v * VEC - shift;
+    if (whole(v)) return *reinterpret_cast<const uint4*>(z + lo);
+    float f[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = lo + j >= 0 && lo + j < V ? to_f32(z[lo + j]) : -INFINITY;
+    return pack16<T>(f);
+  }
+  __device__ __forceinline__ uint4 load(int v) const { return no_nan<T>(held ? held[v] : fetch(v)); }
+  // f(logit, vector, place in it) for this warp's logits
+  template <class F>
+  __device__ __forceinline__ void each(int lane, F f) const {
+#pragma unroll 2
+    for (int v = vlo + lane; v < vhi; v += 32) {
+      float x[VEC];
+      unpack16<T>(load(v), x);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f(x[j], v, j);
+    }
+  }
+};
+
+struct Filters {
+  int k;
+  double p;
+  u64 least;
+};
+
+// The cumulated mass that the drawn token's exceeds.
+__device__ __forceinline__ u64 draw_target(const SampleArgs& a, int row, u64 total) {
+  double u = a.u64bit ? static_cast<const double*>(a.u)[row] : double(static_cast<const float*>(a.u)[row]);
+  u = u > 0.0 ? fmin(u, 1.0) : 0.0;
+  return min(u64(u * double(total)), total - 1);
+}
+__device__ __forceinline__ void write_token(const SampleArgs& a, int row, int token, float z, const Weigh& q, u64 total) {
+  a.tokens[row] = token;
+  if (a.logprobs) a.logprobs[row] = float(((z == q.m ? 0.0 : (double(z) - q.md) * q.k) - log2(double(total) / kMassOne)) * 0.693147180559945309417232121458);
+}
+
+// n tokens in list (key and token): who stays, and which of them is drawn.
+template <typename T>
+__device__ __forceinline__ void short_list(const SampleArgs& a, int row, const Weigh& q, const Filters& by, int n, u64* list, SampleShared& sh) {
+  u64* weight = list + kSampleFew;
+  u64* mass_before = weight + kSampleFew;
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) weight[i] = mass_of(Key<T>::value(uint32_t(list[i] >> 32)), q, sh.table);
+  if (threadIdx.x == 0) sh.found[0] = 0;
+  __syncthreads();
+  // a quarter of a warp to a token: its place in the order, and the mass of those in front of it
+  for (int i0 = threadIdx.x >> 3; i0 - (lane >> 3) < n; i0 += blockDim.x >> 3) {
+    const int i = min(i0, n - 1);
+    const u64 mine = list[i];
+    uint32_t place = 0;
+    u64 before = 0;
+    for (int o = lane & 7; o < n; o += 8) {
+      const u64 other = list[o];
+      // greater key, or the same and a lower token
+      const bool ahead = (other >> 32) > (mine >> 32) || ((other >> 32) == (mine >> 32) && uint32_t(other) < uint32_t(mine));
+      place += ahead;
+      before += ahead ? weight[o] : 0ull;
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      place += __shfl_xor_sync(0xffffffffu, place, o);
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    if (i0 < n && (lane & 7) == 0) {
+      const bool in = by.k <= 0 || place < uint32_t(by.k);
+      mass_before[i] = in ? before : ~0ull;                   // (~0: does not stay)
+      if (in) atomicMax(&sh.found[0], before + weight[i]);    // in the end the mass of the first k; for top-p alone the list may lack tokens
+    }
+  }
+  __syncthreads();
+  u64 want = ~0ull;
+  if (by.p < 1.0) {
+    const u64 all = by.k > 0 ? sh.found[0] : sh.found[1];
+    want = max(1ull, u64(ceil(fmax(by.p, 0.0) * double(all))));
+  }
+  for (int i = threadIdx.x; i < n; i += blockDim.x)
+    if (!(mass_before[i] < want) || weight[i] < by.least) weight[i] = 0;
+  __syncthreads();
+  // cumulated masses in the order of the tokens' numbers
+  u64 total = 0;
+  for (int i = lane; i < n; i += 32) total += weight[i];
+  total = warp_add64(total);
+  const u64 target = draw_target(a, row, total);
+  for (int i0 = threadIdx.x >> 3; i0 - (lane >> 3) < n; i0 += blockDim.x >> 3) {
+    const int i = min(i0, n - 1);
+    const uint32_t token = uint32_t(list[i]);
+    u64 before = 0;
+    for (int o = lane & 7; o < n; o += 8) before += uint32_t(list[o]) < token ? weight[o] : 0ull;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (i0 < n && (lane & 7) == 0 && before <= target && target < before + weight[i]) write_token(a, row, int(token), Key<T>::value(uint32_t(list[i] >> 32)), q, total);
+  }
+}
+
+// The general way, for filters that leave many tokens: every step goes over the row again (in L2).
+// `bound`: tokens below it do not stay for top-k and top-p.  mass: that of all tokens, if top-p is the only limit and the row is held.
+template <typename T>
+__device__ __noinline__ void sample_general(const SampleArgs& a, const SampleRow<T>& r, const Weigh& q, const Filters& by, float bound, u64 mass, int row, int rank,
+                                            SampleShared& sh) {
   constexpr int VEC = kVec<T>;
-  __shared__ uint32_t hist[kSampleBins];
-  __shared__ u64 mass[kSampleBins];
-  __shared__ u64 part[2];                                     // what the other CTAs of the cluster read
-  __shared__ u64 wsum[kSampleWarps];
-  __shared__ uint32_t wcnt[kSampleWarps];
-  __shared__ u64 found[3];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int C = a.ctas, rank = C > 1 ? int(cluster_ctarank()) : 0;
-  const int row = blockIdx.x / C;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const T* z = static_cast<const T*>(a.z) + row * a.ldz;
+  const int C = a.ctas, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
   auto everywhere = [&] {                                     // all CTAs of the row are here, and see what was written before
     if (C > 1) cluster_sync_all();
     else __syncthreads();
   };
-
-  double tau = a.tau ? double(a.tau[row]) : a.tau1;
-  double p = a.top_p ? double(a.top_p[row]) : a.top_p1;
-  const double low = a.min_p ? double(a.min_p[row]) : a.min_p1;
-  int k = a.top_k ? a.top_k[row] : a.top_k1;
-  if (!(tau > 0.0)) { k = 1; tau = 1.0; }
-  if (k == 1) p = 1.0;
-  const double inv_tau = 1.0 / tau;
-  const u64 least = low > 0.0 ? u64(ceil(fmin(low, 1.0) * kMassOne)) : 0ull;
-
-  // vectors of the row: [vlo, vhi) are this warp's, and of all warps of all CTAs in index order
-  const int shift = int(reinterpret_cast<uintptr_t>(z) & 15) / int(sizeof(T));
-  const int vecs = (a.V + shift + VEC - 1) / VEC;
-  const int vcta = (vecs + C - 1) / C, vwarp = (vcta + kSampleWarps - 1) / kSampleWarps;
-  const int cend = min(vecs, (rank + 1) * vcta);
-  const int vlo = min(cend, rank * vcta + warp * vwarp), vhi = min(cend, vlo + vwarp);
-  auto load = [&](int v, float (&f)[VEC]) {
-    const int lo = v * VEC - shift;
-    if (lo >= 0 && lo + VEC <= a.V) {
-      unpack16<T>(*reinterpret_cast<const uint4*>(z + lo), f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = f[j] == f[j] ? f[j] : -INFINITY;
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        f[j] = lo + j >= 0 && lo + j < a.V ? to_f32(z[lo + j]) : -INFINITY;
-        f[j] = f[j] == f[j] ? f[j] : -INFINITY;
-      }
-    }
-  };
-
-  // ---- the maximum
-  float m = -INFINITY;
-  for (int v = vlo + lane; v < vhi; v += 32) {
-    float f[VEC];
-    load(v, f);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) m = fmaxf(m, f[j]);
-  }
-  uint32_t top = __reduce_max_sync(0xffffffffu, Key<float>::of(m));
-  if (lane == 0) wcnt[warp] = top;
-  __syncthreads();
-  for (int w = 0; w < kSampleWarps; ++w) top = max(top, wcnt[w]);
-  if (C > 1) {
-    if (threadIdx.x == 0) part[0] = top;
-    cluster_sync_all();
-    for (int c = 0; c < C; ++c) top = max(top, uint32_t(*cluster_peer(part, c)));
-    cluster_sync_all();
-  }
-  m = Key<float>::value(top);
-  if (m == -INFINITY) {
-    if (rank == 0 && threadIdx.x == 0) {
-      a.tokens[row] = -1;
-      if (a.logprobs) a.logprobs[row] = -INFINITY;
-    }
-    return;
-  }
-
   // Sum of v over the threads of all CTAs, for all of them.
   auto sum_all = [&](u64 v) {
     v = warp_add64(v);
     __syncthreads();
-    if (lane == 0) wsum[warp] = v;
+    if (lane == 0) sh.wsum[warp] = v;
     __syncthreads();
     v = 0;
-    for (int w = 0; w < kSampleWarps; ++w) v += wsum[w];
+    for (int w = 0; w < nw; ++w) v += sh.wsum[w];
     if (C > 1) {
-      if (threadIdx.x == 0) part[0] = v;
+      if (threadIdx.x == 0) sh.part[0] = v;
       cluster_sync_all();
       v = 0;
-      for (int c = 0; c < C; ++c) v += *cluster_peer(part, c);
+      for (int c = 0; c < C; ++c) v += *cluster_peer(sh.part, c);
       cluster_sync_all();
     }
     return v;
   };
-
   // What stays: keys above `limit`, and the first `ties` of those at it.
   uint32_t limit = 0;
-  u64 ties = ~0ull, all = 0;                                  // all: mass of what stays after top-k
-  constexpr int kBits = Key<T>::kBits;
-  constexpr int kDigit = 11;
-  // The key at which the running sum over keys from the top (counts, or masses with the first `ties` of those at `limit`) reaches `want`, and the sum above it.
+  u64 ties = ~0ull;
+  const uint32_t key_lo = Key<T>::of(bound), key_hi = Key<T>::of(q.m);
+  // The key at which the running sum over keys from the top (counts, or masses with the first `ties` of those at `limit`) reaches `want`, and the sum above it:
+  // the interval of the keys is cut into up to 2048 pieces until they are single keys.
   auto select = [&](bool by_mass, u64 want, u64& above) {
-    uint32_t prefix = 0;
+    uint32_t lo = key_lo, hi = key_hi;
     above = 0;
-    for (int left = kBits; left > 0;) {
-      const int bits = min(kDigit, left), sh = left - bits;
-      const uint32_t low_mask = (1u << bits) - 1u;
-      for (int i = threadIdx.x; i < kSampleBins; i += kSampleThreads) {
-        hist[i] = 0u;
-        if (by_mass) mass[i] = 0ull;
+    for (;;) {
+      const int width = 32 - __clz(int(hi - lo)), cut = max(0, width - 11);
+      for (int i = threadIdx.x; i < kSampleBins; i += blockDim.x) {
+        sh.hist[i] = 0u;
+        sh.mass[i] = 0ull;
       }
       __syncthreads();
-      for (int v = vlo + lane; v < vhi; v += 32) {
-        float f[VEC];
-        load(v, f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const uint32_t key = Key<T>::of(f[j]);
-          if (f[j] == -INFINITY || (left < 32 && (key >> (left & 31)) != prefix)) continue;
-          if (!by_mass) atomicAdd(&hist[(key >> sh) & low_mask], 1u);
-          else if (key > limit || (key == limit && ties == ~0ull)) {
-            const u64 w = mass_of(f[j], m, inv_tau);
-            if (w) atomicAdd(&mass[(key >> sh) & low_mask], w);
-          }
+      r.each(lane, [&](float z, int, int) {
+        const uint32_t key = Key<T>::of(z);
+        if (z == -INFINITY || key < lo || key > hi) return;
+        if (!by_mass) atomicAdd(&sh.hist[(key - lo) >> cut], 1u);
+        else if (key > limit || (key == limit && ties == ~0ull)) {
+          const u64 w = mass_of(z, q, sh.table);
+          if (w) atomicAdd(&sh.mass[(key - lo) >> cut], w);
         }
-      }
-      if (by_mass && ties != ~0ull && rank == 0 && threadIdx.x == 0 && (left >= 32 || (limit >> (left & 31)) == prefix))
-        atomicAdd(&mass[(limit >> sh) & low_mask], ties * mass_of(Key<T>::value(limit), m, inv_tau));
+      });
+      if (by_mass && ties != ~0ull && rank == 0 && threadIdx.x == 0 && limit >= lo && limit <= hi)
+        atomicAdd(&sh.mass[(limit - lo) >> cut], ties * mass_of(Key<T>::value(limit), q, sh.table));
       everywhere();
       // bins from the top, 2048 / threads to a thread
-      constexpr int PER = kSampleBins / kSampleThreads;
-      u64 v[PER], own = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int bin = kSampleBins - 1 - (int(threadIdx.x) * PER + i);
-        v[i] = 0;
-        for (int c = 0; c < C; ++c) v[i] += by_mass ? (C > 1 ? *cluster_peer(mass + bin, c) : mass[bin]) : u64(C > 1 ? *cluster_peer(hist + bin, c) : hist[bin]);
-        own += v[i];
-      }
-      u64 incl = own;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 x = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += x;
-      }
-      if (lane == 31) wsum[warp] = incl;
+      const int per = kSampleBins / int(blockDim.x);
+      auto bin = [&](int i) {
+        const int at = kSampleBins - 1 - (int(threadIdx.x) * per + i);
+        u64 v = 0;
+        for (int c = 0; c < C; ++c) v += by_mass ? (C > 1 ? *cluster_peer(sh.mass + at, c) : sh.mass[at]) : u64(C > 1 ? *cluster_peer(sh.hist + at, c) : sh.hist[at]);
+        return v;
+      };
+      u64 own = 0;
+      for (int i = 0; i < per; ++i) own += bin(i);
+      const u64 incl = warp_scan64(own, lane);
+      if (lane == 31) sh.wsum[warp] = incl;
       __syncthreads();
       u64 before = above + incl - own;
-      for (int w = 0; w < warp; ++w) before += wsum[w];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        if (before < want && want <= before + v[i]) {
-          found[0] = u64(kSampleBins - 1 - (int(threadIdx.x) * PER + i));
-          found[1] = before;
+      for (int w = 0; w < warp; ++w) before += sh.wsum[w];
+      if (before < want && want <= before + own)
+        for (int i = 0; i < per; ++i) {
+          const u64 v = bin(i);
+          if (before < want && want <= before + v) {
+            sh.found[0] = u64(kSampleBins - 1 - (int(threadIdx.x) * per + i));
+            sh.found[1] = before;
+          }
+          before += v;
         }
-        before += v[i];
-      }
       everywhere();
-      prefix = (prefix << bits) | uint32_t(found[0]);
-      above = found[1];
-      left = sh;
+      lo += uint32_t(sh.found[0]) << cut;
+      above = sh.found[1];
       __syncthreads();
+      if (cut == 0) return lo;
+      hi = min(hi, lo + ((1u << cut) - 1u));
     }
-    return prefix;
   };
 
-  // ---- top-k
-  if (k > 0 && k < a.V) {
+  if (by.k > 0 && by.k < a.V) {
     u64 have = 0;
-    if (k == 1) {
-      limit = Key<T>::of(m);
-      ties = 1;
-    } else {
-      for (int v = vlo + lane; v < vhi; v += 32) {
-        float f[VEC];
-        load(v, f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) have += f[j] != -INFINITY;
-      }
-      if (sum_all(have) > u64(k)) {
-        u64 above;
-        limit = select(false, u64(k), above);
-        ties = u64(k) - above;
-      }
+    r.each(lane, [&](float z, int, int) { have += z != -INFINITY; });
+    if (sum_all(have) > u64(by.k)) {
+      u64 above;
+      limit = select(false, u64(by.k), above);
+      ties = u64(by.k) - above;
     }
   }
-  // ---- top-p
-  if (p < 1.0) {
-    u64 own = 0;
-    for (int v = vlo + lane; v < vhi; v += 32) {
-      float f[VEC];
-      load(v, f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const uint32_t key = Key<T>::of(f[j]);
-        if (key > limit || (key == limit && ties == ~0ull)) own += mass_of(f[j], m, inv_tau);
-      }
+  if (by.p < 1.0) {
+    u64 all = mass;
+    if (by.k > 0 || !r.held) {
+      u64 own = 0;
+      r.each(lane, [&](float z, int, int) {
+        const uint32_t key = Key<T>::of(z);
+        const u64 w = mass_of(z, q, sh.table);
+        own += key > limit || (key == limit && ties == ~0ull) ? w : 0ull;
+      });
+      if (ties != ~0ull && rank == 0 && threadIdx.x == 0) own += ties * mass_of(Key<T>::value(limit), q, sh.table);
+      all = sum_all(own);
     }
-    if (ties != ~0ull && rank == 0 && threadIdx.x == 0) own += ties * mass_of(Key<T>::value(limit), m, inv_tau);
-    all = sum_all(own);
-    const u64 want = max(1ull, u64(ceil(fmax(p, 0.0) * double(all))));     // (the first always stays)
+    const u64 want = min(all, max(1ull, u64(ceil(fmax(by.p, 0.0) * double(all)))));       // (the first always stays)
     u64 above;
-    const uint32_t key = select(true, min(want, all), above);
-    const u64 w = mass_of(Key<T>::value(key), m, inv_tau);
-    limit = key;
-    ties = (min(want, all) - above + w - 1) / w;
+    limit = select(true, want, above);
+    const u64 w = mass_of(Key<T>::value(limit), q, sh.table);
+    ties = (want - above + w - 1) / w;
   }
 
-  // ---- the draw
-  const u64 tie_w = ties == ~0ull ? 0ull : mass_of(Key<T>::value(limit), m, inv_tau);
-  const bool tie_in = tie_w >= least && tie_w > 0;
+  // the draw
+  const u64 tie_w = ties == ~0ull ? 0ull : mass_of(Key<T>::value(limit), q, sh.table);
+  const bool tie_in = tie_w >= by.least && tie_w > 0;
   auto stays = [&](float f, uint32_t key) -> u64 {            // mass of an element that stays whatever its place among equals
-    if (!(key > limit || (key == limit && ties == ~0ull))) return 0ull;
-    const u64 w = mass_of(f, m, inv_tau);
-    return w >= least ? w : 0ull;
+    const u64 w = mass_of(f, q, sh.table);
+    return w >= by.least && (key > limit || (key == limit && ties == ~0ull)) ? w : 0ull;
   };
   u64 sum = 0;
   uint32_t tied = 0;
-  for (int v = vlo + lane; v < vhi; v += 32) {
-    float f[VEC];
-    load(v, f);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const uint32_t key = Key<T>::of(f[j]);
-      sum += stays(f[j], key);
-      tied += tie_in && key == limit;
-    }
-  }
+  r.each(lane, [&](float z, int, int) {
+    const uint32_t key = Key<T>::of(z);
+    sum += stays(z, key);
+    tied += tie_in && key == limit;
+  });
   sum = warp_add64(sum);
   tied = __reduce_add_sync(0xffffffffu, tied);
   __syncthreads();
-  if (lane == 0) { wsum[warp] = sum; wcnt[warp] = tied; }
+  if (lane == 0) { sh.wsum[warp] = sum; sh.wcnt[warp] = tied; }
   __syncthreads();
   u64 csum = 0, ctied = 0;
-  for (int w = 0; w < kSampleWarps; ++w) { csum += wsum[w]; ctied += wcnt[w]; }
-  if (threadIdx.x == 0) { part[0] = csum; part[1] = ctied; }
+  for (int w = 0; w < nw; ++w) { csum += sh.wsum[w]; ctied += sh.wcnt[w]; }
+  if (threadIdx.x == 0) { sh.part[0] = csum; sh.part[1] = ctied; }
   everywhere();
   u64 before = 0, ties_before = 0, total = 0, seen = 0;
   for (int c = 0; c < C; ++c) {
-    const u64* q = C > 1 ? cluster_peer(part, c) : part;
-    const u64 t = q[1], kept = tie_in ? min(t, ties > seen ? ties - seen : 0ull) : 0ull;
-    const u64 x = q[0] + kept * tie_w;
+    const u64* o = C > 1 ? cluster_peer(sh.part, c) : sh.part;
+    const u64 t = o[1], kept = tie_in ? min(t, ties > seen ? ties - seen : 0ull) : 0ull;
+    const u64 x = o[0] + kept * tie_w;
     if (c < rank) { before += x; ties_before += t; }
     total += x;
     seen += t;
   }
   if (C > 1) cluster_sync_all();                              // a CTA's shared memory is read until here
-  double u = a.u64bit ? static_cast<const double*>(a.u)[row] : double(static_cast<const float*>(a.u)[row]);
-  u = u > 0.0 ? fmin(u, 1.0) : 0.0;
-  const u64 target = min(u64(u * double(total)), total - 1);
-  // this warp's mass
+  const u64 target = draw_target(a, row, total);
   for (int w = 0; w < warp; ++w) {
-    const u64 t = wcnt[w], kept = tie_in ? min(t, ties > ties_before ? ties - ties_before : 0ull) : 0ull;
-    before += wsum[w] + kept * tie_w;
+    const u64 t = sh.wcnt[w], kept = tie_in ? min(t, ties > ties_before ? ties - ties_before : 0ull) : 0ull;
+    before += sh.wsum[w] + kept * tie_w;
     ties_before += t;
   }
   {
     const u64 kept = tie_in ? min(u64(tied), ties > ties_before ? ties - ties_before : 0ull) : 0ull;
     if (target < before || target >= before + sum + kept * tie_w) return;
   }
-  for (int v0 = vlo; v0 < vhi; v0 += 32) {
+  for (int v0 = r.vlo; v0 < r.vhi; v0 += 32) {
     const int v = v0 + lane;
     float f[VEC];
     u64 w[VEC], own = 0;
     uint32_t eq = 0;
-    if (v < vhi) load(v, f);
+    if (v < r.vhi) unpack16<T>(r.load(v), f);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      const uint32_t key = v < vhi ? Key<T>::of(f[j]) : 0u;
-      w[j] = v < vhi ? stays(f[j], key) : 0ull;
-      eq += v < vhi && tie_in && key == limit;
+      const uint32_t key = v < r.vhi ? Key<T>::of(f[j]) : 0u;
+      w[j] = v < r.vhi ? stays(f[j], key) : 0ull;
+      eq += v < r.vhi && tie_in && key == limit;
     }
     uint32_t eq_incl = eq;
 #pragma unroll
@@ -355,18 +423,13 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
     u64 nth = ties_before + eq_incl - eq;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      if (v < vhi && tie_in && Key<T>::of(f[j]) == limit) {
+      if (v < r.vhi && tie_in && Key<T>::of(f[j]) == limit) {
         if (nth < ties) w[j] = tie_w;
         ++nth;
       }
       own += w[j];
     }
-    u64 incl = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 x = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += x;
-    }
+    const u64 incl = warp_scan64(own, lane);
     const unsigned hit = __ballot_sync(0xffffffffu, before + incl > target);
     if (hit) {
       if (lane == __ffs(hit) - 1) {
@@ -377,8 +440,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
           at += w[j];
           if (!done && at > target) {
             done = true;
-            a.tokens[row] = (long long)v * VEC - shift + j;
-            if (a.logprobs) a.logprobs[row] = float((f[j] == m ? 0.0 : (double(f[j]) - double(m)) * inv_tau) - log(double(total) / kMassOne));
+            write_token(a, row, v * VEC - r.shift + j, f[j], q, total);
           }
         }
       }
@@ -386,6 +448,250 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleArgs a) {
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
     ties_before += __shfl_sync(0xffffffffu, eq_incl, 31);
+  }
+}
+
+__constant__ double kSixteenths[16] = {1.0, 1.0442737824274138403, 1.0905077326652576592, 1.1387886347566916537, 1.1892071150027210667, 1.2418578120734840486,
+                                       1.2968395546510096659, 1.3542555469368927283, 1.4142135623730950488, 1.4768261459394993114, 1.5422108254079408236,
+                                       1.6104903319492543082, 1.6817928305074290861, 1.7562521603732994831, 1.8340080864093424635, 1.9152065613971472939};
+
+// A cluster holds a row in its shared memory.  Three ways lead to a token:
+//   no limit in the order  the masses of all tokens are summed by warp; the warp that holds u times the total goes over its tokens again
+//   a short list           a lower bound of what may stay is known: for top-k the k-th largest of the maxima of groups of tokens, for top-p the weight (1 - p) S / V
+//                          (all tokens below it together weigh less than (1 - p) S), for min-p itself.  The tokens from there on go to the first CTA's list, where
+//                          each is compared with each: its place in the order and the mass before it
+//   the general way        where that list would be long
+template <typename T>
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a) {
+  constexpr int VEC = kVec<T>;
+  extern __shared__ uint4 slice[];                            // this CTA's vectors of the row
+  __shared__ SampleShared sh;
+  __shared__ uint32_t all_groups[kSampleGroups];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int C = a.ctas, rank = C > 1 ? int(cluster_ctarank()) : 0;
+  const int row = blockIdx.x / C;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  auto everywhere = [&] {
+    if (C > 1) cluster_sync_all();
+    else __syncthreads();
+  };
+  SampleRow<T> r;
+  r.z = static_cast<const T*>(a.z) + row * a.ldz;
+  r.V = a.V;
+  r.shift = int(reinterpret_cast<uintptr_t>(r.z) & 15) / int(sizeof(T));
+  const int vecs = (a.V + r.shift + VEC - 1) / VEC, vcta = (vecs + C - 1) / C, vwarp = (vcta + nw - 1) / nw;
+  const int cend = min(vecs, (rank + 1) * vcta);
+  r.vlo = min(cend, rank * vcta + warp * vwarp);
+  r.vhi = min(cend, r.vlo + vwarp);
+  r.held = nullptr;
+  if (a.held) {                                               // (every thread reads the vectors that it fetches here)
+    r.held = slice - rank * vcta;
+    for (int v = r.vlo + lane; v < r.vhi; v += 32) {
+      if (r.whole(v)) copy_async16(smem_u32(slice + (v - rank * vcta)), r.z + v * VEC - r.shift);
+      else slice[v - rank * vcta] = r.fetch(v);
+    }
+  }
+  if (threadIdx.x < 16) sh.table[threadIdx.x] = kSixteenths[threadIdx.x];
+  if (threadIdx.x == 0) sh.count = 0;
+
+  double tau = a.tau ? double(a.tau[row]) : a.tau1;
+  Filters by;
+  by.p = a.top_p ? double(a.top_p[row]) : a.top_p1;
+  by.k = a.top_k ? a.top_k[row] : a.top_k1;
+  const double low = a.min_p ? double(a.min_p[row]) : a.min_p1;
+  if (!(tau > 0.0)) { by.k = 1; tau = 1.0; }
+  if (by.k == 1) by.p = 1.0;
+  if (by.k >= a.V) by.k = 0;
+  by.least = low > 0.0 ? u64(ceil(fmin(low, 1.0) * kMassOne)) : 0ull;
+  Weigh q;
+  q.k = 1.4426950408889634074 / tau;
+
+  // ---- maxima of groups of 32 / 2^per lanes, as many groups as top-k takes; the largest of them
+  int per = 0;
+  if (by.k > 1)
+    while (per < 5 && (nw * C << per) < by.k + by.k / 4 && (nw * C << (per + 1)) <= kSampleGroups) ++per;
+  const int own_groups = nw << per, groups = own_groups * C;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  {
+    float m = -INFINITY;
+    r.each(lane, [&](float z, int, int) { m = fmaxf(m, z); });
+    uint32_t key = Key<T>::of(m);
+    for (int o = 1; o < 32 >> per; o <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+    if ((lane & ((32 >> per) - 1)) == 0) sh.groups[(warp << per) + lane / (32 >> per)] = key;
+  }
+  everywhere();
+  uint32_t top = 0;
+  for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+    const uint32_t key = C > 1 ? cluster_peer(sh.groups, g / own_groups)[g % own_groups] : sh.groups[g];
+    all_groups[g] = key;
+    top = max(top, key);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) sh.wcnt[warp] = top;
+  __syncthreads();
+  for (int w = 0; w < nw; ++w) top = max(top, sh.wcnt[w]);
+  q.m = Key<T>::value(top);
+  q.md = double(q.m);
+  if (q.m == -INFINITY) {
+    if (rank == 0 && threadIdx.x == 0) {
+      a.tokens[row] = -1;
+      if (a.logprobs) a.logprobs[row] = -INFINITY;
+    }
+    if (C > 1) cluster_sync_all();                            // a CTA's shared memory is read until here
+    return;
+  }
+
+  const bool ordered = by.k > 0 || by.p < 1.0;                // a limit in the order
+  float bound = -INFINITY, from = -INFINITY;                  // what lies below does not stay for the limits in the order, or for min-p either
+  u64 mass = 0;
+  bool listed = false;
+  if ((ordered || by.least > 0) && a.held) {
+    if (by.k == 1) {
+      bound = q.m;
+      listed = true;
+    } else if (by.k > 0) {
+      if (by.k <= groups) {
+        // the k-th largest of the groups' maxima: the one with fewer than k above it, and k or more from it on
+        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+          const uint32_t key = all_groups[g];
+          int above = 0, same = 0;
+#pragma unroll 8
+          for (int o = 0; o < groups; ++o) {
+            above += all_groups[o] > key;
+            same += all_groups[o] == key;
+          }
+          if (above < by.k && by.k <= above + same) sh.found[0] = key;
+        }
+        __syncthreads();
+        bound = Key<T>::value(uint32_t(sh.found[0]));
+        listed = true;
+      }
+    } else if (by.p < 1.0) {
+      r.each(lane, [&](float z, int, int) { mass += mass_of(z, q, sh.table); });
+      mass = warp_add64(mass);
+      if (lane == 0) sh.wsum[warp] = mass;
+      __syncthreads();
+      mass = 0;
+      for (int w = 0; w < nw; ++w) mass += sh.wsum[w];
+      if (C > 1) {
+        if (threadIdx.x == 0) sh.part[0] = mass;
+        cluster_sync_all();
+        mass = 0;
+        for (int c = 0; c < C; ++c) mass += *cluster_peer(sh.part, c);
+      }
+      const double least = (1.0 - fmax(by.p, 0.0)) * double(mass) / kMassOne / double(a.V) * (1.0 - 1e-9) - 1e-13;
+      // (NaN, of infinite logits and temperature, becomes the largest: nothing else weighs)
+      if (least > 0.0) bound = fminf(__double2float_rd(q.md + tau * log(least) * (1.0 + 1e-12) - 1e-30), q.m);
+      listed = true;
+    }
+    // (with top-k and top-p the mass of the first k counts those that min-p leaves out)
+    if (low > 1e-12 && !(by.k > 0 && by.p < 1.0)) {
+      from = fmaxf(from, __double2float_rd(q.md + tau * log(fmin(low, 1.0) - 1e-13) * (1.0 + 1e-12) - 1e-30));
+      listed = listed || !ordered;
+    }
+    from = fminf(fmaxf(from, bound), q.m);
+  }
+  if (listed) {
+    // ---- the short list
+    u64* list = sh.mass;                                      // [256] key and token, then [256] weights and [256] masses
+    u64* to = C > 1 ? cluster_peer(list, 0) : list;
+    uint32_t* count = C > 1 ? cluster_peer(&sh.count, 0) : &sh.count;
+    for (int v = r.vlo + lane; v < r.vhi; v += 32) {
+      float f[VEC];
+      unpack16<T>(r.load(v), f);
+      uint32_t n = 0;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) n += f[j] >= from && f[j] != -INFINITY;
+      if (n) {
+        uint32_t at = atomicAdd(count, n);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (f[j] >= from && f[j] != -INFINITY) {
+            if (at < kSampleFew) to[at] = u64(Key<T>::of(f[j])) << 32 | uint32_t(v * VEC - r.shift + j);
+            ++at;
+          }
+      }
+    }
+    everywhere();
+    const int n = int(*count);
+    if (n <= kSampleFew) {
+      if (C > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        if (rank != 0) {
+          asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+          return;
+        }
+      }
+      if (threadIdx.x == 0) sh.found[1] = mass;
+      short_list<T>(a, row, q, by, n, list, sh);
+      if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+      return;
+    }
+    everywhere();                                             // (the list's place is used again)
+  }
+  if (ordered || !a.held) {
+    sample_general<T>(a, r, q, by, bound, mass, row, rank, sh);
+    return;
+  }
+
+  // ---- no limit in the order
+  u64 sum = 0;
+  r.each(lane, [&](float z, int, int) {
+    const u64 w = mass_of(z, q, sh.table);
+    sum += w >= by.least ? w : 0ull;
+  });
+  sum = warp_add64(sum);
+  if (lane == 0) sh.wsum[warp] = sum;
+  __syncthreads();
+  u64 csum = 0, before = 0, total = 0;
+  for (int w = 0; w < nw; ++w) {
+    if (w < warp) before += sh.wsum[w];
+    csum += sh.wsum[w];
+  }
+  if (C > 1) {
+    if (threadIdx.x == 0) sh.part[0] = csum;
+    cluster_sync_all();
+    for (int c = 0; c < C; ++c) {
+      const u64 x = *cluster_peer(sh.part, c);
+      if (c < rank) before += x;
+      total += x;
+    }
+    cluster_sync_all();                                       // a CTA's shared memory is read until here
+  } else {
+    total = csum;
+  }
+  const u64 target = draw_target(a, row, total);
+  if (target < before || target >= before + sum) return;
+  for (int v0 = r.vlo; v0 < r.vhi; v0 += 32) {
+    const int v = v0 + lane;
+    float f[VEC];
+    u64 w[VEC], own = 0;
+    if (v < r.vhi) unpack16<T>(r.load(v), f);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      w[j] = v < r.vhi ? mass_of(f[j], q, sh.table) : 0ull;
+      w[j] = w[j] >= by.least ? w[j] : 0ull;
+      own += w[j];
+    }
+    const u64 incl = warp_scan64(own, lane);
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > target);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) {
+        u64 at = before + incl - own;
+        bool done = false;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          at += w[j];
+          if (!done && at > target) {
+            done = true;
+            write_token(a, row, v * VEC - r.shift + j, f[j], q, total);
+          }
+        }
+      }
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
   }
 }
 
@@ -401,14 +707,27 @@ int lt_sample_tokens(int type, const void* z, long long ldz, const void* u, int 
   using namespace lt;
   if (type < 0 || type > 2 || rows < 0 || V < 1 || V > (1 << 19)) return -int(kStatusBadArgument);
   if (rows == 0) return 0;
-  int ctas = 1;
-  while (ctas < kSampleCluster && (long long)rows * ctas * 2 <= 2 * sm_count() && V / ctas >= 8192) ctas *= 2;
+  const int vecs = V / (type == kElemF32 ? 4 : 8) + 2;
+  int ctas = 1, threads = kSampleThreads;
+  while (ctas < kSampleCluster && (vecs / ctas + 1) * 16 > kSampleHoldTwo) ctas *= 2;
+  // few rows: more CTAs for each
+  while (ctas < kSampleCluster && (long long)rows * ctas * 2 <= sm_count() && V / ctas >= 8192) ctas *= 2;
+  while (threads > 128 && vecs / ctas + 1 <= threads / 2 * ((long long)rows * ctas > sm_count() ? 4 : 1)) threads /= 2;
   if ((long long)rows * ctas > 0x7fffffffll) return -int(kStatusBadArgument);
-  SampleArgs a{z, ldz, u, u64bit, tau, top_p, min_p, top_k, tau1, top_p1, min_p1, top_k1, rows, V, ctas, tokens, logprobs};
+  const bool held = (vecs / ctas + 1) * 16 <= kSampleHold;
+  const int smem = held ? (vecs / ctas + 1) * 16 : 0;
+  SampleArgs a{z, ldz, u, u64bit, tau, top_p, min_p, top_k, tau1, top_p1, min_p1, top_k1, rows, V, ctas, held, tokens, logprobs};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto kernel = type == kElemF32 ? sample_kernel<float> : type == kElemBf16 ? sample_kernel<__nv_bfloat16> : sample_kernel<__half>;
-  if (ctas > 1) LT_RETURN_IF_CUDA(launch_chained_clusters(kernel, rows * ctas, kSampleThreads, 0, ctas, st, a));
-  else LT_RETURN_IF_CUDA(launch_chained(kernel, rows, kSampleThreads, 0, st, a));
+  static OncePerDevice once;
+  if (once.pending()) {
+    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(sample_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleHold));
+    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(sample_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleHold));
+    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(sample_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleHold));
+    once.finish();
+  }
+  if (ctas > 1) LT_RETURN_IF_CUDA(launch_chained_clusters(kernel, rows * ctas, threads, smem, ctas, st, a));
+  else LT_RETURN_IF_CUDA(launch_chained(kernel, rows, threads, smem, st, a));
   return 0;
 }
 
