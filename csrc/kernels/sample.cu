@@ -17,9 +17,8 @@
 
 namespace lt {
 
-constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32, kSampleBins = 2048, kSampleCluster = 8;
-constexpr int kSampleHold = 192 * 1024;                       // bytes of a row that a CTA holds at most, and such that two CTAs share an SM
-constexpr int kSampleHoldTwo = 80 * 1024;
+constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32, kSampleBins = 1024, kSampleCluster = 8;
+constexpr int kSampleHold = 192 * 1024, kSampleHoldMany = 32 * 1024;   // bytes of a row that a CTA holds at most, and such that four CTAs share an SM
 constexpr int kSampleFew = 256;                               // tokens that are compared each with each
 constexpr int kSampleGroups = 512;                            // maxima of groups of tokens
 constexpr double kMassOne = 17592186044416.0;                 // 2^44
@@ -127,7 +126,9 @@ __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) { as
 
 struct SampleShared {
   uint32_t hist[kSampleBins];
-  u64 mass[kSampleBins];        // histograms of the general way; the short list's tokens and weights lie in the same place
+  // of the general way: sums over the cluster, and a CTA's histograms (counts, or 15 bits of the masses each; 64-bit atomics are loops)
+  u64 sums[kSampleBins];        // the short list's tokens and weights lie in the same place
+  uint32_t mid[kSampleBins], high[kSampleBins];
   u64 part[2];                  // what the other CTAs of the cluster read
   u64 wsum[kSampleWarps];
   uint32_t wcnt[kSampleWarps];
@@ -154,15 +155,14 @@ struct SampleRow {
     return pack16<T>(f);
   }
   __device__ __forceinline__ uint4 load(int v) const { return no_nan<T>(held ? held[v] : fetch(v)); }
-  // f(logit, vector, place in it) for this warp's logits
+  // f(logits, vector) for this warp's vectors
   template <class F>
   __device__ __forceinline__ void each(int lane, F f) const {
 #pragma unroll 2
     for (int v = vlo + lane; v < vhi; v += 32) {
       float x[VEC];
       unpack16<T>(load(v), x);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f(x[j], v, j);
+      f(x, v);
     }
   }
 };
@@ -191,7 +191,6 @@ __device__ __forceinline__ void short_list(const SampleArgs& a, int row, const W
   u64* mass_before = weight + kSampleFew;
   const int lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < n; i += blockDim.x) weight[i] = mass_of(Key<T>::value(uint32_t(list[i] >> 32)), q, sh.table);
-  if (threadIdx.x == 0) sh.found[0] = 0;
   __syncthreads();
   // a quarter of a warp to a token: its place in the order, and the mass of those in front of it
   for (int i0 = threadIdx.x >> 3; i0 - (lane >> 3) < n; i0 += blockDim.x >> 3) {
@@ -212,9 +211,8 @@ __device__ __forceinline__ void short_list(const SampleArgs& a, int row, const W
       before += __shfl_xor_sync(0xffffffffu, before, o);
     }
     if (i0 < n && (lane & 7) == 0) {
-      const bool in = by.k <= 0 || place < uint32_t(by.k);
-      mass_before[i] = in ? before : ~0ull;                   // (~0: does not stay)
-      if (in) atomicMax(&sh.found[0], before + weight[i]);    // in the end the mass of the first k; for top-p alone the list may lack tokens
+      mass_before[i] = by.k <= 0 || place < uint32_t(by.k) ? before : ~0ull;       // (~0: does not stay)
+      if (by.k > 0 && place + 1 == uint32_t(min(by.k, n))) sh.found[0] = before + weight[i];       // the mass of the first k
     }
   }
   __syncthreads();
@@ -275,36 +273,77 @@ __device__ __noinline__ void sample_general(const SampleArgs& a, const SampleRow
   u64 ties = ~0ull;
   const uint32_t key_lo = Key<T>::of(bound), key_hi = Key<T>::of(q.m);
   // The key at which the running sum over keys from the top (counts, or masses with the first `ties` of those at `limit`) reaches `want`, and the sum above it:
-  // the interval of the keys is cut into up to 2048 pieces until they are single keys.
+  // the interval of the keys is cut into up to 1024 pieces until they are single keys.
   auto select = [&](bool by_mass, u64 want, u64& above) {
     uint32_t lo = key_lo, hi = key_hi;
     above = 0;
     for (;;) {
-      const int width = 32 - __clz(int(hi - lo)), cut = max(0, width - 11);
+      const int width = 32 - __clz(int(hi - lo)), cut = max(0, width - 10);
       for (int i = threadIdx.x; i < kSampleBins; i += blockDim.x) {
-        sh.hist[i] = 0u;
-        sh.mass[i] = 0ull;
+        sh.hist[i] = sh.mid[i] = sh.high[i] = 0u;
       }
       __syncthreads();
-      r.each(lane, [&](float z, int, int) {
-        const uint32_t key = Key<T>::of(z);
-        if (z == -INFINITY || key < lo || key > hi) return;
-        if (!by_mass) atomicAdd(&sh.hist[(key - lo) >> cut], 1u);
-        else if (key > limit || (key == limit && ties == ~0ull)) {
-          const u64 w = mass_of(z, q, sh.table);
-          if (w) atomicAdd(&sh.mass[(key - lo) >> cut], w);
+      r.each(lane, [&](const float (&z)[VEC], int) {
+        uint32_t key[VEC];
+        bool in[VEC], any = false;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          key[j] = Key<T>::of(z[j]);
+          in[j] = z[j] != -INFINITY && key[j] >= lo && key[j] <= hi && (!by_mass || key[j] > limit || (key[j] == limit && ties == ~0ull));
+          any = any || in[j];
+        }
+        if (!any) return;
+        if (by_mass && cut > 0) {
+          u64 w[VEC];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) w[j] = mass_of(z[j], q, sh.table);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (in[j] && w[j]) {
+              const uint32_t at = (key[j] - lo) >> cut;
+              atomicAdd(&sh.hist[at], uint32_t(w[j]) & 0x7fffu);
+              atomicAdd(&sh.mid[at], uint32_t(w[j] >> 15) & 0x7fffu);
+              if (w[j] >> 30) atomicAdd(&sh.high[at], uint32_t(w[j] >> 30));
+            }
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (in[j]) atomicAdd(&sh.hist[(key[j] - lo) >> cut], 1u);
         }
       });
-      if (by_mass && ties != ~0ull && rank == 0 && threadIdx.x == 0 && limit >= lo && limit <= hi)
-        atomicAdd(&sh.mass[(limit - lo) >> cut], ties * mass_of(Key<T>::value(limit), q, sh.table));
       everywhere();
-      // bins from the top, 2048 / threads to a thread
+      // every CTA adds up its share of the bins over the cluster, and gives the sums to all
+      {
+        const int share = kSampleBins / C;
+        for (int i = threadIdx.x; i < share; i += blockDim.x) {
+          const int at = rank * share + i;
+          u64 v[kSampleCluster], sum = 0;
+#pragma unroll
+          for (int c = 0; c < kSampleCluster; ++c) {
+            v[c] = 0;
+            if (c < C) {
+              v[c] = C > 1 ? *cluster_peer(sh.hist + at, c) : sh.hist[at];
+              if (by_mass && cut > 0) v[c] += (u64(C > 1 ? *cluster_peer(sh.mid + at, c) : sh.mid[at]) << 15) + (u64(C > 1 ? *cluster_peer(sh.high + at, c) : sh.high[at]) << 30);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < kSampleCluster; ++c) sum += v[c];
+          if (by_mass) {
+            const bool at_limit = ties != ~0ull && limit >= lo && limit <= hi && (limit - lo) >> cut == uint32_t(at);
+            if (cut == 0 && sum) sum *= mass_of(Key<T>::value(lo + uint32_t(at)), q, sh.table);       // equal logits
+            if (at_limit) sum += ties * mass_of(Key<T>::value(limit), q, sh.table);
+          }
+#pragma unroll
+          for (int c = 0; c < kSampleCluster; ++c)
+            if (c < C) *(C > 1 ? cluster_peer(sh.sums + at, c) : sh.sums + at) = sum;
+        }
+      }
+      everywhere();
+      // bins from the top, 1024 / threads to a thread
       const int per = kSampleBins / int(blockDim.x);
       auto bin = [&](int i) {
         const int at = kSampleBins - 1 - (int(threadIdx.x) * per + i);
-        u64 v = 0;
-        for (int c = 0; c < C; ++c) v += by_mass ? (C > 1 ? *cluster_peer(sh.mass + at, c) : sh.mass[at]) : u64(C > 1 ? *cluster_peer(sh.hist + at, c) : sh.hist[at]);
-        return v;
+        return sh.sums[at];
       };
       u64 own = 0;
       for (int i = 0; i < per; ++i) own += bin(i);
@@ -322,7 +361,7 @@ __device__ __noinline__ void sample_general(const SampleArgs& a, const SampleRow
           }
           before += v;
         }
-      everywhere();
+      __syncthreads();
       lo += uint32_t(sh.found[0]) << cut;
       above = sh.found[1];
       __syncthreads();
@@ -333,7 +372,10 @@ __device__ __noinline__ void sample_general(const SampleArgs& a, const SampleRow
 
   if (by.k > 0 && by.k < a.V) {
     u64 have = 0;
-    r.each(lane, [&](float z, int, int) { have += z != -INFINITY; });
+    r.each(lane, [&](const float (&z)[VEC], int) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) have += z[j] != -INFINITY;
+    });
     if (sum_all(have) > u64(by.k)) {
       u64 above;
       limit = select(false, u64(by.k), above);
@@ -344,10 +386,13 @@ __device__ __noinline__ void sample_general(const SampleArgs& a, const SampleRow
     u64 all = mass;
     if (by.k > 0 || !r.held) {
       u64 own = 0;
-      r.each(lane, [&](float z, int, int) {
-        const uint32_t key = Key<T>::of(z);
-        const u64 w = mass_of(z, q, sh.table);
-        own += key > limit || (key == limit && ties == ~0ull) ? w : 0ull;
+      r.each(lane, [&](const float (&z)[VEC], int) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const uint32_t key = Key<T>::of(z[j]);
+          const u64 w = mass_of(z[j], q, sh.table);
+          own += key > limit || (key == limit && ties == ~0ull) ? w : 0ull;
+        }
       });
       if (ties != ~0ull && rank == 0 && threadIdx.x == 0) own += ties * mass_of(Key<T>::value(limit), q, sh.table);
       all = sum_all(own);
@@ -368,10 +413,17 @@ __device__ __noinline__ void sample_general(const SampleArgs& a, const SampleRow
   };
   u64 sum = 0;
   uint32_t tied = 0;
-  r.each(lane, [&](float z, int, int) {
-    const uint32_t key = Key<T>::of(z);
-    sum += stays(z, key);
-    tied += tie_in && key == limit;
+  r.each(lane, [&](const float (&z)[VEC], int) {
+    bool any = false;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const uint32_t key = Key<T>::of(z[j]);
+      any = any || key > limit || (key == limit && ties == ~0ull);
+      tied += tie_in && key == limit;
+    }
+    if (!any) return;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum += stays(z[j], Key<T>::of(z[j]));
   });
   sum = warp_add64(sum);
   tied = __reduce_add_sync(0xffffffffu, tied);
@@ -461,8 +513,8 @@ __constant__ double kSixteenths[16] = {1.0, 1.0442737824274138403, 1.09050773266
 //                          (all tokens below it together weigh less than (1 - p) S), for min-p itself.  The tokens from there on go to the first CTA's list, where
 //                          each is compared with each: its place in the order and the mass before it
 //   the general way        where that list would be long
-template <typename T>
-__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a) {
+template <typename T, int THREADS>                            // up to so many
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleArgs a) {
   constexpr int VEC = kVec<T>;
   extern __shared__ uint4 slice[];                            // this CTA's vectors of the row
   __shared__ SampleShared sh;
@@ -510,12 +562,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
   // ---- maxima of groups of 32 / 2^per lanes, as many groups as top-k takes; the largest of them
   int per = 0;
   if (by.k > 1)
-    while (per < 5 && (nw * C << per) < by.k + by.k / 4 && (nw * C << (per + 1)) <= kSampleGroups) ++per;
+    while (per < 5 && (nw * C << per) < 2 * by.k && (nw * C << (per + 1)) <= kSampleGroups) ++per;
   const int own_groups = nw << per, groups = own_groups * C;
   asm volatile("cp.async.wait_all;" ::: "memory");
   {
     float m = -INFINITY;
-    r.each(lane, [&](float z, int, int) { m = fmaxf(m, z); });
+    r.each(lane, [&](const float (&z)[VEC], int) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) m = fmaxf(m, z[j]);
+    });
     uint32_t key = Key<T>::of(m);
     for (int o = 1; o < 32 >> per; o <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
     if ((lane & ((32 >> per) - 1)) == 0) sh.groups[(warp << per) + lane / (32 >> per)] = key;
@@ -568,7 +623,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
         listed = true;
       }
     } else if (by.p < 1.0) {
-      r.each(lane, [&](float z, int, int) { mass += mass_of(z, q, sh.table); });
+      r.each(lane, [&](const float (&z)[VEC], int) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) mass += mass_of(z[j], q, sh.table);
+      });
       mass = warp_add64(mass);
       if (lane == 0) sh.wsum[warp] = mass;
       __syncthreads();
@@ -594,7 +652,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
   }
   if (listed) {
     // ---- the short list
-    u64* list = sh.mass;                                      // [256] key and token, then [256] weights and [256] masses
+    u64* list = sh.sums;                                      // [256] key and token, then [256] weights and [256] masses
     u64* to = C > 1 ? cluster_peer(list, 0) : list;
     uint32_t* count = C > 1 ? cluster_peer(&sh.count, 0) : &sh.count;
     for (int v = r.vlo + lane; v < r.vhi; v += 32) {
@@ -637,9 +695,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
 
   // ---- no limit in the order
   u64 sum = 0;
-  r.each(lane, [&](float z, int, int) {
-    const u64 w = mass_of(z, q, sh.table);
-    sum += w >= by.least ? w : 0ull;
+  r.each(lane, [&](const float (&z)[VEC], int) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const u64 w = mass_of(z[j], q, sh.table);
+      sum += w >= by.least ? w : 0ull;
+    }
   });
   sum = warp_add64(sum);
   if (lane == 0) sh.wsum[warp] = sum;
@@ -695,6 +756,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(SampleArgs a)
   }
 }
 
+template <typename T>
+int sample(const SampleArgs& a, int threads, int smem, cudaStream_t st) {
+  static OncePerDevice once;
+  if (once.pending()) {
+    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(sample_kernel<T, kSampleThreads / 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleHold));
+    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(sample_kernel<T, kSampleThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleHold));
+    once.finish();
+  }
+  auto kernel = threads > kSampleThreads / 2 ? sample_kernel<T, kSampleThreads> : sample_kernel<T, kSampleThreads / 2>;
+  if (a.ctas > 1) LT_RETURN_IF_CUDA(launch_chained_clusters(kernel, a.rows * a.ctas, threads, smem, a.ctas, st, a));
+  else LT_RETURN_IF_CUDA(launch_chained(kernel, a.rows, threads, smem, st, a));
+  return 0;
+}
+
 }  // namespace lt
 
 extern "C" {
@@ -708,27 +783,21 @@ int lt_sample_tokens(int type, const void* z, long long ldz, const void* u, int 
   if (type < 0 || type > 2 || rows < 0 || V < 1 || V > (1 << 19)) return -int(kStatusBadArgument);
   if (rows == 0) return 0;
   const int vecs = V / (type == kElemF32 ? 4 : 8) + 2;
-  int ctas = 1, threads = kSampleThreads;
-  while (ctas < kSampleCluster && (vecs / ctas + 1) * 16 > kSampleHoldTwo) ctas *= 2;
+  auto bytes = [&](int ctas) { return (vecs / ctas + 1) * 16; };
+  int ctas = 1;
+  while (ctas < kSampleCluster && bytes(ctas) > kSampleHoldMany) ctas *= 2;
   // few rows: more CTAs for each
   while (ctas < kSampleCluster && (long long)rows * ctas * 2 <= sm_count() && V / ctas >= 8192) ctas *= 2;
-  while (threads > 128 && vecs / ctas + 1 <= threads / 2 * ((long long)rows * ctas > sm_count() ? 4 : 1)) threads /= 2;
   if ((long long)rows * ctas > 0x7fffffffll) return -int(kStatusBadArgument);
-  const bool held = (vecs / ctas + 1) * 16 <= kSampleHold;
-  const int smem = held ? (vecs / ctas + 1) * 16 : 0;
+  const bool many = (long long)rows * ctas > 2 * sm_count(), small = many && bytes(ctas) <= kSampleHoldMany;
+  int threads = small ? kSampleThreads / 2 : kSampleThreads;
+  while (threads > 128 && vecs / ctas + 1 <= threads / 2 * (many ? 4 : 1)) threads /= 2;
+  const bool held = bytes(ctas) <= kSampleHold;
+  const int smem = held ? bytes(ctas) : 0;
   SampleArgs a{z, ldz, u, u64bit, tau, top_p, min_p, top_k, tau1, top_p1, min_p1, top_k1, rows, V, ctas, held, tokens, logprobs};
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto kernel = type == kElemF32 ? sample_kernel<float> : type == kElemBf16 ? sample_kernel<__nv_bfloat16> : sample_kernel<__half>;
-  static OncePerDevice once;
-  if (once.pending()) {
-    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(sample_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleHold));
-    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(sample_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleHold));
-    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(sample_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleHold));
-    once.finish();
-  }
-  if (ctas > 1) LT_RETURN_IF_CUDA(launch_chained_clusters(kernel, rows * ctas, threads, smem, ctas, st, a));
-  else LT_RETURN_IF_CUDA(launch_chained(kernel, rows, threads, smem, st, a));
-  return 0;
+  if (type == kElemF32) return sample<float>(a, threads, smem, static_cast<cudaStream_t>(stream));
+  if (type == kElemBf16) return sample<__nv_bfloat16>(a, threads, smem, static_cast<cudaStream_t>(stream));
+  return sample<__half>(a, threads, smem, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
