@@ -59,6 +59,20 @@ __device__ __forceinline__ uint4 pack16(const float (&f)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The largest element of 16 bytes (NaN only if there is nothing else).
+template <typename T> __device__ __forceinline__ float max16(uint4 u) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else if constexpr (__is_same(T, __nv_bfloat16)) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+}
 // The object at p's place in the shared memory of CTA `cta` of the cluster.
 template <typename P>
 __device__ __forceinline__ P* cluster_peer(P* p, uint32_t cta) {

@@ -166,23 +166,10 @@ __device__ __noinline__ float chained_p(const float2* entries, const LINK* link,
     }
   return n > 1 ? float(double(sum) * (1.0 / 4611686018427387904.0)) : p;
 }
-// -inf in every element, and the largest element of 16 bytes (NaN only if there is nothing else).
+// -inf in every element.
 template <typename T> __device__ __forceinline__ uint32_t minus_inf() { return 0xff800000u; }
 template <> __device__ __forceinline__ uint32_t minus_inf<__nv_bfloat16>() { return 0xff80ff80u; }
 template <> __device__ __forceinline__ uint32_t minus_inf<__half>() { return 0xfc00fc00u; }
-template <typename T> __device__ __forceinline__ float max16(uint4 u) {
-  if constexpr (sizeof(T) == 4) {
-    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
-  } else if constexpr (__is_same(T, __nv_bfloat16)) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
-  } else {
-    const __half2* h = reinterpret_cast<const __half2*>(&u);
-    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
-  }
-}
 // An 8-byte store to the place `dst` of CTA `cta`'s shared memory that is counted on the barrier `bar` there.
 __device__ __forceinline__ void send8(uint32_t dst, uint32_t bar, uint32_t cta, float2 v) {
   asm volatile(

@@ -67,26 +67,25 @@ typedef unsigned long long u64;
 
 // What the weights of a row go by.
 struct Weigh {
-  float m;                      // the largest logit
-  double md, k;                 // the same, and log2(e) / tau
+  float m, cut;                 // the largest logit; below the other one weights are nothing (-45.5 powers of two)
+  double md, k;                 // the largest logit, log2(e) / tau
 };
 // 2^44 times the weight of a logit, to the nearest whole number: 2^y with y = 16ths + r, |r| <= 1/32, the 16ths from a table, 2^r by the exponential series up to the
-// fifth power (the next term is below 2^-42).  Adding 256 to the weight leaves the whole number in the low bits of the sum.
+// fifth power (the next term is below 2^-42).  Adding 256 to the weight leaves the whole number in the low bits of the sum.  No branches: the compiler works at
+// several at once, each of which is a long chain.  Of an infinite largest logit only its equals weigh anything.
 __device__ __forceinline__ u64 mass_of(float z, const Weigh& q, const double* table) {
-  // (no branches: the compiler works at several at once, each of which is a long chain)
-  const double y = (double(z) - q.md) * q.k;
+  const double y = (double(z) - q.md) * q.k;                  // (the difference first: it is exact, and 0 for the largest)
   const double shifted = fma(y, 16.0, 6755399441055744.0);    // (1.5 2^52: the sum's low bits are 16 y rounded)
   const int n = __double2loint(shifted);
-  const double r = fma(shifted - 6755399441055744.0, -0.0625, y);
+  const double r = fma(shifted - 6755399441055744.0, -0.0625, y), t = table[n & 15];
   constexpr double L = 0.693147180559945309417232121458;
   double p = fma(r, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
   p = fma(p, r, L * L * L / 6.0);
   p = fma(p, r, L * L / 2.0);
   p = fma(p, r, L);
-  p = fma(p, r, 1.0) * table[n & 15];
-  p = __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p)) + 256.0;
-  const u64 w = y > -45.5 ? u64(__double_as_longlong(p)) & 0xfffffffffffffull : 0ull;
-  return z == q.m ? u64(kMassOne) : w;                        // (an infinite one too)
+  p = fma(fma(p, r, 1.0), __hiloint2double(__double2hiint(t) + (n & ~15) * 65536, __double2loint(t)), 256.0);
+  const u64 w = u64(__double_as_longlong(p)) & 0xfffffffffffffull;
+  return z >= q.cut ? q.m == INFINITY ? u64(kMassOne) : w : 0ull;
 }
 __device__ __forceinline__ u64 warp_add64(u64 v) {
 #pragma unroll
@@ -134,6 +133,10 @@ struct SampleShared {
   uint32_t wcnt[kSampleWarps];
   u64 found[2];
   double table[16];
+  double k, top_p, low;         // log2(e) / tau and limits of the row
+  u64 least;
+  float from[2];                // what lies below does not stay for the limits in the order, or for min-p either
+  double tau;
   uint32_t groups[kSampleGroups];
   uint32_t count;               // of the short list (the first CTA's)
 };
@@ -154,7 +157,8 @@ struct SampleRow {
     for (int j = 0; j < VEC; ++j) f[j] = lo + j >= 0 && lo + j < V ? to_f32(z[lo + j]) : -INFINITY;
     return pack16<T>(f);
   }
-  __device__ __forceinline__ uint4 load(int v) const { return no_nan<T>(held ? held[v] : fetch(v)); }
+  __device__ __forceinline__ uint4 raw(int v) const { return held ? held[v] : fetch(v); }
+  __device__ __forceinline__ uint4 load(int v) const { return no_nan<T>(raw(v)); }
   // f(logits, vector) for this warp's vectors
   template <class F>
   __device__ __forceinline__ void each(int lane, F f) const {
@@ -547,17 +551,21 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
   if (threadIdx.x < 16) sh.table[threadIdx.x] = kSixteenths[threadIdx.x];
   if (threadIdx.x == 0) sh.count = 0;
 
-  double tau = a.tau ? double(a.tau[row]) : a.tau1;
   Filters by;
-  by.p = a.top_p ? double(a.top_p[row]) : a.top_p1;
   by.k = a.top_k ? a.top_k[row] : a.top_k1;
-  const double low = a.min_p ? double(a.min_p[row]) : a.min_p1;
-  if (!(tau > 0.0)) { by.k = 1; tau = 1.0; }
-  if (by.k == 1) by.p = 1.0;
-  if (by.k >= a.V) by.k = 0;
-  by.least = low > 0.0 ? u64(ceil(fmin(low, 1.0) * kMassOne)) : 0ull;
-  Weigh q;
-  q.k = 1.4426950408889634074 / tau;
+  {
+    const double tau = a.tau ? double(a.tau[row]) : a.tau1;
+    if (!(tau > 0.0)) by.k = 1;
+    if (by.k >= a.V && a.V > 1) by.k = 0;
+    if (threadIdx.x == 32) {                                  // (divisions of 64 bits are long: one thread does them for all)
+      const double low = a.min_p ? double(a.min_p[row]) : a.min_p1;
+      sh.top_p = by.k == 1 ? 1.0 : a.top_p ? double(a.top_p[row]) : a.top_p1;
+      sh.low = low;
+      sh.tau = tau > 0.0 ? tau : 1.0;
+      sh.k = fmin(1.4426950408889634074 / sh.tau, 1e300);
+      sh.least = low > 0.0 ? u64(ceil(fmin(low, 1.0) * kMassOne)) : 0ull;
+    }
+  }
 
   // ---- maxima of groups of 32 / 2^per lanes, as many groups as top-k takes; the largest of them
   int per = 0;
@@ -567,10 +575,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
   asm volatile("cp.async.wait_all;" ::: "memory");
   {
     float m = -INFINITY;
-    r.each(lane, [&](const float (&z)[VEC], int) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) m = fmaxf(m, z[j]);
-    });
+#pragma unroll 4
+    for (int v = r.vlo + lane; v < r.vhi; v += 32) m = fmaxf(m, max16<T>(r.raw(v)));
     uint32_t key = Key<T>::of(m);
     for (int o = 1; o < 32 >> per; o <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
     if ((lane & ((32 >> per) - 1)) == 0) sh.groups[(warp << per) + lane / (32 >> per)] = key;
@@ -586,8 +592,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
   if (lane == 0) sh.wcnt[warp] = top;
   __syncthreads();
   for (int w = 0; w < nw; ++w) top = max(top, sh.wcnt[w]);
+  Weigh q;
   q.m = Key<T>::value(top);
+  q.k = sh.k;
   q.md = double(q.m);
+  by.p = sh.top_p;
+  by.least = sh.least;
   if (q.m == -INFINITY) {
     if (rank == 0 && threadIdx.x == 0) {
       a.tokens[row] = -1;
@@ -597,6 +607,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
     return;
   }
 
+  // (infinite factors, of tiny or huge temperatures and logits, leave the largest alone, or all that are finite, in their places)
+  {
+    const double cut = q.md - 45.5 / q.k;
+    q.cut = cut == cut ? fminf(__double2float_ru(cut), q.m) : q.m;
+    if (q.m == INFINITY) q.cut = q.m;
+    q.cut = fmaxf(q.cut, -3.4028234663852886e38f);
+  }
   const bool ordered = by.k > 0 || by.p < 1.0;                // a limit in the order
   float bound = -INFINITY, from = -INFINITY;                  // what lies below does not stay for the limits in the order, or for min-p either
   u64 mass = 0;
@@ -638,15 +655,22 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
         mass = 0;
         for (int c = 0; c < C; ++c) mass += *cluster_peer(sh.part, c);
       }
-      const double least = (1.0 - fmax(by.p, 0.0)) * double(mass) / kMassOne / double(a.V) * (1.0 - 1e-9) - 1e-13;
       // (NaN, of infinite logits and temperature, becomes the largest: nothing else weighs)
-      if (least > 0.0) bound = fminf(__double2float_rd(q.md + tau * log(least) * (1.0 + 1e-12) - 1e-30), q.m);
+      if (threadIdx.x == 0) {
+        const double least = (1.0 - fmax(by.p, 0.0)) * double(mass) / kMassOne / double(a.V) * (1.0 - 1e-9) - 1e-13;
+        sh.from[0] = least > 0.0 ? fminf(__double2float_rd(q.md + sh.tau * log(least) * (1.0 + 1e-12) - 1e-30), q.m) : -INFINITY;
+      }
+      __syncthreads();
+      bound = sh.from[0];
       listed = true;
     }
     // (with top-k and top-p the mass of the first k counts those that min-p leaves out)
-    if (low > 1e-12 && !(by.k > 0 && by.p < 1.0)) {
-      from = fmaxf(from, __double2float_rd(q.md + tau * log(fmin(low, 1.0) - 1e-13) * (1.0 + 1e-12) - 1e-30));
-      listed = listed || !ordered;
+    if (by.least > 0 && !(by.k > 0 && by.p < 1.0)) {
+      if (threadIdx.x == 0)
+        sh.from[1] = sh.low > 1e-12 ? __double2float_rd(q.md + sh.tau * log(fmin(sh.low, 1.0) - 1e-13) * (1.0 + 1e-12) - 1e-30) : -INFINITY;
+      __syncthreads();
+      from = sh.from[1];
+      listed = listed || (!ordered && sh.low > 1e-12);
     }
     from = fminf(fmaxf(from, bound), q.m);
   }
@@ -656,8 +680,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
     u64* to = C > 1 ? cluster_peer(list, 0) : list;
     uint32_t* count = C > 1 ? cluster_peer(&sh.count, 0) : &sh.count;
     for (int v = r.vlo + lane; v < r.vhi; v += 32) {
+      const uint4 u = r.raw(v);
+      const float largest = max16<T>(u);
+      if (!(largest >= from) || largest == -INFINITY) continue;
       float f[VEC];
-      unpack16<T>(r.load(v), f);
+      unpack16<T>(no_nan<T>(u), f);
       uint32_t n = 0;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) n += f[j] >= from && f[j] != -INFINITY;
@@ -695,13 +722,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
 
   // ---- no limit in the order
   u64 sum = 0;
-  r.each(lane, [&](const float (&z)[VEC], int) {
+  if (by.least == 0)
+    r.each(lane, [&](const float (&z)[VEC], int) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const u64 w = mass_of(z[j], q, sh.table);
-      sum += w >= by.least ? w : 0ull;
-    }
-  });
+      for (int j = 0; j < VEC; ++j) sum += mass_of(z[j], q, sh.table);
+    });
+  else
+    r.each(lane, [&](const float (&z)[VEC], int) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const u64 w = mass_of(z[j], q, sh.table);
+        sum += w >= by.least ? w : 0ull;
+      }
+    });
   sum = warp_add64(sum);
   if (lane == 0) sh.wsum[warp] = sum;
   __syncthreads();
