@@ -18,7 +18,7 @@
 namespace lt {
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32, kSampleBins = 1024, kSampleCluster = 8;
-constexpr int kSampleHold = 192 * 1024, kSampleHoldMany = 32 * 1024;   // bytes of a row that a CTA holds at most, and such that four CTAs share an SM
+constexpr int kSampleHold = 80 * 1024;                        // bytes of a row that a CTA holds at most: two share an SM
 constexpr int kSampleFew = 256;                               // tokens that are compared each with each
 constexpr int kSampleGroups = 512;                            // maxima of groups of tokens
 constexpr double kMassOne = 17592186044416.0;                 // 2^44
@@ -245,7 +245,7 @@ __device__ __forceinline__ void short_list(const SampleArgs& a, int row, const W
 }
 
 // The general way, for filters that leave many tokens: every step goes over the row again (in L2).
-// `bound`: tokens below it do not stay for top-k and top-p.  mass: that of all tokens, if top-p is the only limit and the row is held.
+// `bound`: tokens below it do not stay for top-k and top-p.  mass: that of all tokens, if top-p is the only limit.
 template <typename T>
 __device__ __noinline__ void sample_general(const SampleArgs& a, const SampleRow<T>& r, const Weigh& q, const Filters& by, float bound, u64 mass, int row, int rank,
                                             SampleShared& sh) {
@@ -388,7 +388,7 @@ __device__ __noinline__ void sample_general(const SampleArgs& a, const SampleRow
   }
   if (by.p < 1.0) {
     u64 all = mass;
-    if (by.k > 0 || !r.held) {
+    if (by.k > 0) {
       u64 own = 0;
       r.each(lane, [&](const float (&z)[VEC], int) {
 #pragma unroll
@@ -511,7 +511,7 @@ __constant__ double kSixteenths[16] = {1.0, 1.0442737824274138403, 1.09050773266
                                        1.2968395546510096659, 1.3542555469368927283, 1.4142135623730950488, 1.4768261459394993114, 1.5422108254079408236,
                                        1.6104903319492543082, 1.6817928305074290861, 1.7562521603732994831, 1.8340080864093424635, 1.9152065613971472939};
 
-// A cluster holds a row in its shared memory.  Three ways lead to a token:
+// A cluster takes a row, and holds it in its shared memory if it fits.  Three ways lead to a token:
 //   no limit in the order  the masses of all tokens are summed by warp; the warp that holds u times the total goes over its tokens again
 //   a short list           a lower bound of what may stay is known: for top-k the k-th largest of the maxima of groups of tokens, for top-p the weight (1 - p) S / V
 //                          (all tokens below it together weigh less than (1 - p) S), for min-p itself.  The tokens from there on go to the first CTA's list, where
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
   float bound = -INFINITY, from = -INFINITY;                  // what lies below does not stay for the limits in the order, or for min-p either
   u64 mass = 0;
   bool listed = false;
-  if ((ordered || by.least > 0) && a.held) {
+  if (ordered || by.least > 0) {
     if (by.k == 1) {
       bound = q.m;
       listed = true;
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleA
     }
     everywhere();                                             // (the list's place is used again)
   }
-  if (ordered || !a.held) {
+  if (ordered) {
     sample_general<T>(a, r, q, by, bound, mass, row, rank, sh);
     return;
   }
@@ -816,17 +816,16 @@ int lt_sample_tokens(int type, const void* z, long long ldz, const void* u, int 
   if (type < 0 || type > 2 || rows < 0 || V < 1 || V > (1 << 19)) return -int(kStatusBadArgument);
   if (rows == 0) return 0;
   const int vecs = V / (type == kElemF32 ? 4 : 8) + 2;
-  auto bytes = [&](int ctas) { return (vecs / ctas + 1) * 16; };
-  int ctas = 1;
-  while (ctas < kSampleCluster && bytes(ctas) > kSampleHoldMany) ctas *= 2;
-  // few rows: more CTAs for each
-  while (ctas < kSampleCluster && (long long)rows * ctas * 2 <= sm_count() && V / ctas >= 8192) ctas *= 2;
+  auto bytes = [&](int n) { return (vecs / n + 1) * 16; };
+  // as many CTAs as hold the row, and for few rows as many as two an SM with 8192 tokens or more each
+  int ctas = 1, threads = kSampleThreads;
+  while (ctas < kSampleCluster && bytes(ctas) > kSampleHold) ctas *= 2;
+  while (ctas < kSampleCluster && (long long)rows * ctas * 2 <= 2 * sm_count() && V / ctas >= 8192) ctas *= 2;
   if ((long long)rows * ctas > 0x7fffffffll) return -int(kStatusBadArgument);
-  const bool many = (long long)rows * ctas > 2 * sm_count(), small = many && bytes(ctas) <= kSampleHoldMany;
-  int threads = small ? kSampleThreads / 2 : kSampleThreads;
-  while (threads > 128 && vecs / ctas + 1 <= threads / 2 * (many ? 4 : 1)) threads /= 2;
-  const bool held = bytes(ctas) <= kSampleHold;
-  const int smem = held ? bytes(ctas) : 0;
+  const bool many = (long long)rows * ctas > 2 * sm_count();
+  while (threads > (many && bytes(ctas) > 48 * 1024 ? 256 : 128) && (many || vecs / ctas + 1 <= threads / 2)) threads /= 2;
+  const bool held = (vecs / ctas + 1) * 16 <= kSampleHold;
+  const int smem = held ? (vecs / ctas + 1) * 16 : 0;
   SampleArgs a{z, ldz, u, u64bit, tau, top_p, min_p, top_k, tau1, top_p1, min_p1, top_k1, rows, V, ctas, held, tokens, logprobs};
   if (type == kElemF32) return sample<float>(a, threads, smem, static_cast<cudaStream_t>(stream));
   if (type == kElemBf16) return sample<__nv_bfloat16>(a, threads, smem, static_cast<cudaStream_t>(stream));
