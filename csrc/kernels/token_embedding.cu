@@ -6,12 +6,15 @@
 // once, so that results do not change from run to run (bf16 atomics, as in lt_embedding_bwd, round every addition and add in
 // any order).
 //
-// The gradient takes three steps:
-//   sort   one cluster of CTAs sorts (token, place) by token with a stable counting sort of 9 bits a pass: within a token the places stay in order
-//   sum    a CTA takes `tile` neighbours of the sorted list and adds their rows; what begins and ends inside goes to the table, what goes
-//          on in a neighbouring tile to a workspace
-//   join   adds the pieces of a token that several tiles share, in order
+// The gradient takes four launches:
+//   sort   one cluster of CTAs sorts (token, place) by token with a stable counting sort of up to 9 bits a pass: within a token the places stay in order
+//   clear  the table becomes zero, beside the sort
+//   sum    a CTA takes `tile` neighbours of the sorted list and adds their rows.  A token with up to 64 places is summed where it begins; of one with more,
+//          each tile leaves its piece in a workspace
+//   join   adds the pieces, in order
 #include "lt_cuda.h"
+
+#include <algorithm>
 
 #include "common/elem.cuh"
 #include "common/host.h"
@@ -19,127 +22,158 @@
 
 namespace lt {
 
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBits = 9, kSortBins = 1 << kSortBits;
-constexpr int kMaxTile = 256;
+constexpr int kSortThreads = 1024, kSortBits = 9, kSortBins = 1 << kSortBits;
+constexpr int kMaxTile = 64, kShort = 64;                     // places of a token that are summed at once
+constexpr int kJoinTiles = 4;                                 // tiles that a CTA looks through
 
 // ---------------------------------------------------------------------------------------------- forward
-template <typename T, typename IDX, int VEC>
-__global__ void __launch_bounds__(256) token_embedding_fwd_kernel(const IDX* idx, const T* table, T* out, long long n, int D, int V, float scale) {
+// 2^log threads to a row, each with every 2^log-th of its vectors, of four rows at once: a row alone keeps an SM waiting most of the time.
+template <typename T, typename IDX>
+__global__ void __launch_bounds__(256) token_embedding_fwd_kernel(const IDX* idx, const T* table, T* out, long long n, int D, int V, float scale, int log) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int U = 4;
-  const int vpr = D / VEC;
+  constexpr int VEC = kVec<T>, R = 4, U = 2;
+  const int rows = 256 >> log;
+  const long long first = (long long)blockIdx.x * (rows * R) + (threadIdx.x >> log);
+  const T* from[R];
+  bool in[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const long long row = first + r * rows, tok = row < n ? (long long)idx[row] : -1;
+    in[r] = tok >= 0 && tok < V;
+    from[r] = table + (in[r] ? tok : 0) * D;
+  }
+  const int step = VEC << log;
+  for (int c0 = (threadIdx.x & ((1 << log) - 1)) * VEC; c0 < D; c0 += U * step) {
+    uint4 u[R][U];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (in[r] && c0 + k * step < D) u[r][k] = *reinterpret_cast<const uint4*>(from[r] + c0 + k * step);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (first + r * rows >= n || c0 + k * step >= D) continue;
+        float f[VEC];
+        unpack16<T>(u[r][k], f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] = in[r] ? f[j] * scale : 0.f;
+        *reinterpret_cast<uint4*>(out + (first + r * rows) * D + c0 + k * step) = pack16<T>(f);
+      }
+  }
+}
+
+// Rows that do not begin at 16 bytes: elements of the result in their order, eight to a thread, so that warps write whole lines.
+template <typename T, typename IDX>
+__global__ void __launch_bounds__(256) token_embedding_flat_kernel(const IDX* idx, const T* table, T* out, long long n, int D, int V, float scale, float inv) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int U = 8;
   const long long first = (long long)blockIdx.x * (256 * U);
-  const long long row0 = first / vpr;
-  const int rem = int(first - row0 * vpr);
-  long long row[U], tok[U];
-  int col[U];
+  const long long row0 = first / D;
+  const int off = int(first - row0 * D);
+  long long from[U];
 #pragma unroll
   for (int k = 0; k < U; ++k) {
-    const unsigned at = unsigned(rem + k * 256 + int(threadIdx.x));
-    row[k] = row0 + at / unsigned(vpr);
-    col[k] = int(at % unsigned(vpr)) * VEC;
-    tok[k] = row[k] < n ? (long long)idx[row[k]] : -1;
+    const unsigned at = unsigned(off) + k * 256 + threadIdx.x;
+    unsigned q = unsigned(__uint2float_rz(at) * inv);         // at / D, or one or two off
+    while (q * (unsigned long long)D > at) --q;
+    while ((q + 1ull) * D <= at) ++q;
+    const long long row = row0 + q, tok = row < n ? (long long)idx[row] : -1;
+    from[k] = tok >= 0 && tok < V ? tok * D + (at - q * D) : -1;
   }
-  if constexpr (VEC == 1) {
+  float f[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k)
-      if (row[k] < n) out[row[k] * D + col[k]] = from_f32<T>(tok[k] >= 0 && tok[k] < V ? to_f32(table[tok[k] * D + col[k]]) * scale : 0.f);
-  } else {
-    uint4 u[U];
+  for (int k = 0; k < U; ++k) f[k] = from[k] >= 0 ? to_f32(table[from[k]]) * scale : 0.f;
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      u[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (tok[k] >= 0 && tok[k] < V) u[k] = *reinterpret_cast<const uint4*>(table + tok[k] * D + col[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (row[k] >= n) continue;
-      float f[VEC];
-      unpack16<T>(u[k], f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] = tok[k] >= 0 && tok[k] < V ? f[j] * scale : 0.f;
-      *reinterpret_cast<uint4*>(out + row[k] * D + col[k]) = pack16<T>(f);
-    }
-  }
+  for (int k = 0; k < U; ++k)
+    if (first + k * 256 + threadIdx.x < n * D) out[first + k * 256 + threadIdx.x] = from_f32<T>(f[k]);
 }
 
 // ---------------------------------------------------------------------------------------------- sort
 // Sorted list of (token, place); tokens without a gradient get V and come last.  One cluster; every CTA holds the list's next n / CTAs entries, every warp
 // the next part of those, so that entries of one digit stay in order.  Lists between two passes lie in global memory (in L2).
 template <typename IDX>
-__global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const IDX* idx, int n, int V, long long pad, uint2* buf0, uint2* buf1, int passes, int ctas) {
+__global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const IDX* idx, int n, int V, long long pad, uint2* buf0, uint2* buf1, int passes, int bits, int ctas) {
   extern __shared__ uint32_t sort_smem[];
-  uint32_t(*cnt)[kSortBins] = reinterpret_cast<uint32_t(*)[kSortBins]>(sort_smem);        // [warp][digit]: how many, then places within the CTA
-  uint32_t* total = sort_smem + kSortWarps * kSortBins;
-  uint32_t* start = total + kSortBins;
   __shared__ uint32_t scan[32];
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();                                    // (behind the wait: what starts now may write at once)
+  const int bins = 1 << bits, nt = blockDim.x, nw = nt >> 5;
+  uint32_t* cnt = sort_smem;                                  // [warp][digit]: how many, then places within the CTA
+  uint32_t* total = sort_smem + nw * bins;
+  uint32_t* start = total + bins;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = int(cluster_ctarank());
+  const int rank = ctas > 1 ? int(cluster_ctarank()) : 0;
   const int part = (n + ctas - 1) / ctas;
   const int lo = min(n, rank * part), hi = min(n, lo + part);
-  const int wpart = ((hi - lo + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+  const int wpart = ((hi - lo + nw - 1) / nw + 31) / 32 * 32;
   const int wlo = min(hi, lo + warp * wpart), whi = min(hi, wlo + wpart);
   for (int p = 0; p < passes; ++p) {
     const uint2* src = (p & 1) ? buf0 : buf1;
     uint2* dst = (p & 1) ? buf1 : buf0;
-    const int shift = p * kSortBits;
+    const int shift = p * bits;
     auto entry = [&](int i) {
       if (p > 0) return __ldcg(src + i);
       const long long t = (long long)idx[i];
       return make_uint2(t >= 0 && t < V && t != pad ? uint32_t(t) : uint32_t(V), uint32_t(i));
     };
-    for (int i = threadIdx.x; i < kSortWarps * kSortBins; i += kSortThreads) sort_smem[i] = 0u;
+    for (int i = threadIdx.x; i < nw * bins; i += nt) cnt[i] = 0u;
     __syncthreads();
-    for (int i = wlo + lane; i < whi; i += 32) atomicAdd(&cnt[warp][(entry(i).x >> shift) & (kSortBins - 1)], 1u);
+#pragma unroll 4
+    for (int i = wlo + lane; i < whi; i += 32) atomicAdd(&cnt[warp * bins + ((entry(i).x >> shift) & (bins - 1))], 1u);
     __syncthreads();
-    uint32_t mine = 0;
-    if (threadIdx.x < kSortBins) {
+    for (int d = threadIdx.x; d < bins; d += nt) {
+      uint32_t sum = 0;
 #pragma unroll 8
-      for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = cnt[w][threadIdx.x];
-        cnt[w][threadIdx.x] = mine;
-        mine += c;
+      for (int w = 0; w < nw; ++w) {
+        const uint32_t c = cnt[w * bins + d];
+        cnt[w * bins + d] = sum;
+        sum += c;
       }
-      total[threadIdx.x] = mine;
+      total[d] = sum;
     }
     if (ctas > 1) cluster_sync_all();
     else __syncthreads();
-    uint32_t before = 0, all = 0;
-    if (threadIdx.x < kSortBins) {
-      for (int c = 0; c < ctas; ++c) {
-        const uint32_t v = ctas > 1 ? *cluster_peer(total + threadIdx.x, c) : mine;
-        before += c < rank ? v : 0u;
-        all += v;
-      }
-    }
-    uint32_t incl = all;
+    uint32_t carry = 0;                                       // entries of the digits before
+    for (int d0 = 0; d0 < bins; d0 += nt) {
+      const int d = d0 + threadIdx.x;
+      uint32_t before = 0, all = 0;
+      if (d < bins)
+        for (int c = 0; c < ctas; ++c) {
+          const uint32_t v = ctas > 1 ? *cluster_peer(total + d, c) : total[d];
+          before += c < rank ? v : 0u;
+          all += v;
+        }
+      uint32_t incl = all;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      uint32_t base = carry + incl - all + before;
+      for (int w = 0; w < nw; ++w) {
+        if (w < warp) base += scan[w];
+        carry += scan[w];
+      }
+      if (d < bins) start[d] = base;
+      __syncthreads();
     }
-    if (lane == 31) scan[warp] = incl;
-    __syncthreads();
-    if (threadIdx.x < kSortBins) {
-      uint32_t base = incl - all + before;
-      for (int w = 0; w < warp; ++w) base += scan[w];
-      start[threadIdx.x] = base;
-    }
-    __syncthreads();
     for (int i0 = wlo; i0 < whi; i0 += 32) {
       const int i = i0 + lane;
       const unsigned live = __ballot_sync(0xffffffffu, i < whi);
       if (i < whi) {
         const uint2 e = entry(i);
-        const uint32_t d = (e.x >> shift) & (kSortBins - 1);
+        const uint32_t d = (e.x >> shift) & (bins - 1);
         const unsigned peers = __match_any_sync(live, d);
-        const uint32_t at = start[d] + cnt[warp][d];
+        const uint32_t at = start[d] + cnt[warp * bins + d];
         dst[at + __popc(peers & ((1u << lane) - 1u))] = e;
         __syncwarp(live);
-        if ((peers >> lane) == 1u) cnt[warp][d] += __popc(peers);         // the last of its digit
+        if ((peers >> lane) == 1u) cnt[warp * bins + d] += __popc(peers);         // the last of its digit
       }
       __syncwarp();
     }
@@ -148,142 +182,259 @@ __global__ void __launch_bounds__(kSortThreads) embed_sort_kernel(const IDX* idx
   }
 }
 
+// Zeros, 16 KB a CTA (1.05 GB: 65536 CTAs 7.4 TB/s, a few that stay 6.2).  Starts when the sort has begun (everything before that is complete) and runs beside it; the
+// last CTA waits for the sort's end, so that the end of this launch is the end of both.
+constexpr int kClear = 16384;
+__global__ void __launch_bounds__(512) embed_clear_kernel(unsigned char* grad, long long bytes) {
+  pdl_launch_dependents();
+  const long long at = (long long)blockIdx.x * kClear;
+  const int size = int(min((long long)kClear, bytes - at));
+  if ((reinterpret_cast<uintptr_t>(grad) & 15) == 0) {
+    for (int i = threadIdx.x; i < size / 16; i += 512) reinterpret_cast<uint4*>(grad + at)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (threadIdx.x < size % 16) grad[at + size / 16 * 16 + threadIdx.x] = 0;
+  } else {
+    for (int i = threadIdx.x; i < size; i += 512) grad[at + i] = 0;
+  }
+  if (blockIdx.x == gridDim.x - 1) pdl_wait();
+}
+
 // ---------------------------------------------------------------------------------------------- sum
-template <typename T, int VEC>
-__device__ __forceinline__ void store_row(T* p, const float (&acc)[VEC], float scale) {
-  if constexpr (VEC == 1) *p = from_f32<T>(acc[0] * scale);
-  else {
-    float f[VEC];
+// Columns of a thread: a vector of 16 bytes, or (where rows do not begin at 16 bytes) four that lie a CTA's width apart.
+template <typename T, bool WIDE> constexpr int kCols = WIDE ? kVec<T> : 4;
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store_row(T* row, int c, int D, const float (&acc)[kCols<T, WIDE>], float scale) {
+  if constexpr (WIDE) {
+    float f[kCols<T, WIDE>];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = acc[j] * scale;
-    *reinterpret_cast<uint4*>(p) = pack16<T>(f);
+    for (int j = 0; j < kCols<T, WIDE>; ++j) f[j] = acc[j] * scale;
+    *reinterpret_cast<uint4*>(row + c) = pack16<T>(f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j * int(blockDim.x) < D) row[c + j * blockDim.x] = from_f32<T>(acc[j] * scale);
   }
 }
 
-// part[tile][0]: the sum of a segment that began before the tile; part[tile][1]: of one that begins in it and goes on behind it.
-template <typename T, int VEC>
+// How many of the entries at s[from], s[from + dir], ... have the key, up to `most`; the whole warp.
+__device__ __forceinline__ int run_length(const uint2* s, int from, int dir, uint32_t key, int most, int lane) {
+  int n = 0;
+  while (n < most) {
+    const bool same = n + lane < most && s[from + dir * (n + lane)].x == key;
+    const unsigned m = __ballot_sync(0xffffffffu, same);
+    if (m != 0xffffffffu) return n + __ffs(~m) - 1;
+    n += 32;
+  }
+  return n;
+}
+
+// part[tile][0]: the piece of a long segment that began before the tile; part[tile][1]: of one that begins in it.
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) embed_sum_kernel(const uint2* order, const T* dout, long long ldd, T* grad, float* part, int n, int D, int V,
                                                         float scale, int tile, int chunks) {
-  __shared__ uint2 s[kMaxTile + 2];                            // the tile with a neighbour on either side
+  __shared__ uint2 all[kShort + kMaxTile + kShort + 1];        // the tile with its neighbours on either side
   pdl_launch_dependents();
   pdl_wait();
-  const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x & 31;
   const int first = t * tile, cnt = min(tile, n - first);
-  for (int i = threadIdx.x; i < cnt + 2; i += blockDim.x) {
-    const int at = first - 1 + i;
-    s[i] = at >= 0 && at < n ? order[at] : make_uint2(0xffffffffu, 0u);
+  for (int i = threadIdx.x; i < kShort + cnt + kShort + 1; i += blockDim.x) {
+    const long long at = (long long)first - kShort + i;
+    all[i] = at >= 0 && at < n ? order[at] : make_uint2(0xffffffffu, 0u);
   }
   __syncthreads();
-  const int c = (chunk * int(blockDim.x) + int(threadIdx.x)) * VEC;
+  const uint2* s = all + kShort;
+  // the segment that comes from the tile before, and the one that goes on in the next
+  const uint32_t head = s[0].x, tail = s[cnt - 1].x;
+  if (head >= uint32_t(V)) return;
+  int begin = 0, end = cnt;
+  bool head_long = false, tail_long = false;
+  const int back = run_length(s, -1, -1, head, kShort, lane);
+  if (back > 0) {
+    const int ahead = run_length(s, 0, 1, head, cnt + kShort, lane);
+    head_long = back + ahead > kShort;
+    if (!head_long) begin = min(ahead, cnt);                  // summed where it began
+  }
+  if (begin < cnt && tail < uint32_t(V)) {
+    const int ahead = run_length(s, cnt, 1, tail, kShort, lane);
+    if (ahead > 0) {
+      const int own = run_length(s, cnt - 1, -1, tail, cnt, lane);
+      tail_long = (own == cnt && back > 0 && head_long) || own + ahead > kShort;
+      if (!tail_long) end = cnt + ahead;
+    }
+  }
+  constexpr int NC = kCols<T, WIDE>;
+  const int c = WIDE ? (chunk * int(blockDim.x) + int(threadIdx.x)) * NC : chunk * int(blockDim.x) * NC + int(threadIdx.x);
   if (c >= D) return;
   constexpr int U = 8;
-  float acc[VEC];
+  float acc[NC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-  for (int e0 = 0; e0 < cnt; e0 += U) {
+  for (int j = 0; j < NC; ++j) acc[j] = 0.f;
+  for (int e0 = begin; e0 < end; e0 += U) {
     uint4 u[U];
-    T one[U];
+    T one[U][4];
 #pragma unroll
     for (int k = 0; k < U; ++k)
-      if (e0 + k < cnt && s[e0 + k + 1].x < uint32_t(V)) {
-        const T* p = dout + (long long)s[e0 + k + 1].y * ldd + c;
-        if constexpr (VEC == 1) one[k] = *p;
-        else u[k] = *reinterpret_cast<const uint4*>(p);
+      if (e0 + k < end && s[e0 + k].x < uint32_t(V)) {
+        const T* p = dout + (long long)s[e0 + k].y * ldd + c;
+        if constexpr (WIDE) u[k] = *reinterpret_cast<const uint4*>(p);
+        else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + j * int(blockDim.x) < D) one[k][j] = p[j * blockDim.x];
+        }
       }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int e = e0 + k;
-      if (e >= cnt || s[e + 1].x >= uint32_t(V)) break;
-      const uint32_t key = s[e + 1].x;
-      if constexpr (VEC == 1) acc[0] += to_f32(one[k]);
-      else {
-        float f[VEC];
+      if (e >= end || s[e].x >= uint32_t(V)) break;
+      const uint32_t key = s[e].x;
+      if constexpr (!WIDE) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j * int(blockDim.x) < D) acc[j] += to_f32(one[k][j]);
+      } else {
+        float f[NC];
         unpack16<T>(u[k], f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += f[j];
+        for (int j = 0; j < NC; ++j) acc[j] += f[j];
       }
-      const bool ends = s[e + 2].x != key, began = s[0].x != key;
-      if (ends || e == cnt - 1) {
-        if (ends && began) store_row<T, VEC>(grad + (long long)key * D + c, acc, scale);
+      if (e == end - 1 || s[e + 1].x != key) {
+        const bool from_before = head_long && key == head;
+        if (!from_before && !(tail_long && key == tail)) store_row<T, WIDE>(grad + (long long)key * D, c, D, acc, scale);
         else {
-          float* p = part + ((long long)t * 2 + (began ? 1 : 0)) * D + c;
+          float* p = part + ((long long)t * 2 + (from_before ? 0 : 1)) * D + c;
+          if constexpr (WIDE) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) p[j] = acc[j];
+            for (int j = 0; j < NC; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+              if (c + j * int(blockDim.x) < D) p[j * blockDim.x] = acc[j];
+          }
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+        for (int j = 0; j < NC; ++j) acc[j] = 0.f;
       }
     }
   }
 }
 
-// The tile in which a token begins that goes on behind it adds the pieces.
-template <typename T, int VEC>
+// The pieces of long segments.  A CTA takes those that begin in its tiles; a long segment goes on behind the tile in which it begins, or fills it.
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) embed_join_kernel(const uint2* order, const float* part, T* grad, int n, int D, int V, float scale, int tile, int chunks) {
+  __shared__ int until[kJoinTiles];                           // the last tile of the segment that begins in a tile, or -1
   pdl_launch_dependents();
   pdl_wait();
-  const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
-  const int first = t * tile, last = min(n, first + tile) - 1;
-  if (last + 1 >= n) return;
-  const uint32_t key = order[last].x;
-  if (key >= uint32_t(V) || order[last + 1].x != key || (first > 0 && order[first - 1].x == key)) return;
-  int lo = last + 1, hi = n;                                   // first place behind the token
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (order[mid].x == key) lo = mid + 1;
-    else hi = mid;
+  const int group = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x & 31;
+  const int tiles = (n + tile - 1) / tile;
+  for (int w = threadIdx.x >> 5; w < kJoinTiles; w += blockDim.x >> 5) {
+    const int t = group * kJoinTiles + w;
+    int end = -1;
+    if (t < tiles - 1) {
+      const int first = t * tile, next = first + tile;
+      const uint32_t key = order[next].x;
+      // places of the token in this tile (of up to 64 places, two to a lane), if it is not in the one before too
+      const bool a = lane < tile && order[first + lane].x == key, b = lane + 32 < tile && order[first + lane + 32].x == key;
+      const int own = __popc(__ballot_sync(0xffffffffu, a)) + __popc(__ballot_sync(0xffffffffu, b));
+      const bool begins = key < uint32_t(V) && own > 0 && (first == 0 || order[first - 1].x != key);
+      if (begins && (long long)next - own + kShort < n && order[next - own + kShort].x == key) {
+        for (int o = t + 1; end < 0; o += 32) {               // the first tile that does not end with it
+          const long long last = min((long long)n, (long long)(o + lane + 1) * tile) - 1;
+          const bool goes_on = o + lane < tiles - 1 && order[last].x == key;
+          const unsigned m = __ballot_sync(0xffffffffu, !goes_on);
+          if (m) {
+            end = o + __ffs(m) - 1;
+            if (order[(long long)end * tile].x != key) --end;
+          }
+        }
+      }
+    }
+    if (lane == 0) until[w] = end;
   }
-  const int end = (lo - 1) / tile;
-  const int c = (chunk * int(blockDim.x) + int(threadIdx.x)) * VEC;
+  __syncthreads();
+  constexpr int NC = kCols<T, WIDE>;
+  const int c = WIDE ? (chunk * int(blockDim.x) + int(threadIdx.x)) * NC : chunk * int(blockDim.x) * NC + int(threadIdx.x);
   if (c >= D) return;
-  float acc[VEC];
+  for (int i = 0; i < kJoinTiles; ++i) {
+    const int t = group * kJoinTiles + i;
+    if (until[i] < 0) continue;
+    float acc[NC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = part[((long long)t * 2 + 1) * D + c + j];
+    for (int j = 0; j < NC; ++j) acc[j] = 0.f;
 #pragma unroll 4
-  for (int k = t + 1; k <= end; ++k)
+    for (int k = t; k <= until[i]; ++k) {
+      const float* p = part + ((long long)k * 2 + (k == t ? 1 : 0)) * D + c;
+      if constexpr (WIDE) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] += part[(long long)k * 2 * D + c + j];
-  store_row<T, VEC>(grad + (long long)key * D + c, acc, scale);
+        for (int j = 0; j < NC; j += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p + j);
+          acc[j] += v.x; acc[j + 1] += v.y; acc[j + 2] += v.z; acc[j + 3] += v.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+          if (c + j * int(blockDim.x) < D) acc[j] += p[j * blockDim.x];
+      }
+    }
+    store_row<T, WIDE>(grad + (long long)order[min(n, t * tile + tile) - 1].x * D, c, D, acc, scale);
+  }
 }
 
 template <typename T, typename IDX>
 int embedding_fwd(const void* idx, const void* table, void* out, long long n, int D, int V, float scale, cudaStream_t st) {
   const bool vec = D % kVec<T> == 0 && ((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  const long long items = n * (vec ? D / kVec<T> : D);
-  const unsigned grid = unsigned((items + 1023) / 1024);
-  auto kernel = vec ? token_embedding_fwd_kernel<T, IDX, kVec<T>> : token_embedding_fwd_kernel<T, IDX, 1>;
-  LT_RETURN_IF_CUDA(launch_chained(kernel, grid, 256, 0, st, static_cast<const IDX*>(idx), static_cast<const T*>(table), static_cast<T*>(out), n, D, V, scale));
+  auto i = static_cast<const IDX*>(idx);
+  auto w = static_cast<const T*>(table);
+  auto y = static_cast<T*>(out);
+  if (vec) {
+    int log = 0;
+    while (log < 8 && (1 << log) < D / kVec<T>) ++log;
+    const int rows = 1024 >> log;                             // of a CTA
+    LT_RETURN_IF_CUDA(launch_chained(token_embedding_fwd_kernel<T, IDX>, unsigned((n + rows - 1) / rows), 256, 0, st, i, w, y, n, D, V, scale, log));
+  } else {
+    const long long ctas = (n * D + 2047) / 2048;
+    if (ctas > 0x7fffffffll) return -int(kStatusBadArgument);
+    LT_RETURN_IF_CUDA(launch_chained(token_embedding_flat_kernel<T, IDX>, unsigned(ctas), 256, 0, st, i, w, y, n, D, V, scale, 1.f / float(D)));
+  }
   return 0;
 }
 
 template <typename T, typename IDX>
 int embedding_bwd(const void* idx, const void* dout, long long ldd, void* grad, int n, int D, int V, float scale, long long pad, void* order, float* part,
                   int tile, cudaStream_t st) {
-  LT_RETURN_IF_CUDA(cudaMemsetAsync(grad, 0, size_t(V) * D * sizeof(T), st));
-  if (n == 0) return 0;
-  constexpr int smem = (kSortWarps * kSortBins + 2 * kSortBins) * 4;
+  const size_t bytes = size_t(V) * D * sizeof(T);
+  if (n == 0) {
+    LT_RETURN_IF_CUDA(cudaMemsetAsync(grad, 0, bytes, st));
+    return 0;
+  }
   static OncePerDevice once;
   if (once.pending()) {
-    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(embed_sort_kernel<IDX>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    LT_RETURN_IF_CUDA(cudaFuncSetAttribute(embed_sort_kernel<IDX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortThreads / 32 + 2) * kSortBins * 4));
     once.finish();
   }
-  int passes = 1, ctas = 1;
-  while (passes * kSortBits < 32 && (V >> (passes * kSortBits)) != 0) ++passes;
-  while (ctas < 8 && n > ctas * 2048) ctas *= 2;
+  int width = 1, passes = 1, ctas = 1, nt = kSortThreads;
+  while (width < 31 && (V >> width) != 0) ++width;
+  while (passes * kSortBits < width) ++passes;
+  const int bits = (width + passes - 1) / passes;
+  while (ctas < 8 && n > ctas * 1024) ctas *= 2;
+  while (nt > 128 && n <= ctas * nt / 2) nt /= 2;
   uint2* buf0 = static_cast<uint2*>(order);
   uint2* buf1 = buf0 + n;
   const uint2* sorted = (passes & 1) ? buf0 : buf1;
-  LT_RETURN_IF_CUDA(launch_chained_clusters(embed_sort_kernel<IDX>, ctas, kSortThreads, smem, ctas, st, static_cast<const IDX*>(idx), n, V, pad, buf0, buf1, passes, ctas));
-  const bool vec = D % kVec<T> == 0 && ldd % kVec<T> == 0 && ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
-  const int per = vec ? D / kVec<T> : D;
+  const int smem = (nt / 32 + 2) * (1 << bits) * 4;
+  LT_RETURN_IF_CUDA(launch_chained_clusters(embed_sort_kernel<IDX>, ctas, nt, smem, ctas, st, static_cast<const IDX*>(idx), n, V, pad, buf0, buf1, passes, bits, ctas));
+  if (bytes > size_t(kClear) * 0x7fffffff) return -int(kStatusBadArgument);
+  LT_RETURN_IF_CUDA(launch_chained(embed_clear_kernel, unsigned((bytes + kClear - 1) / kClear), 512, 0, st, static_cast<unsigned char*>(grad), (long long)bytes));
+  const bool vec = D % kVec<T> == 0 && ldd % kVec<T> == 0 && ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(part)) & 15) == 0;
+  const int per = vec ? D / kVec<T> : (D + 3) / 4;
   const int threads = per >= 256 ? 256 : (per + 31) / 32 * 32;
   const int chunks = (per + threads - 1) / threads, tiles = (n + tile - 1) / tile;
   if ((long long)tiles * chunks > 0x7fffffffll) return -int(kStatusBadArgument);
-  auto sum = vec ? embed_sum_kernel<T, kVec<T>> : embed_sum_kernel<T, 1>;
-  auto join = vec ? embed_join_kernel<T, kVec<T>> : embed_join_kernel<T, 1>;
+  auto sum = vec ? embed_sum_kernel<T, true> : embed_sum_kernel<T, false>;
+  auto join = vec ? embed_join_kernel<T, true> : embed_join_kernel<T, false>;
   LT_RETURN_IF_CUDA(launch_chained(sum, tiles * chunks, threads, 0, st, sorted, static_cast<const T*>(dout), ldd, static_cast<T*>(grad), part, n, D, V, scale, tile, chunks));
-  if (tiles > 1)
-    LT_RETURN_IF_CUDA(launch_chained(join, tiles * chunks, threads, 0, st, sorted, static_cast<const float*>(part), static_cast<T*>(grad), n, D, V, scale, tile, chunks));
+  if (n > kShort)
+    LT_RETURN_IF_CUDA(launch_chained(join, (tiles + kJoinTiles - 1) / kJoinTiles * chunks, threads, 0, st, sorted, static_cast<const float*>(part), static_cast<T*>(grad), n, D, V, scale, tile, chunks));
   return 0;
 }
 
@@ -296,7 +447,7 @@ int lt_token_embedding_fwd(int type, const void* idx, int idx32, const void* tab
   using namespace lt;
   if (type < 0 || type > 2 || n < 0 || D < 0 || V < 1) return -int(kStatusBadArgument);
   if (n == 0 || D == 0) return 0;
-  if (n > (0x7fffffffll * 1024) / D) return -int(kStatusBadArgument);
+  if (n > 0x7fffffffll) return -int(kStatusBadArgument);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (type == kElemF32) return idx32 ? embedding_fwd<float, int>(idx, table, out, n, D, V, scale, st) : embedding_fwd<float, long long>(idx, table, out, n, D, V, scale, st);
   if (type == kElemBf16)
@@ -305,7 +456,7 @@ int lt_token_embedding_fwd(int type, const void* idx, int idx32, const void* tab
 }
 
 // grad[V, D] = scale * sums of dout's rows (pitch ldd) by token; tokens outside [0, V) and `pad` give nothing (pad < 0: there is none).  All of grad is written.
-// order: 2 n entries of 8 bytes; part: 2 ceil(n / tile) rows of D floats; tile: up to 256 sorted rows a CTA.
+// order: 2 n entries of 8 bytes; part: 2 ceil(n / tile) rows of D floats; tile: up to 64 sorted rows a CTA.
 int lt_token_embedding_bwd(int type, const void* idx, int idx32, const void* dout, long long ldd, void* grad, long long n, int D, int V, float scale, long long pad,
                            void* order, float* part, int tile, void* stream) {
   using namespace lt;

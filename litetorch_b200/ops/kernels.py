@@ -146,7 +146,7 @@ class LlamaLayer(ctypes.Structure):
 _bound = {}
 
 # Kernels launched per native call; `launch_count()` is what bench.py reports as "gpu_launches".
-_LAUNCHES_PER_CALL = {"lt_gemm_num_tiles": 0, "lt_token_embedding_bwd": 3, "lt_gemm_skinny_set_target": 0, "lt_adam_q8": 3, "lt_set_wait_budget_cycles": 0, "lt_norm_bwd": 2, "lt_paged_decode": 2, "lt_paged_decode_window": 2, "lt_mlstm_prefill": 4, "lt_rglru_scan": 3, "lt_rglru_step": 2, "lt_flash_bwd": 3, "lt_flash_bwd_rope": 3, "lt_llama_layer_fwd": 8, "lt_llama_layer_bwd": 16, "lt_status_fetch": 0, "lt_sm_count": 0, "lt_gemm_set_tail_split": 0, "lt_reduce_parts": 0, "lt_reduce_all": 2, "lt_gemm_set_pair_mode": 0, "lt_flash_bwd_set_trace": 0, "lt_flash_fwd_set_trace": 0, "lt_norm_bwd_ctas": 0, "lt_paged_decode_places": 0,
+_LAUNCHES_PER_CALL = {"lt_gemm_num_tiles": 0, "lt_token_embedding_bwd": 4, "lt_gemm_skinny_set_target": 0, "lt_adam_q8": 3, "lt_set_wait_budget_cycles": 0, "lt_norm_bwd": 2, "lt_paged_decode": 2, "lt_paged_decode_window": 2, "lt_mlstm_prefill": 4, "lt_rglru_scan": 3, "lt_rglru_step": 2, "lt_flash_bwd": 3, "lt_flash_bwd_rope": 3, "lt_llama_layer_fwd": 8, "lt_llama_layer_bwd": 16, "lt_status_fetch": 0, "lt_sm_count": 0, "lt_gemm_set_tail_split": 0, "lt_reduce_parts": 0, "lt_reduce_all": 2, "lt_gemm_set_pair_mode": 0, "lt_flash_bwd_set_trace": 0, "lt_flash_fwd_set_trace": 0, "lt_norm_bwd_ctas": 0, "lt_paged_decode_places": 0,
                       "lt_adam_chunk_elems": 0}
 _launches = [0]
 
@@ -1653,12 +1653,17 @@ def token_embedding_grad(idx: torch.Tensor, dout: torch.Tensor, vocab: int, scal
         dout = dout.contiguous()
     n, D = dout.shape
     grad = torch.empty((vocab, D), dtype=dout.dtype, device=dout.device)
-    tile = 32
-    order = torch.empty((2, max(n, 1)), dtype=torch.int64, device=dout.device)
-    part = torch.empty(((n + tile - 1) // tile, 2, D), dtype=torch.float32, device=dout.device)
+    # sorted rows that a CTA sums of 256 vectors of 16 bytes, or of 1024 columns: up to 32, so that there are eight CTAs an SM
+    size = dout.element_size()
+    chunks = -(-D // (256 * 16 // size if D * size % 16 == 0 else 1024))
+    tile = 8
+    while tile < 32 and n * chunks >= 2 * tile * 8 * 148:
+        tile *= 2
+    # the sorted list twice, 8 bytes an entry, and two rows for the pieces of every tile
+    room = torch.empty(16 * n + (n + tile - 1) // tile * 8 * D, dtype=torch.uint8, device=dout.device)
     with _on(dout):
         _check(_fn("lt_token_embedding_bwd")(_ELEM[dout.dtype], idx.data_ptr(), 1 if idx.dtype == torch.int32 else 0, dout.data_ptr(), dout.stride(0), grad.data_ptr(),
-                                             n, D, int(vocab), float(scale), int(padding_idx), order.data_ptr(), part.data_ptr(), tile, _stream()),
+                                             n, D, int(vocab), float(scale), int(padding_idx), room.data_ptr(), room.data_ptr() + 16 * n, tile, _stream()),
                "lt_token_embedding_bwd")
     return grad
 
