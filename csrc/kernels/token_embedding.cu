@@ -65,31 +65,33 @@ __global__ void __launch_bounds__(256) token_embedding_fwd_kernel(const IDX* idx
   }
 }
 
-// Rows that do not begin at 16 bytes: elements of the result in their order, eight to a thread, so that warps write whole lines.
+// Rows that do not begin at 16 bytes: four at once again, elements a CTA's width apart.  (Loads behind the end of a row take its last element.)
 template <typename T, typename IDX>
-__global__ void __launch_bounds__(256) token_embedding_flat_kernel(const IDX* idx, const T* table, T* out, long long n, int D, int V, float scale, float inv) {
+__global__ void __launch_bounds__(256) token_embedding_odd_kernel(const IDX* idx, const T* table, T* out, long long n, int D, int V, float scale) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int U = 8;
-  const long long first = (long long)blockIdx.x * (256 * U);
-  const long long row0 = first / D;
-  const int off = int(first - row0 * D);
-  long long from[U];
+  constexpr int R = 4, U = 4;
+  const long long first = (long long)blockIdx.x * R;
+  const T* from[R];
+  bool in[R];
 #pragma unroll
-  for (int k = 0; k < U; ++k) {
-    const unsigned at = unsigned(off) + k * 256 + threadIdx.x;
-    unsigned q = unsigned(__uint2float_rz(at) * inv);         // at / D, or one or two off
-    while (q * (unsigned long long)D > at) --q;
-    while ((q + 1ull) * D <= at) ++q;
-    const long long row = row0 + q, tok = row < n ? (long long)idx[row] : -1;
-    from[k] = tok >= 0 && tok < V ? tok * D + (at - q * D) : -1;
+  for (int r = 0; r < R; ++r) {
+    const long long tok = first + r < n ? (long long)idx[first + r] : -1;
+    in[r] = tok >= 0 && tok < V;
+    from[r] = table + (in[r] ? tok : 0) * D;
   }
-  float f[U];
+  for (int c0 = threadIdx.x; c0 < D; c0 += U * 256) {
+    T one[R][U];
 #pragma unroll
-  for (int k = 0; k < U; ++k) f[k] = from[k] >= 0 ? to_f32(table[from[k]]) * scale : 0.f;
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-  for (int k = 0; k < U; ++k)
-    if (first + k * 256 + threadIdx.x < n * D) out[first + k * 256 + threadIdx.x] = from_f32<T>(f[k]);
+      for (int k = 0; k < U; ++k) one[r][k] = from[r][min(c0 + k * 256, D - 1)];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (first + r < n && c0 + k * 256 < D) out[(first + r) * D + c0 + k * 256] = from_f32<T>(in[r] ? to_f32(one[r][k]) * scale : 0.f);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------- sort
@@ -392,9 +394,7 @@ int embedding_fwd(const void* idx, const void* table, void* out, long long n, in
     const int rows = 1024 >> log;                             // of a CTA
     LT_RETURN_IF_CUDA(launch_chained(token_embedding_fwd_kernel<T, IDX>, unsigned((n + rows - 1) / rows), 256, 0, st, i, w, y, n, D, V, scale, log));
   } else {
-    const long long ctas = (n * D + 2047) / 2048;
-    if (ctas > 0x7fffffffll) return -int(kStatusBadArgument);
-    LT_RETURN_IF_CUDA(launch_chained(token_embedding_flat_kernel<T, IDX>, unsigned(ctas), 256, 0, st, i, w, y, n, D, V, scale, 1.f / float(D)));
+    LT_RETURN_IF_CUDA(launch_chained(token_embedding_odd_kernel<T, IDX>, unsigned((n + 3) / 4), 256, 0, st, i, w, y, n, D, V, scale));
   }
   return 0;
 }

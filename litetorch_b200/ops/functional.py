@@ -492,22 +492,27 @@ def embedding(idx, table):
     return F.embedding(idx.to(torch.int64), table)
 
 
+def _once(name: str) -> None:
+    # (a second derivative would silently be that of a constant)
+    if torch.is_grad_enabled():
+        raise RuntimeError("%s is differentiable once" % name)
+
+
 class _TokenEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, idx, table, scale, pad):
-        idx = K._dense_index(idx, torch.int64, torch.int32)
         ctx.save_for_backward(idx)
-        ctx.vocab, ctx.scale, ctx.pad = table.shape[0], scale, pad
-        return K.token_embedding(idx, table.contiguous(), scale)
+        ctx.rest = table.shape[0], scale, pad
+        return K.token_embedding(idx, table, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        (idx,) = ctx.saved_tensors
-        return None, K.token_embedding_grad(idx, dout, ctx.vocab, ctx.scale, ctx.pad), None, None
+        _once("token_embedding")
+        return None, K.token_embedding_grad(*ctx.saved_tensors, dout, *ctx.rest), None, None
 
 
 _KERNEL_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_INDEX_TYPES = (torch.int64, torch.int32)
 
 
 def _whole(name: str, t: torch.Tensor) -> None:
@@ -519,25 +524,28 @@ def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0, 
     """scale * table[idx] for tokens idx [...] and a table [V, D]: [..., D], rounded once from fp32.  A token outside [0, V) gives a row of zeros and no
     gradient; `padding_idx` (negative: from the end) gives its row and no gradient.  The table's gradient is summed over the sorted tokens in fp32 and in their
     order, then rounded once, where `embedding` adds bf16 numbers with atomics: it is the same from run to run."""
-    _whole("token_embedding", idx)
     if table.dim() != 2 or not table.is_floating_point():
         raise TypeError("token_embedding: the table is a matrix of floating-point numbers")
     V, D = table.shape
+    if idx.dtype not in _INDEX_TYPES:
+        _whole("token_embedding", idx)
+        idx = idx.to(torch.int64)
     if idx.device != table.device:
         raise ValueError("token_embedding: tokens on %s, table on %s" % (idx.device, table.device))
-    if V < 1 or V >= (1 << 31) - 1 or idx.numel() > (1 << 31) - 4097:
+    if V < 1 or V >= (1 << 31) - 1 or D >= 1 << 31 or idx.numel() > (1 << 31) - 4097:
         raise ValueError("token_embedding: a table of 1 to 2^31 - 2 rows and fewer than 2^31 - 4096 tokens are expected")
     pad = -1
     if padding_idx is not None:
         if not -V <= padding_idx < V:
             raise ValueError("token_embedding: padding_idx %d is not among %d rows" % (padding_idx, V))
         pad = int(padding_idx) % V
+    flat = idx if idx.dim() == 1 and idx.is_contiguous() else idx.reshape(-1).contiguous()
     if table.is_cuda and table.dtype in _KERNEL_TYPES:
-        return _TokenEmbedding.apply(idx.reshape(-1), table, float(scale), pad).view(*idx.shape, D)
-    flat = idx.reshape(-1).to(torch.int64)
+        out = _TokenEmbedding.apply(flat, table if table.is_contiguous() else table.contiguous(), float(scale), pad)
+        return out if flat is idx else out.view(*idx.shape, D)
     inside = ((flat >= 0) & (flat < V))[:, None]
     wide = table if table.dtype == torch.float64 else table.float()
-    rows = wide[flat.clamp(0, V - 1)]
+    rows = wide[flat.to(torch.int64).clamp(0, V - 1)]
     if pad >= 0:
         rows = torch.where((flat == pad)[:, None], rows.detach(), rows)
     return torch.where(inside, rows * scale, torch.zeros_like(rows)).to(table.dtype).view(*idx.shape, D)
@@ -558,13 +566,13 @@ class _Distillation(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, up):
+        _once("distillation_loss")
         z, room = ctx.saved_tensors
         ahead, ctx.ahead = ctx.ahead, None                     # handed out once
         if ahead is not None and torch.cuda.is_current_stream_capturing():
             ahead = None
-        return K.distill_grad(z, room, *ctx.rest, up.contiguous(), ahead), None, None, None, None
+        return K.distill_grad(z, room, *ctx.rest, up if up.is_contiguous() else up.contiguous(), ahead), None, None, None, None
 
 
 def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_idx: torch.Tensor, temperature: float = 1.0,
@@ -577,7 +585,9 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     reduction: "mean" over the rows that have a teacher, "sum", or "none" (a loss for every row, fp32).  The teacher gets no gradient."""
     if not logits.is_floating_point() or not teacher_logits.is_floating_point():
         raise TypeError("distillation_loss: logits are floating-point numbers")
-    _whole("distillation_loss", teacher_idx)
+    if teacher_idx.dtype not in _INDEX_TYPES:
+        _whole("distillation_loss", teacher_idx)
+        teacher_idx = teacher_idx.to(torch.int64)
     if logits.dim() < 1 or teacher_logits.shape != teacher_idx.shape or teacher_logits.shape[:-1] != logits.shape[:-1] or teacher_logits.dim() != logits.dim():
         raise ValueError("distillation_loss: logits %s, teacher's logits %s at %s" % (list(logits.shape), list(teacher_logits.shape), list(teacher_idx.shape)))
     if not logits.device == teacher_logits.device == teacher_idx.device:
@@ -589,14 +599,17 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     V, top = logits.shape[-1], teacher_idx.shape[-1]
     if not 1 <= top <= 1024 or V < 1:
         raise ValueError("distillation_loss: 1 to 1024 of the teacher's logits and at least one class are expected")
-    lead = logits.shape[:-1]
-    z, t, idx = logits.reshape(-1, V), teacher_logits.detach().reshape(-1, top), teacher_idx.reshape(-1, top)
-    if z.shape[0] >= 1 << 31 or V >= 1 << 30:
+    lead, rows = logits.shape[:-1], teacher_idx.numel() // top
+    if rows >= 1 << 31 or V >= 1 << 30:
         raise ValueError("distillation_loss: too many rows or classes")
-    if z.is_cuda and z.dtype in _KERNEL_TYPES and z.shape[0] > 0:
+    z, t, idx = logits, teacher_logits, teacher_idx
+    if logits.dim() != 2:
+        z, t, idx = z.reshape(rows, V), t.reshape(rows, top), idx.reshape(rows, top)
+    if z.is_cuda and z.dtype in _KERNEL_TYPES and rows > 0:
         loss = _Distillation.apply(z, t if t.dtype in _KERNEL_TYPES else t.float(), idx, float(temperature), reduction)
     else:
         wide = torch.promote_types(z.dtype, torch.float32)
+        t = t.detach()
         there = (idx >= 0) & (idx < V) & (t != -math.inf)
         has = there.any(1)
         log_p = torch.log_softmax((t.to(wide) / temperature).masked_fill(~there, -math.inf).masked_fill(~has[:, None], 0.0), -1)
@@ -607,10 +620,11 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         if reduction != "none":
             loss = loss.sum() / (has.sum().clamp(min=1) if reduction == "mean" else 1)
         loss = loss if wide == torch.float64 else loss.float()
-    return loss.view(lead) if reduction == "none" else loss
+    return loss.view(lead) if reduction == "none" and len(lead) != 1 else loss
 
 
 # ---------------------------------------------------------------------------------------------- sampling
+@torch.no_grad()
 def _sample_plain(z, u, tau, k, p, low):
     """(tokens, log probabilities) in 64 bits; parameters as columns."""
     V = z.shape[1]
@@ -638,7 +652,6 @@ def _sample_plain(z, u, tau, k, p, low):
     return torch.where(empty, -1, tokens), torch.where(empty, -math.inf, logprobs).float()
 
 
-@torch.no_grad()
 def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """(tokens, log probabilities) for logits [..., V], drawn with the given random numbers uniform [...] in [0, 1).  With w = e^((z - max z) / temperature)
     and the tokens in order of their logit, of equals the lowest index first:
@@ -657,20 +670,25 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
         raise ValueError("sample_tokens: 1 to 524288 tokens are expected, not %d" % V)
     if not torch.is_tensor(uniform) or not uniform.is_floating_point() or uniform.shape != lead or uniform.device != logits.device:
         raise ValueError("sample_tokens: a random number for every row, on the logits' device, is expected")
-    z = logits.detach().reshape(-1, V)
+    z, u = logits, uniform
+    if z.dim() != 2:
+        z, u = z.reshape(u.numel(), V), u.reshape(-1)
     rows = z.shape[0]
-    u = uniform.detach().reshape(-1)
-    u = (u if u.dtype == torch.float64 else u.float()).contiguous()
     if rows >= 1 << 28:
         raise ValueError("sample_tokens: too many rows")
+    if u.dtype not in (torch.float32, torch.float64):
+        u = u.float()
+    if not u.is_contiguous():
+        u = u.contiguous()
     given = []
     for name, v, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if torch.is_tensor(v):
+        if isinstance(v, torch.Tensor):
             if v.device != logits.device or v.shape not in (lead, torch.Size(())):
                 raise ValueError("sample_tokens: %s has one number, or one for every row on the logits' device" % name)
             if dtype == torch.int32:
                 _whole("sample_tokens: top_k", v)
-                v = v.clamp(0, V)
+                if v.dtype != torch.int32:
+                    v = v.clamp(0, V)
             v = v.detach().expand(lead).reshape(-1).to(dtype).contiguous()
         elif dtype == torch.int32:
             v = index(v)
@@ -684,9 +702,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
     elif z.is_cuda and z.dtype in _KERNEL_TYPES:
         tokens, logprobs = K.sample_tokens(z if z.stride(1) == 1 else z.contiguous(), u, *given)
     else:
-        tokens, logprobs = _sample_plain(z, u.double(), *(v.double()[:, None] if torch.is_tensor(v) else torch.full((rows, 1), float(v), dtype=torch.float64, device=z.device)
-                                                          for v in given))
-    return tokens.view(lead), logprobs.view(lead)
+        tokens, logprobs = _sample_plain(z.detach(), u.detach().double(),
+                                         *(v.double()[:, None] if torch.is_tensor(v) else torch.full((rows, 1), float(v), dtype=torch.float64, device=z.device) for v in given))
+    return (tokens, logprobs) if len(lead) == 1 else (tokens.view(lead), logprobs.view(lead))
 
 
 # ------------------------------------------------------------------------------------------------ softmax / dropout / router

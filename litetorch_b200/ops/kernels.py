@@ -1685,7 +1685,7 @@ def distill_loss(z, t, idx, temperature: float, reduction: str, with_grad: bool)
     (N, V), top = z.shape, t.shape[1]
     assert t.shape == idx.shape == (N, top) and z.dtype in _ELEM and t.dtype in _ELEM and z.device == t.device == idx.device and 1 <= top <= 1024
     z = z if z.stride(1) == 1 else z.contiguous()
-    t, idx = t.contiguous(), idx.to(torch.int64).contiguous()
+    t, idx = t.contiguous(), (idx if idx.dtype == torch.int64 else idx.to(torch.int64)).contiguous()
     mean = reduction == "mean"
     # [N, K, 2] entries and a counter, [N, 2] references and sums, [N] losses, [N] bytes
     room = z.new_empty(N * (2 * top + 3) + 2 + (N + 3) // 4, dtype=torch.float32)
