@@ -30,7 +30,7 @@ struct DistillArgs {
   const float* up;               // upstream gradient: one (up_rows 0) or one for every row; null: 1
   int up_rows;
   int skip_one;                  // with one upstream gradient: return where it is 1 (the gradient is there)
-  float2* stats;                 // [N] reference (the maximum of z log2(e) / T) and sum of 2^(z log2(e) / T - reference)
+  float2* stats;                 // [N] maximum of z, and the sum of 2^(z log2(e) / T - reference) with the maximum's reference
   int have_stats;
   float* loss;                   // [N] or null
   void* grad;                    // [N, V] (pitch ldg, rows where those of z lie within 16 bytes) or null
@@ -103,11 +103,32 @@ __device__ __forceinline__ float warp_max(float v) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
   return y;
 }
-// (reference, sum of 2^(. - reference)) over the warp.  Logits enter as fma(z, c, -reference), so that the reference is exact whatever its own rounding.
-__device__ __forceinline__ void warp_max_sum(float& m, float& s) {
+// Powers of two are taken of z c - ref, with ref = c times the largest logit m: z enters as fma(z, c, -ref), so that the reference is exact whatever its own
+// rounding (which scales all of a row's powers alike, by up to 2^64 here).  From |ref| = 2^31 on (masks of the type's lowest value everywhere, say) what lies
+// below m lies 128 or more below it and weighs nothing: any factor does that leaves its multiples finite and far apart, so it is the power of two that brings m to
+// 2^60.
+struct Scale {
+  float c, ref;
+};
+__device__ __forceinline__ bool far_out(float ref) { return fabsf(ref) >= 0x1p31f; }
+__device__ __forceinline__ Scale scale_of(float m, float c) {
+  Scale q{c, __fmul_rn(m, c)};
+  if (far_out(q.ref) && fabsf(m) != INFINITY) {
+    q.c = __uint_as_float((314u - (__float_as_uint(m) >> 23 & 255u)) << 23);
+    q.ref = m * q.c;
+  }
+  return q;
+}
+// A sum that belongs to the maximum `own` as one that belongs to m.
+__device__ __forceinline__ float moved(float s, float own, float m, float c) {
+  const float ref = __fmul_rn(m, c);                          // (not contracted: as scale_of rounds it)
+  return own == m || own == -INFINITY ? s : s * (far_out(ref) ? 0.f : ex2(__fmul_rn(own, c) - ref));
+}
+// (maximum, sum) over the warp.
+__device__ __forceinline__ void warp_max_sum(float& m, float& s, float c) {
   const float own = m;
   m = warp_max(m);
-  if (own != -INFINITY) s *= ex2(own - m);
+  s = moved(s, own, m, c);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
 }
@@ -217,16 +238,15 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
   if (a.flags) weight /= float(max(1, count_flags(a.flags, a.N, isum)));
   if (a.up && !a.up_rows) weight *= a.up[0];
   const float c = a.c;
-  const uint64_t c2 = pack_f32x2(c, c);
   const int tid = threadIdx.x, lane = tid & 31, nt = blockDim.x, nw = nt >> 5;
   const int clog = a.cluster_log, rank = clog ? int(cluster_ctarank()) : 0;
   const int vpt = a.vpt, room = vpt * nt;
   const int first = (tid >> 5) * vpt * 32 + lane;             // this thread's vectors: first, first + 32, ... of the CTA's
   uint4* vectors = reinterpret_cast<uint4*>(smem) + first;    // [3][vpt nt]
-  float2* entry_buf = reinterpret_cast<float2*>(smem + S::entries(nt, vpt));   // [4][K]
-  float2* peers = reinterpret_cast<float2*>(smem + S::peers(nt, vpt, a.K));    // [4][CTAs][warps]: (reference, sum)
-  LINK* heads = reinterpret_cast<LINK*>(smem + S::heads(nt, vpt, a.K));        // [3][nt][8]: number of a vector's first entry + 1
-  LINK* links = reinterpret_cast<LINK*>(smem + S::links(nt, vpt, a.K));        // [3][K]: that of an entry's next
+  float2* entry_buf = reinterpret_cast<float2*>(smem + S::entries(nt, vpt));   // [5][K]
+  float2* peers = reinterpret_cast<float2*>(smem + S::peers(nt, vpt, a.K));    // [4][CTAs][warps]: (maximum, sum)
+  LINK* heads = reinterpret_cast<LINK*>(smem + S::heads(nt, vpt, a.K));        // [4][nt][8]: number of a vector's first entry + 1
+  LINK* links = reinterpret_cast<LINK*>(smem + S::links(nt, vpt, a.K));        // [4][K]: that of an entry's next
   const int pairs = nw << clog;
   const uint32_t bar0 = smem_u32(bars);
   if (tid == 0) {
@@ -306,7 +326,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
       if (a.grad) {
         const float2* entries = entry_buf + entry_cur * a.K;
         const int elo = r.lo * VEC - r.shift, ehi = r.end * VEC - r.shift;
-            for (int k = tid; k < a.K; k += nt) {
+        for (int k = tid; k < a.K; k += nt) {
           const int i = __float_as_int(entries[k].y);
           if (i >= max(elo, 0) && i < ehi) {
             const int v = (i - elo) / VEC, w = v / (32 * vpt), owner = w * 32 + v % 32;
@@ -333,10 +353,10 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
         float m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) m = fmaxf(m, max16<T>(u[k]));
-        m *= c;
-        const float from = m == -INFINITY ? 0.f : -m;
+        const Scale q = scale_of(m, c);
+        const float from = m == -INFINITY ? 0.f : -q.ref;
         uint64_t part[VEC / 2];
-        const uint64_t from2 = pack_f32x2(from, from);
+        const uint64_t from2 = pack_f32x2(from, from), c2 = pack_f32x2(q.c, q.c);
 #pragma unroll
         for (int j = 0; j < VEC / 2; ++j) part[j] = 0ull;
 #pragma unroll
@@ -357,7 +377,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
         float s, s1;
         unpack_f32x2(part[0], s, s1);
         s += s1;
-        warp_max_sum(m, s);
+        warp_max_sum(m, s, c);
         const int at = (turn * kDistillCluster + rank) * nw + (tid >> 5);
         if (clog) {
           if (lane >> clog == 0) send8(smem_u32(peers + at), bar0 + 8 * turn, lane, make_float2(m, s));
@@ -400,7 +420,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
         m = warp_max(m);
 #pragma unroll
         for (int i = 0; i < kDistillCluster * kDistillWarps / 32; ++i)
-          if (i * 32 < pairs) s += q[i].x == -INFINITY ? q[i].y : q[i].y * ex2(q[i].x - m);
+          if (i * 32 < pairs) s += moved(q[i].y, q[i].x, m, c);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (a.stats && rank == 0 && tid == 0) a.stats[old] = make_float2(m, s);
@@ -408,6 +428,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
       if (a.grad) {
         T* g = static_cast<T*>(a.grad) + (long long)old * a.ldg;
         const float w = a.up_rows ? weight * a.up[old] : weight, scale = __fdividef(w, s);
+        const Scale by = scale_of(m, c);
         T* to = g - r.shift + (r.lo + first) * VEC;
         const int end = r.end - r.lo - first;
         const bool cuts = !EVEN && (r.shift != 0 || r.vecs * VEC != a.V);
@@ -423,7 +444,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
 #pragma unroll
           for (int j = 0; j < VEC / 2; ++j) {
             float x, y;
-            unpack_f32x2(fma_f32x2(pack_f32x2(f[2 * j], f[2 * j + 1]), c2, pack_f32x2(-m, -m)), x, y);
+            unpack_f32x2(fma_f32x2(pack_f32x2(f[2 * j], f[2 * j + 1]), pack_f32x2(by.c, by.c), pack_f32x2(-by.ref, -by.ref)), x, y);
             unpack_f32x2(mul_f32x2(pack_f32x2(ex2(x), ex2(y)), pack_f32x2(scale, scale)), f[2 * j], f[2 * j + 1]);
           }
           return pack16<T>(f);
@@ -468,7 +489,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
                 float p = ex2(entries[e - 1].x);
                 if (link[e - 1]) p = chained_p(entries, link, e, p);
                 const float x = to_f32(reinterpret_cast<const T*>(mine + v * 32)[j]);
-                g[i] = from_f32<T>((__fdividef(ex2(fmaf(x, c, -m)), s) - p) * w);
+                g[i] = from_f32<T>((__fdividef(ex2(fmaf(x, by.c, -by.ref)), s) - p) * w);
               }
             }
           }
@@ -517,40 +538,42 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
       for (int i = tid; i < vecs; i += kLongThreads) {
         float f[VEC];
         unpack16<T>(*reinterpret_cast<const uint4*>(z + head + i * VEC), f);
-        float vm = -INFINITY;
+        float vm = m;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) vm = fmaxf(vm, f[j]);
-        vm = fmaxf(m, vm * c);
-        const float from = vm == -INFINITY ? 0.f : vm;
-        s = m == -INFINITY ? s : s * ex2(m - vm);
+        const Scale q = scale_of(vm, c);
+        const float from = vm == -INFINITY ? 0.f : -q.ref;
+        s = moved(s, m, vm, c);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s += ex2(fmaf(f[j], c, -from));
+        for (int j = 0; j < VEC; ++j) s += ex2(fmaf(f[j], q.c, from));
         m = vm;
       }
       for (int i = tid; i < rest; i += kLongThreads) {
-        const float f = to_f32(z[edge(i)]), vm = fmaxf(m, f * c);
-        s = (m == -INFINITY ? s : s * ex2(m - vm)) + ex2(fmaf(f, c, vm == -INFINITY ? 0.f : -vm));
+        const float f = to_f32(z[edge(i)]), vm = fmaxf(m, f);
+        const Scale q = scale_of(vm, c);
+        s = moved(s, m, vm, c) + ex2(fmaf(f, q.c, vm == -INFINITY ? 0.f : -q.ref));
         m = vm;
       }
-      warp_max_sum(m, s);
+      warp_max_sum(m, s, c);
       if (lane == 0) red[warp] = make_float2(m, s);
       __syncthreads();
       m = lane < kLongWarps ? red[lane].x : -INFINITY;
       s = lane < kLongWarps ? red[lane].y : 0.f;
-      warp_max_sum(m, s);
+      warp_max_sum(m, s, c);
       if (a.stats && tid == 0) a.stats[row] = make_float2(m, s);
     }
     if (g) {
       const float w = a.up_rows ? weight * a.up[row] : weight;
       const float scale = w / s;
+      const Scale by = scale_of(m, c);
       for (int i = tid; i < vecs; i += kLongThreads) {
         float f[VEC];
         unpack16<T>(*reinterpret_cast<const uint4*>(z + head + i * VEC), f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = empty ? 0.f : ex2(fmaf(f[j], c, -m)) * scale;
+        for (int j = 0; j < VEC; ++j) f[j] = empty ? 0.f : ex2(fmaf(f[j], by.c, -by.ref)) * scale;
         *reinterpret_cast<uint4*>(g + head + i * VEC) = pack16<T>(f);
       }
-      for (int i = tid; i < rest; i += kLongThreads) g[edge(i)] = from_f32<T>(empty ? 0.f : ex2(fmaf(to_f32(z[edge(i)]), c, -m)) * scale);
+      for (int i = tid; i < rest; i += kLongThreads) g[edge(i)] = from_f32<T>(empty ? 0.f : ex2(fmaf(to_f32(z[edge(i)]), by.c, -by.ref)) * scale);
       __syncthreads();
       for (int k = tid; k < a.K; k += kLongThreads) {
         const int i = __float_as_int(entries[k].y);
@@ -562,14 +585,15 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
             first = first && o >= k;
             p += ex2(entries[o].x);
           }
-        if (first) g[i] = from_f32<T>((ex2(fmaf(to_f32(z[i]), c, -m)) / s - p) * w);
+        if (first) g[i] = from_f32<T>((ex2(fmaf(to_f32(z[i]), by.c, -by.ref)) / s - p) * w);
       }
     }
     __syncthreads();
   }
 }
 
-// The losses, a warp to a row, from the rows' references and sums; the last CTA to finish makes their mean over the rows that have a teacher, or their sum.
+// The losses, a warp to a row, from the rows' maxima m and sums: log q = (z - m) / T - log sum e^((z' - m) / T), where what the reference's rounding took from the
+// sum's exponents is put back (logits of a type's lowest value stay finite so); the last CTA to finish makes their mean over the rows that have a teacher, or their sum.
 template <typename T>
 __global__ void __launch_bounds__(256) distill_loss_kernel(DistillArgs a, float* out, unsigned* finished) {
   pdl_launch_dependents();
@@ -582,18 +606,20 @@ __global__ void __launch_bounds__(256) distill_loss_kernel(DistillArgs a, float*
     const T* z = static_cast<const T*>(a.z) + (long long)row * a.ldz;
     const float2* entries = a.entries + (long long)row * a.K;
     const float2 q = a.stats[row];
-    const float ls = log2f(q.y);
+    constexpr float kLn2 = 0.6931471805599453f;
+    const Scale by = scale_of(q.x, a.c);
+    const float base = kLn2 * (log2f(q.y) - fmaf(q.x, by.c, -by.ref)), inv = 1.f / a.temperature;
     float part = 0.f;
 #pragma unroll 4
     for (int k = lane; k < a.K; k += 32) {
       const float2 e = entries[k];
       const int i = __float_as_int(e.y);
       const float x = i >= 0 ? to_f32(z[i]) : 0.f, p = ex2(e.x);
-      if (i >= 0 && !(p == 0.f)) part += p * (e.x - (fmaf(x, a.c, -q.x) - ls));
+      if (i >= 0 && !(p == 0.f)) part += p * (fmaf(kLn2, e.x, base) - (x - q.x) * inv);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-    if (lane == 0) a.loss[row] = part * 0.6931471805599453f * a.temperature * a.temperature;
+    if (lane == 0) a.loss[row] = part * a.temperature * a.temperature;
   }
   if (!out) return;
   __threadfence();
@@ -705,7 +731,7 @@ int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t
                unsigned char* flags, const float* up, int up_rows, int skip_one, float* stats, int have_stats, float* loss, float* out, void* grad, long long ldg,
                void* stream) {
   using namespace lt;
-  if (type < 0 || type > 2 || t_type < 0 || t_type > 2 || N < 0 || V < 1 || K < 1 || K > kDistillTop || !(temperature > 0.f) || (out && !loss) || (loss && (!stats || !t)) ||
+  if (type < 0 || type > 2 || t_type < 0 || t_type > 2 || N < 0 || N >= 1 << 30 || V < 1 || V >= 1 << 30 || K < 1 || K > kDistillTop || !(temperature >= 0x1p-60f && temperature <= 0x1p60f) || (out && !loss) || (loss && (!stats || !t)) ||
       (reinterpret_cast<uintptr_t>(entries) & 7) != 0)
     return -int(kStatusBadArgument);
   if (N == 0) return 0;

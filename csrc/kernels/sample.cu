@@ -353,6 +353,7 @@ __device__ __noinline__ void sample_general(const SampleArgs& a, const SampleRow
       for (int i = 0; i < per; ++i) own += bin(i);
       const u64 incl = warp_scan64(own, lane);
       if (lane == 31) sh.wsum[warp] = incl;
+      if (threadIdx.x == 0) { sh.found[0] = 0; sh.found[1] = above; }        // (always found below; whatever the sums say, the interval becomes shorter)
       __syncthreads();
       u64 before = above + incl - own;
       for (int w = 0; w < warp; ++w) before += sh.wsum[w];

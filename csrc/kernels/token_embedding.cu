@@ -445,7 +445,7 @@ extern "C" {
 // out[n, D] = scale * table[idx] of fp32 (type 0), bf16 (1) or fp16 (2) elements; zeros where a token is outside [0, V).  idx32: the tokens are 32-bit.
 int lt_token_embedding_fwd(int type, const void* idx, int idx32, const void* table, void* out, long long n, int D, int V, float scale, void* stream) {
   using namespace lt;
-  if (type < 0 || type > 2 || n < 0 || D < 0 || V < 1) return -int(kStatusBadArgument);
+  if (type < 0 || type > 2 || n < 0 || D < 0 || D > 1 << 30 || V < 1) return -int(kStatusBadArgument);
   if (n == 0 || D == 0) return 0;
   if (n > 0x7fffffffll) return -int(kStatusBadArgument);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -460,7 +460,7 @@ int lt_token_embedding_fwd(int type, const void* idx, int idx32, const void* tab
 int lt_token_embedding_bwd(int type, const void* idx, int idx32, const void* dout, long long ldd, void* grad, long long n, int D, int V, float scale, long long pad,
                            void* order, float* part, int tile, void* stream) {
   using namespace lt;
-  if (type < 0 || type > 2 || n < 0 || n > 0x7fffffffll - 4096 || D < 0 || V < 1 || V == 0x7fffffff || tile < 1 || tile > kMaxTile) return -int(kStatusBadArgument);
+  if (type < 0 || type > 2 || n < 0 || n > 0x7fffffffll - 4096 || D < 0 || D > 1 << 30 || V < 1 || V == 0x7fffffff || tile < 1 || tile > kMaxTile) return -int(kStatusBadArgument);
   if (D == 0) return 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int m = int(n);

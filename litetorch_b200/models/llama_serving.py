@@ -19,7 +19,7 @@ import torch
 
 from ..serving import PagedKVCache
 from .llama import LlamaEngine
-from .serving_base import Sampler, ServingModel, _ints, generate          # noqa: F401  (their names live here as well)
+from .serving_base import Sampler, ServingModel, TokenSampler, _ints, generate          # noqa: F401  (their names live here as well)
 
 
 class LlamaKVModel(ServingModel):

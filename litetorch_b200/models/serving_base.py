@@ -18,12 +18,15 @@ for, ends when everything before it has run.
 """
 from __future__ import annotations
 
+import contextlib
 import gc
 from operator import index
 from typing import List, Optional, Sequence
 
 import numpy as np
 import torch
+
+from ..ops.functional import sample_tokens
 
 
 def _ints(values: Sequence[int], n: int, dtype=np.int32) -> np.ndarray:
@@ -43,7 +46,7 @@ class ServingModel:
         self.block_size = block_size
         self.graphs = graphs                 # record the decode step per (batch size, table width) and replay it
         self._graphs = {}
-        self.sampler = None                  # None: greedy on the device; else a callable logits [rows, vocab] -> tokens
+        self._sampler = None
         self.last_logits = None              # [rows, vocab] of the newest step (kept for inspection and tests)
         self.prefill_tokens_computed = 0
         self.prefill_tokens_reused = 0
@@ -64,8 +67,21 @@ class ServingModel:
         return host
 
     # ------------------------------------------------------------------ tokens from logits
+    @property
+    def sampler(self):
+        """None: greedy on the device; else a callable logits [rows, vocab] -> tokens (`Sampler`: eager steps only), or a `TokenSampler`."""
+        return self._sampler
+
+    @sampler.setter
+    def sampler(self, sampler):
+        if sampler is not self._sampler:
+            self._graphs.clear()                               # recorded steps pick their tokens as the one before did
+        self._sampler = sampler
+
     def _pick(self, logits: torch.Tensor) -> torch.Tensor:
         self.last_logits = logits
+        if isinstance(self.sampler, TokenSampler):
+            return self.sampler(logits)
         if self.sampler is not None:
             return self.sampler(logits.float())
         return self.e.K.argmax_rows(logits)
@@ -97,6 +113,12 @@ class ServingModel:
         """(logits [S, vocab], next tokens [S]).  On a GPU the step's launches are recorded once per (batch size,
         block-table width) into a CUDA graph and replayed: the step then costs its kernels, not their launch overhead.  The
         inputs of a replay are copied into the graph's static input block first."""
+        if isinstance(self.sampler, TokenSampler):
+            with self.sampler.drawn(len(last_tokens), self.e.device):
+                return self._run_step(last_tokens, positions, block_tables, slots)
+        return self._run_step(last_tokens, positions, block_tables, slots)
+
+    def _run_step(self, last_tokens, positions, block_tables, slots):
         dev = self.e.device
         S = len(last_tokens)
         bs = self.block_size
@@ -243,23 +265,69 @@ class Sampler:
         return torch.multinomial(torch.softmax(z, -1), 1, generator=self.gen).squeeze(-1)
 
 
+class TokenSampler:
+    """Temperature / top-k / nucleus / min-p sampling of next tokens from logits [rows, vocab] by `functional.sample_tokens`, with random numbers of its own
+    generator, so that a run is reproducible from its seed.  Every parameter is a number, or a tensor of one number on the device that recorded steps read anew.
+    A recorded step takes its random numbers from a place that `drawn` fills before every replay.  `logprobs` are those of the newest tokens."""
+
+    def __init__(self, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0, device="cpu"):
+        for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+            if isinstance(v, torch.Tensor) and v.dim() > 0:
+                raise ValueError("TokenSampler: one %s for all rows is expected (functional.sample_tokens takes one for every row)" % name)
+        self.params = temperature, top_k, top_p, min_p
+        self.gen = torch.Generator(device=device).manual_seed(int(seed))
+        self._places = {}                                 # rows -> random numbers and log probabilities of a decode step
+        self._given = None
+        self.logprobs = None
+
+    def _draw(self, rows: int) -> torch.Tensor:
+        return torch.rand(rows, generator=self.gen, device=self.gen.device)
+
+    @contextlib.contextmanager
+    def drawn(self, rows: int, device):
+        """The calls within take these random numbers, drawn now."""
+        place = self._places.get(rows)
+        if place is None:
+            place = self._places[rows] = torch.empty(2, rows, dtype=torch.float32, device=device)
+        place[0].copy_(self._draw(rows))
+        self._given = place
+        try:
+            yield
+        finally:
+            self._given = None
+        self.logprobs = place[1]
+
+    def __call__(self, logits: torch.Tensor) -> torch.Tensor:
+        if self._given is None:
+            tokens, self.logprobs = sample_tokens(logits, self._draw(logits.shape[0]).to(logits.device), *self.params)
+            return tokens
+        tokens, logprobs = sample_tokens(logits, self._given[0], *self.params)
+        self._given[1].copy_(logprobs)                    # (a replay runs no Python: the step's numbers have one place)
+        return tokens
+
+
 @torch.no_grad()
 def generate(engine, prompts: Sequence[Sequence[int]], max_new_tokens: int, *, temperature: float = 0.0,
              top_k: int = 0, top_p: float = 1.0, seed: int = 0, eos_id: int = -1, block_size: int = 16,
              max_num_seqs: int = 64, max_num_batched_tokens: int = 4096, kv_dtype=None,
-             prefix_cache_bytes: int = 0) -> List[List[int]]:
+             prefix_cache_bytes: int = 0, min_p: float = 0.0, sampler: str = "torch") -> List[List[int]]:
     """Continue every prompt by up to `max_new_tokens` tokens (stopping at `eos_id`) with continuous batching on a paged KV
     cache sized for the request, and return the new tokens per prompt.  Greedy by default (the decode step is replayed
-    from CUDA graphs on a GPU); with `temperature > 0` the next tokens are drawn by `Sampler` (eager decode steps).
+    from CUDA graphs on a GPU); with `temperature > 0` the next tokens are drawn by `Sampler` (eager decode steps), or, with
+    `sampler="kernel"` or a `min_p`, by `TokenSampler` in the recorded step (its own random numbers: other tokens for the same seed).
     `engine`: any engine of `models.registry`."""
     from ..serving import Request, ServingScheduler
     from .registry import new_serving
     need = sum((len(p) + max_new_tokens + block_size - 1) // block_size for p in prompts)
     greedy = temperature <= 0.0 or top_k == 1
+    if sampler not in ("torch", "kernel"):
+        raise ValueError("generate: sampler %r" % (sampler,))
+    kernel = sampler == "kernel" or min_p > 0.0
     model = new_serving(engine, num_blocks=need + 1, block_size=block_size, max_num_seqs=max_num_seqs, kv_dtype=kv_dtype,
-                        graphs=greedy, prefix_cache_bytes=prefix_cache_bytes)  # prompts of one call that share a prefix reuse its blocks
+                        graphs=greedy or kernel, prefix_cache_bytes=prefix_cache_bytes)  # prompts of one call that share a prefix reuse its blocks
     if not greedy:
-        model.sampler = Sampler(temperature, top_k, top_p, seed, device=engine.device)
+        model.sampler = (TokenSampler(temperature, top_k, top_p, min_p, seed, device=engine.device) if kernel
+                         else Sampler(temperature, top_k, top_p, seed, device=engine.device))
     sched = ServingScheduler(num_blocks=need + 1, block_size=block_size, max_num_seqs=max_num_seqs,
                              max_num_batched_tokens=max_num_batched_tokens, eos_id=eos_id)
     limit = engine.cfg.max_seq                            # None: the model's positions have no end

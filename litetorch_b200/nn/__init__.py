@@ -189,14 +189,18 @@ class QLoRALinear(Module):
 
 
 class Embedding(Module):
-    """Rows of an N(0,1)-initialised table; indices may be floats (src/nn/embedding.cpp:30-160)."""
+    """Rows of an N(0,1)-initialised table; indices may be floats (src/nn/embedding.cpp:30-160).  With a scale, a padding index (whose row gets no gradient)
+    or `sorted_grad` the gradient is summed by sorted tokens in fp32 (`functional.token_embedding`)."""
 
-    def __init__(self, num_embeddings: int, embedding_dim: int):
+    def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: Optional[int] = None, sorted_grad: bool = False):
         super().__init__()
         self.num_embeddings, self.embedding_dim = num_embeddings, embedding_dim
+        self.scale, self.padding_idx, self.sorted_grad = scale, padding_idx, sorted_grad or scale != 1.0 or padding_idx is not None
         self.weight = _param(torch.randn(num_embeddings, embedding_dim))
 
     def forward(self, idx: Tensor) -> Tensor:
+        if self.sorted_grad:
+            return Tensor(Fn.token_embedding(_unwrap(idx).to(torch.int64), _unwrap(self.weight), self.scale, self.padding_idx))
         return Tensor(Fn.embedding(_unwrap(idx).to(torch.int64), _unwrap(self.weight)))
 
 
@@ -383,6 +387,17 @@ class MSELoss(Module):
 
 class CrossEntropyLoss(Module):
     def forward(self, x, y): return Ops.cross_entropy_loss(x, y)
+
+
+class DistillationLoss(Module):
+    """`Ops.distillation_loss` of logits against a teacher's top logits and their classes."""
+
+    def __init__(self, temperature: float = 1.0, reduction: str = "mean"):
+        super().__init__()
+        self.temperature, self.reduction = temperature, reduction
+
+    def forward(self, logits, teacher_logits, teacher_idx):
+        return Ops.distillation_loss(logits, teacher_logits, teacher_idx, self.temperature, self.reduction)
 
 
 class BCELoss(Module):

@@ -247,11 +247,33 @@ class Ops:
         return _w((total / N).reshape(1))
 
     @staticmethod
+    def distillation_loss(logits, teacher_logits, teacher_idx, temperature: float = 1.0, reduction: str = "mean"):
+        """Kullback-Leibler distance of a student's logits [..., V] from a teacher of whom the top K logits [..., K] are known, at the classes
+        teacher_idx [..., K] (floats or integers; -1: not there), times temperature^2; `functional.distillation_loss` has the formula."""
+        it = _unwrap(teacher_idx)
+        loss = Fn.distillation_loss(_unwrap(logits), _unwrap(teacher_logits), it.to(torch.int64) if it.is_floating_point() else it, temperature, reduction)
+        return _w(loss if reduction == "none" else loss.reshape(1))
+
+    @staticmethod
     def clip_grad_norm_(params: Sequence[Tensor], max_norm: float, norm_type: float = 2.0) -> float:
         ts = [_unwrap(p) for p in params if _unwrap(p).grad is not None]
         if not ts:
             return 0.0
         return float(torch.nn.utils.clip_grad_norm_(ts, max_norm, norm_type))
+
+    # ------------------------------------------------------------------ tokens
+    @staticmethod
+    def embedding(idx, table, scale: float = 1.0, padding_idx: Optional[int] = None):
+        """scale * table[idx] (indices may be floats); the table's gradient is summed by sorted tokens in fp32, none of it for `padding_idx`."""
+        it = _unwrap(idx)
+        return _w(Fn.token_embedding(it.to(torch.int64) if it.is_floating_point() else it, _unwrap(table), scale, padding_idx))
+
+    @staticmethod
+    def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Tuple[Tensor, Tensor]:
+        """(tokens, log probabilities) of logits [..., V], drawn with the random numbers uniform [...] in [0, 1); every parameter is a number or a tensor with
+        one for every row (`functional.sample_tokens` says what they do)."""
+        tokens, logprobs = Fn.sample_tokens(_unwrap(logits), _unwrap(uniform), *(_unwrap(v) if isinstance(v, Tensor) else v for v in (temperature, top_k, top_p, min_p)))
+        return _w(tokens), _w(logprobs)
 
     # ------------------------------------------------------------------ transformer ops
     @staticmethod

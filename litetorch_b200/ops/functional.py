@@ -532,8 +532,8 @@ def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0, 
         idx = idx.to(torch.int64)
     if idx.device != table.device:
         raise ValueError("token_embedding: tokens on %s, table on %s" % (idx.device, table.device))
-    if V < 1 or V >= (1 << 31) - 1 or D >= 1 << 31 or idx.numel() > (1 << 31) - 4097:
-        raise ValueError("token_embedding: a table of 1 to 2^31 - 2 rows and fewer than 2^31 - 4096 tokens are expected")
+    if V < 1 or V >= (1 << 31) - 1 or D > 1 << 30 or idx.numel() > (1 << 31) - 4097:
+        raise ValueError("token_embedding: a table of 1 to 2^31 - 2 rows of up to 2^30 columns and fewer than 2^31 - 4096 tokens are expected")
     pad = -1
     if padding_idx is not None:
         if not -V <= padding_idx < V:
@@ -594,13 +594,13 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         raise ValueError("distillation_loss: student and teacher are on different devices")
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("distillation_loss: reduction %r" % (reduction,))
-    if not (0.0 < temperature < math.inf):
-        raise ValueError("distillation_loss: a temperature above 0 is expected, not %r" % (temperature,))
+    if not 2.0 ** -60 <= temperature <= 2.0 ** 60:
+        raise ValueError("distillation_loss: a temperature above 0 (2^-60 to 2^60) is expected, not %r" % (temperature,))
     V, top = logits.shape[-1], teacher_idx.shape[-1]
     if not 1 <= top <= 1024 or V < 1:
         raise ValueError("distillation_loss: 1 to 1024 of the teacher's logits and at least one class are expected")
     lead, rows = logits.shape[:-1], teacher_idx.numel() // top
-    if rows >= 1 << 31 or V >= 1 << 30:
+    if rows >= 1 << 30 or V >= 1 << 30:
         raise ValueError("distillation_loss: too many rows or classes")
     z, t, idx = logits, teacher_logits, teacher_idx
     if logits.dim() != 2:
@@ -612,8 +612,9 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         t = t.detach()
         there = (idx >= 0) & (idx < V) & (t != -math.inf)
         has = there.any(1)
-        log_p = torch.log_softmax((t.to(wide) / temperature).masked_fill(~there, -math.inf).masked_fill(~has[:, None], 0.0), -1)
-        log_q = torch.log_softmax(z.to(wide) / temperature, -1).gather(1, idx.to(torch.int64).clamp(0, V - 1))
+        below = lambda x: (x - x.detach().amax(1, keepdim=True)) / temperature         # (the largest is taken off first: the type's lowest value has a quotient then)
+        log_p = torch.log_softmax(below(t.to(wide).masked_fill(~there, -math.inf).masked_fill(~has[:, None], 0.0)), -1)
+        log_q = torch.log_softmax(below(z.to(wide)), -1).gather(1, idx.to(torch.int64).clamp(0, V - 1))
         p = log_p.exp().masked_fill(~there, 0.0)
         counts = p != 0
         loss = (p * (torch.where(counts, log_p, 0.0) - torch.where(counts, log_q, 0.0))).sum(1) * temperature ** 2

@@ -1674,8 +1674,7 @@ def _like_rows(z):
     shift = z.data_ptr() % 16 // z.element_size()
     if shift == 0 and (ld == V or N <= 1):
         return torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    if ld < V:                                              # one row for several
-        ld = V + (ld - V) % each
+    ld = V + (ld - V) % each                                # (a slice of something large gets no gradient of that size)
     return torch.empty(shift + N * ld, dtype=z.dtype, device=z.device).as_strided((N, V), (ld, 1), shift)
 
 
@@ -1687,18 +1686,19 @@ def distill_loss(z, t, idx, temperature: float, reduction: str, with_grad: bool)
     z = z if z.stride(1) == 1 else z.contiguous()
     t, idx = t.contiguous(), (idx if idx.dtype == torch.int64 else idx.to(torch.int64)).contiguous()
     mean = reduction == "mean"
-    # [N, K, 2] entries and a counter, [N, 2] references and sums, [N] losses, [N] bytes
+    # [N, K, 2] entries and a counter, [N, 2] maxima and sums, [N] losses (those that go into one number), [N] bytes
     room = z.new_empty(N * (2 * top + 3) + 2 + (N + 3) // 4, dtype=torch.float32)
     at = room.data_ptr()
     stats = at + 8 * (N * top + 1)
     loss, flags = stats + 8 * N, stats + 12 * N
-    out = None if reduction == "none" else z.new_empty((), dtype=torch.float32)
+    out = z.new_empty((N,) if reduction == "none" else (), dtype=torch.float32)
+    rows = out.dim() > 0
     grad = _like_rows(z) if with_grad else None
     with _on(z):
         _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), _ELEM[t.dtype], t.data_ptr(), idx.data_ptr(), at, N, V, top, temperature,
-                                 flags if mean else None, None, 0, 0, stats, 0, loss, _p(out), _p(grad), 0 if grad is None else grad.stride(0), _stream()), "lt_distill")
+                                 flags if mean else None, None, 0, 0, stats, 0, out.data_ptr() if rows else loss, None if rows else out.data_ptr(), _p(grad), 0 if grad is None else grad.stride(0), _stream()), "lt_distill")
     _launches[0] += 2
-    return room[2 * (N * (top + 1) + 1):][:N] if out is None else out, grad, room
+    return out, grad, room
 
 
 def distill_grad(z, room, top: int, temperature: float, mean: bool, up, grad=None):

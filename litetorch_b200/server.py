@@ -10,7 +10,8 @@ for theirs to finish.  Standard library only.
     GET  /health     {"running": r, "pending": p, "free_blocks": f, "served": n}
     GET  /metrics    the same counters and the prefill token counts in the Prometheus text format
 
-Decoding is greedy (the decode step is replayed from CUDA graphs on a GPU).  The reference has the scheduler and no
+Decoding is greedy, or with `--temperature` (and `--top-k`, `--top-p`, `--min-p`) drawn; either way the decode step is replayed from CUDA
+graphs on a GPU.  The reference has the scheduler and no
 server around it (src/llm/continuous_batching.cpp); `EngineLoop` is that missing piece and is usable without HTTP:
 `loop.submit(prompt_ids, max_new_tokens)` returns the finished `Request`.
 """
@@ -230,6 +231,7 @@ def tokenizer(sentencepiece: str = "", byte_level: bool = False):
 def main(argv=None):
     import torch
     from .models import registry
+    from .models.serving_base import TokenSampler
     ap = argparse.ArgumentParser()
     ap.add_argument("--model", required=True, help="model directory (config.json + *.safetensors) of any registered family")
     ap.add_argument("--host", default="127.0.0.1")
@@ -243,10 +245,17 @@ def main(argv=None):
     ap.add_argument("--max-num-seqs", type=int, default=64)
     ap.add_argument("--max-batched-tokens", type=int, default=4096)
     ap.add_argument("--prefix-cache-mb", type=int, default=0, help="keep K / V of finished prompts for reuse by prompts that share a prefix")
+    ap.add_argument("--temperature", type=float, default=0.0, help="0: the likeliest token")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
+    ap.add_argument("--seed", type=int, default=0)
     args = ap.parse_args(argv)
     engine = registry.load_engine(args.model, args.device, getattr(torch, args.dtype))
     model = registry.new_serving(engine, num_blocks=args.kv_blocks, block_size=args.block_size, max_num_seqs=args.max_num_seqs,
                                  prefix_cache_bytes=args.prefix_cache_mb << 20)
+    if args.temperature > 0.0:
+        model.sampler = TokenSampler(args.temperature, args.top_k, args.top_p, args.min_p, args.seed, device=engine.device)
     encode, decode, eos = tokenizer(args.sentencepiece, args.bytes)
     loop = EngineLoop(model, args.kv_blocks, args.block_size, args.max_num_seqs, args.max_batched_tokens, eos_id=eos,
                       max_context=engine.cfg.max_seq)

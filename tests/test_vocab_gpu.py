@@ -423,3 +423,154 @@ def test_an_answer_is_drawn_read_and_learned_from():
     (T * T * (log_p.exp() * (log_p - torch.log_softmax(zz / T, 1).gather(1, top.indices))).sum(1).mean()).backward()
     # products over 64 and 500 numbers in 32 bits (torch's, without TF32): 500 roundings of 2^-24 of their sizes, which are within 8 of the largest gradient
     assert float((table.grad - w.grad).abs().max()) < 500 * 2.0 ** -24 * 8 * float(w.grad.abs().max()) + 1e-7
+
+
+# ---------------------------------------------------------------------------------------------- the lowest value, losses of one's own, slices
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [7, 1000, 1 << 19])
+def test_logits_of_the_lowest_value(dtype, V):
+    """Masks of the type's lowest value: parts of a row, all but one, all of it (then the student knows nothing), and the highest value against them."""
+    g = _gen(V)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    z = torch.randn(6, V, device="cuda", generator=g).to(dtype)
+    z[0, V // 2:] = low
+    z[1] = low
+    z[2] = low
+    z[2, 3] = 0.5
+    z[3, 5] = high
+    z[4] = high
+    z[5] = low
+    z[5, ::2] = -math.inf
+    t = torch.randn(6, 2, device="cuda", generator=g).to(dtype)
+    idx = torch.tensor([[0, 1], [0, V - 1], [3, -1], [5, -1], [1, V - 2], [1, 5]], device="cuda")
+    for T in (1.0, 0.3, 2.0, 2.0 ** 12, 2.0 ** -60):
+        _check_distill(z, t, idx, T, "none", torch.rand(6, device="cuda", generator=g))
+        _check_distill(z, t, idx, T, "mean")
+
+
+def test_a_row_of_its_own_for_every_loss():
+    from litetorch_b200.ops import functional as Fn
+    g = _gen(31)
+    z = torch.randn(4, 900, device="cuda", generator=g).requires_grad_()
+    t, cls = _teacher(4, 900, 2, torch.float32, g)
+    loss = Fn.distillation_loss(z, t, cls, reduction="none")
+    loss *= torch.tensor([1.0, 0.0, 2.0, 0.0], device="cuda")
+    loss.sum().backward()
+    assert not z.grad[1::2].any() and bool(z.grad[::2].any(1).all())
+
+
+def test_the_gradient_of_a_slice_is_of_the_slices_size():
+    """The last positions of long answers: neighbouring rows lie far apart, those of their gradient do not."""
+    from litetorch_b200.ops import functional as Fn
+    g = _gen(32)
+    room = torch.randn(3, 500, 1003, device="cuda", generator=g).bfloat16()
+    t, cls = _teacher(3, 1003, 2, torch.bfloat16, g)
+    z = room[:, -1].requires_grad_()
+    _check_distill(z, t, cls, 1.0, "mean")
+    loss = Fn.distillation_loss(z, t, cls)
+    before = torch.cuda.memory_allocated()
+    grad, = torch.autograd.grad(loss, z)
+    assert grad.untyped_storage().nbytes() < 3 * 1020 * 2 and torch.cuda.memory_allocated() - before < 1 << 16
+
+
+def test_more_rows_than_the_gpu_holds_clusters():
+    g = _gen(33)
+    z = torch.randn(5000, 301, device="cuda", generator=g).half()
+    t, cls = _teacher(5000, 301, 3, torch.float16, g, ragged=True)
+    _check_distill(z, t, cls, 1.0, "mean")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_longer_rows_than_a_cluster_holds(dtype):
+    g = _gen(34)
+    z = torch.randn(3, 300001, device="cuda", generator=g).to(dtype)
+    z[1, 1000:] = -math.inf
+    t, cls = _teacher(3, 300001, 9, dtype, g)
+    cls[1] %= 1000
+    cls[2, 5:] = cls[2, :4]
+    _check_distill(z, t, cls, 1.3, "sum")
+    _check_distill(z, t, cls, 1.3, "none", torch.rand(3, device="cuda", generator=g))
+
+
+def test_two_streams_at_once():
+    """Calls of the same kind on two streams have nothing in common."""
+    from litetorch_b200.ops import functional as Fn
+    g = _gen(35)
+    V, N, D = 5003, 700, 96
+    args = []
+    for _ in range(2):
+        t, cls = _teacher(N, V, 5, torch.float32, g)
+        args.append((torch.randint(0, V, (N,), device="cuda", generator=g), torch.randn(V, D, device="cuda", generator=g), torch.randn(N, D, device="cuda", generator=g),
+                     torch.randn(N, V, device="cuda", generator=g), t, cls, torch.rand(N, device="cuda", generator=g)))
+
+    def work(idx, table, dout, z, t, cls, u):
+        w, s = table.detach().requires_grad_(), z.detach().requires_grad_()
+        loss = Fn.distillation_loss(s, t, cls, 2.0)
+        return [torch.autograd.grad(Fn.token_embedding(idx, w), w, dout)[0], loss.detach(), torch.autograd.grad(loss, s)[0], *Fn.sample_tokens(z, u, 0.8, 0, 0.9)]
+    want = [work(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    got = [None, None]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = work(*args[i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(want, got) for a, b in zip(x, y))
+
+
+# ---------------------------------------------------------------------------------------------- served models
+def _engine():
+    from litetorch_b200.models.llama import LlamaConfig, LlamaEngine
+    return LlamaEngine(LlamaConfig(vocab_size=512, n_layers=2, d_model=128, n_heads=4, n_kv_heads=2, head_dim=64, ffn=256, max_seq=256), "cuda", seed=2)
+
+
+def test_recorded_steps_draw_anew():
+    """A recorded decode step takes other random numbers at each replay, and its tokens are those of its own logits; another sampler records another step."""
+    from litetorch_b200.models import registry
+    from litetorch_b200.models.serving_base import TokenSampler
+    model = registry.new_serving(_engine(), num_blocks=64, block_size=16, max_num_seqs=8)
+    model.sampler = s = TokenSampler(30.0, 100, 0.98, 0.0, seed=7, device="cuda")
+    first = [model.prefill_chunk(list(range(10 + i, 20 + i)), 0, [i], True) for i in range(4)]
+    assert all(0 <= t < 512 for t in first)
+    drawn = set()
+    for _ in range(2):
+        for rows in (4, 2, 4):                                    # graphs of two sizes in turn
+            tokens = model.decode_batch(first[:rows], [10] * rows, [[i] for i in range(rows)])
+            u = s._places[rows][0]
+            want, logs = ref.sample(model.last_logits, u, 30.0, 100, 0.98, 0.0)
+            assert tokens == want.tolist()
+            _within(s.logprobs, logs, logs.abs() * 2.0 ** -23 + 1e-9)
+            drawn.add(tuple(u.tolist()))
+    assert len(drawn) == 6 and set(model._graphs) == {(4, 16), (2, 16)}
+    model.sampler = TokenSampler(0.0)
+    assert not model._graphs
+    assert model.decode_batch(first, [10] * 4, [[i] for i in range(4)]) == model.last_logits.float().argmax(1).tolist()
+    model.sampler = None
+    assert model.decode_batch(first, [10] * 4, [[i] for i in range(4)]) == model.last_logits.float().argmax(1).tolist()
+
+
+def test_parameters_on_the_device_are_read_at_every_replay():
+    from litetorch_b200.models import registry
+    from litetorch_b200.models.serving_base import TokenSampler
+    model = registry.new_serving(_engine(), num_blocks=64, block_size=16, max_num_seqs=8)
+    k = torch.ones((), dtype=torch.int32, device="cuda")
+    model.sampler = s = TokenSampler(50.0, k, seed=7, device="cuda")
+    first = model.prefill_chunk(list(range(10)), 0, [0], True)
+    seen = set()
+    for n in (1, 1, 200, 200, 200):
+        k.fill_(n)
+        token, = model.decode_batch([first], [10], [[0]])
+        assert token == ref.sample(model.last_logits, s._places[1][0], 50.0, n, 1.0, 0.0)[0].item()
+        seen.add(token)
+    assert len(seen) > 1
+
+
+def test_generate_is_seeded_and_greedy_at_its_limits():
+    from litetorch_b200.models.llama_serving import generate
+    engine = _engine()
+    prompts = [[5, 6, 7], [9, 10, 11, 12, 13]]
+    greedy = generate(engine, prompts, 12)
+    a = [generate(engine, prompts, 12, temperature=20.0, top_k=100, seed=seed, sampler="kernel") for seed in (1, 1, 2)]
+    assert a[0] == a[1] != a[2] and a[0] != greedy
+    assert all(len(o) == 12 and all(0 <= t < 512 for t in o) for o in a[2])
