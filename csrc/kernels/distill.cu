@@ -87,8 +87,12 @@ __global__ void __launch_bounds__(256) distill_teacher_kernel(const void* t, int
 }
 
 __device__ __forceinline__ int count_flags(const unsigned char* flags, int N, int* red) {
-  int n = 0;
-  for (int i = threadIdx.x; i < N; i += blockDim.x) n += flags[i];
+  int n = 0;                                                  // (flags are 0 or 1, and lie at 16 bytes)
+  for (int i = threadIdx.x; i < N / 16; i += blockDim.x) {
+    const uint4 u = reinterpret_cast<const uint4*>(flags)[i];
+    n += __popc(u.x) + __popc(u.y) + __popc(u.z) + __popc(u.w);
+  }
+  for (int i = N / 16 * 16 + threadIdx.x; i < N; i += blockDim.x) n += flags[i];
   n = __reduce_add_sync(0xffffffffu, n);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
   __syncthreads();
@@ -105,24 +109,35 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 // Powers of two are taken of z c - ref, with ref = c times the largest logit m: z enters as fma(z, c, -ref), so that the reference is exact whatever its own
 // rounding (which scales all of a row's powers alike, by up to 2^64 here).  From |ref| = 2^31 on (masks of the type's lowest value everywhere, say) what lies
-// below m lies 128 or more below it and weighs nothing: any factor does that leaves its multiples finite and far apart, so it is the power of two that brings m to
-// 2^60.
-struct Scale {
-  float c, ref;
-};
-__device__ __forceinline__ bool far_out(float ref) { return fabsf(ref) >= 0x1p31f; }
-__device__ __forceinline__ Scale scale_of(float m, float c) {
-  Scale q{c, __fmul_rn(m, c)};
-  if (far_out(q.ref) && fabsf(m) != INFINITY) {
-    q.c = __uint_as_float((314u - (__float_as_uint(m) >> 23 & 255u)) << 23);
-    q.ref = m * q.c;
-  }
-  return q;
-}
+// below m lies 128 or more below it: such a row is far out, and nothing but the equals of m weighs anything.
+__device__ __forceinline__ bool far_out(float m, float ref) { return fabsf(ref) >= 0x1p31f && fabsf(m) != INFINITY; }
+// The weight of a logit of a row that is far out (NaN stays).
+__device__ __forceinline__ float far_weight(float f, float m) { return f == m ? 1.f : f != f ? f : 0.f; }
 // A sum that belongs to the maximum `own` as one that belongs to m.
 __device__ __forceinline__ float moved(float s, float own, float m, float c) {
-  const float ref = __fmul_rn(m, c);                          // (not contracted: as scale_of rounds it)
-  return own == m || own == -INFINITY ? s : s * (far_out(ref) ? 0.f : ex2(__fmul_rn(own, c) - ref));
+  const float ref = __fmul_rn(m, c);                          // (not contracted: all round it alike)
+  if (own == -INFINITY) return s;
+  if (far_out(m, ref)) return own == m ? s : s * 0.f;
+  return s * ex2(__fmul_rn(own, c) - ref);
+}
+template <typename T>
+__device__ __noinline__ float far_sum(const uint4* mine, int vpt, float m) {
+  float s = 0.f;
+  for (int k = 0; k < vpt; ++k) {
+    float f[kVec<T>];
+    unpack16<T>(mine[k * 32], f);
+#pragma unroll
+    for (int j = 0; j < kVec<T>; ++j) s += far_weight(f[j], m);
+  }
+  return s;
+}
+template <typename T>
+__device__ __noinline__ uint4 far_gradient(uint4 u, float m, float scale) {
+  float f[kVec<T>];
+  unpack16<T>(u, f);
+#pragma unroll
+  for (int j = 0; j < kVec<T>; ++j) f[j] = far_weight(f[j], m) * scale;
+  return pack16<T>(f);
 }
 // (maximum, sum) over the warp.
 __device__ __forceinline__ void warp_max_sum(float& m, float& s, float c) {
@@ -231,13 +246,10 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
   __shared__ uint4 cut[2];                                    // the row's first and last vector, if they are cut
   __shared__ int isum[kDistillWarps];
   __shared__ int abort_flag;
-  pdl_launch_dependents();
   pdl_wait();
   if (a.skip_one && a.up && a.up[0] == 1.f) return;
-  float weight = a.temperature;
-  if (a.flags) weight /= float(max(1, count_flags(a.flags, a.N, isum)));
-  if (a.up && !a.up_rows) weight *= a.up[0];
   const float c = a.c;
+  const uint64_t c2 = pack_f32x2(c, c);
   const int tid = threadIdx.x, lane = tid & 31, nt = blockDim.x, nw = nt >> 5;
   const int clog = a.cluster_log, rank = clog ? int(cluster_ctarank()) : 0;
   const int vpt = a.vpt, room = vpt * nt;
@@ -313,6 +325,9 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
   };
   __syncthreads();
   for (int i = 0; i < S::kVectors; ++i) fetch(i, i);
+  float weight = a.temperature;
+  if (a.flags) weight /= float(max(1, count_flags(a.flags, a.N, isum)));
+  if (a.up && !a.up_rows) weight *= a.up[0];
   if (clog) cluster_sync_all();                               // every CTA is there to be written to
   int cur = 0, prev = 2;                                      // places of the first pass's vectors and of the second's
   int entry_cur = 0;                                          // place of the first pass's entries
@@ -353,10 +368,9 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
         float m = -INFINITY;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) m = fmaxf(m, max16<T>(u[k]));
-        const Scale q = scale_of(m, c);
-        const float from = m == -INFINITY ? 0.f : -q.ref;
+        const float ref = __fmul_rn(m, c), from = m == -INFINITY ? 0.f : -ref;
         uint64_t part[VEC / 2];
-        const uint64_t from2 = pack_f32x2(from, from), c2 = pack_f32x2(q.c, q.c);
+        const uint64_t from2 = pack_f32x2(from, from);
 #pragma unroll
         for (int j = 0; j < VEC / 2; ++j) part[j] = 0ull;
 #pragma unroll
@@ -377,6 +391,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
         float s, s1;
         unpack_f32x2(part[0], s, s1);
         s += s1;
+        if (far_out(m, ref)) s = far_sum<T>(mine, vpt, m);
         warp_max_sum(m, s, c);
         const int at = (turn * kDistillCluster + rank) * nw + (tid >> 5);
         if (clog) {
@@ -418,17 +433,23 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
           }
         }
         m = warp_max(m);
+        const float ref = __fmul_rn(m, c);
+        if (!far_out(m, ref)) {
 #pragma unroll
-        for (int i = 0; i < kDistillCluster * kDistillWarps / 32; ++i)
-          if (i * 32 < pairs) s += moved(q[i].y, q[i].x, m, c);
+          for (int i = 0; i < kDistillCluster * kDistillWarps / 32; ++i)
+            if (i * 32 < pairs) s += q[i].y * ex2(__fmul_rn(q[i].x, c) - ref);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kDistillCluster * kDistillWarps / 32; ++i) s += q[i].x == m ? q[i].y : q[i].y * 0.f;
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (a.stats && rank == 0 && tid == 0) a.stats[old] = make_float2(m, s);
       }
       if (a.grad) {
         T* g = static_cast<T*>(a.grad) + (long long)old * a.ldg;
-        const float w = a.up_rows ? weight * a.up[old] : weight, scale = __fdividef(w, s);
-        const Scale by = scale_of(m, c);
+        const float w = a.up_rows ? weight * a.up[old] : weight, scale = __fdividef(w, s), ref = __fmul_rn(m, c);
+        const bool far = far_out(m, ref);
         T* to = g - r.shift + (r.lo + first) * VEC;
         const int end = r.end - r.lo - first;
         const bool cuts = !EVEN && (r.shift != 0 || r.vecs * VEC != a.V);
@@ -444,18 +465,18 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
 #pragma unroll
           for (int j = 0; j < VEC / 2; ++j) {
             float x, y;
-            unpack_f32x2(fma_f32x2(pack_f32x2(f[2 * j], f[2 * j + 1]), pack_f32x2(by.c, by.c), pack_f32x2(-by.ref, -by.ref)), x, y);
+            unpack_f32x2(fma_f32x2(pack_f32x2(f[2 * j], f[2 * j + 1]), c2, pack_f32x2(-ref, -ref)), x, y);
             unpack_f32x2(mul_f32x2(pack_f32x2(ex2(x), ex2(y)), pack_f32x2(scale, scale)), f[2 * j], f[2 * j + 1]);
           }
           return pack16<T>(f);
         };
-        if (!empty && full(r)) {
+        if (!empty && !far && full(r)) {
           uint4 u[VPT];
 #pragma unroll
           for (int k = 0; k < VPT; ++k) u[k] = mine[k * 32];
 #pragma unroll
           for (int k = 0; k < VPT; ++k) *reinterpret_cast<uint4*>(to + k * 32 * VEC) = gradient(u[k]);
-        } else if (!empty) {
+        } else if (!empty && !far) {
 #pragma unroll 1
           for (int k = 0; k < vpt; ++k) {
             if (k * 32 < end) {
@@ -465,7 +486,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
         } else {
 #pragma unroll 1
           for (int k = 0; k < vpt; ++k)
-            if (k * 32 < end) store(k, make_uint4(0u, 0u, 0u, 0u));
+            if (k * 32 < end) store(k, empty ? make_uint4(0u, 0u, 0u, 0u) : far_gradient<T>(mine[k * 32], m, scale));
         }
         if (cuts) {                                           // cut vectors by their elements
           if (head == 0 && end > 0)
@@ -489,7 +510,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
                 float p = ex2(entries[e - 1].x);
                 if (link[e - 1]) p = chained_p(entries, link, e, p);
                 const float x = to_f32(reinterpret_cast<const T*>(mine + v * 32)[j]);
-                g[i] = from_f32<T>((__fdividef(ex2(fmaf(x, by.c, -by.ref)), s) - p) * w);
+                g[i] = from_f32<T>((__fdividef(far ? far_weight(x, m) : ex2(fmaf(x, c, -ref)), s) - p) * w);
               }
             }
           }
@@ -502,6 +523,9 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
     cur = cur == S::kVectors - 1 ? 0 : cur + 1;
     entry_cur = entry_cur == S::kEntries - 1 ? 0 : entry_cur + 1;
   }
+  // (not earlier: CTAs of the next launch, which a CTA of this one leaves no registers, would gather on the few SMs that end first, and the losses then
+  // take 24 us instead of 9, 2048 x 32000 with 128 entries a row)
+  pdl_launch_dependents();
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (clog) cluster_sync_all();                               // a CTA's shared memory is written until here
 }
@@ -541,17 +565,16 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
         float vm = m;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) vm = fmaxf(vm, f[j]);
-        const Scale q = scale_of(vm, c);
-        const float from = vm == -INFINITY ? 0.f : -q.ref;
+        const float ref = __fmul_rn(vm, c), from = vm == -INFINITY ? 0.f : -ref;
+        const bool far = far_out(vm, ref);
         s = moved(s, m, vm, c);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s += ex2(fmaf(f[j], q.c, from));
+        for (int j = 0; j < VEC; ++j) s += far ? far_weight(f[j], vm) : ex2(fmaf(f[j], c, from));
         m = vm;
       }
       for (int i = tid; i < rest; i += kLongThreads) {
-        const float f = to_f32(z[edge(i)]), vm = fmaxf(m, f);
-        const Scale q = scale_of(vm, c);
-        s = moved(s, m, vm, c) + ex2(fmaf(f, q.c, vm == -INFINITY ? 0.f : -q.ref));
+        const float f = to_f32(z[edge(i)]), vm = fmaxf(m, f), ref = __fmul_rn(vm, c);
+        s = moved(s, m, vm, c) + (far_out(vm, ref) ? far_weight(f, vm) : ex2(fmaf(f, c, vm == -INFINITY ? 0.f : -ref)));
         m = vm;
       }
       warp_max_sum(m, s, c);
@@ -565,15 +588,19 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
     if (g) {
       const float w = a.up_rows ? weight * a.up[row] : weight;
       const float scale = w / s;
-      const Scale by = scale_of(m, c);
+      const float ref = __fmul_rn(m, c);
+      const bool far = far_out(m, ref);
       for (int i = tid; i < vecs; i += kLongThreads) {
         float f[VEC];
         unpack16<T>(*reinterpret_cast<const uint4*>(z + head + i * VEC), f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = empty ? 0.f : ex2(fmaf(f[j], by.c, -by.ref)) * scale;
+        for (int j = 0; j < VEC; ++j) f[j] = empty ? 0.f : (far ? far_weight(f[j], m) : ex2(fmaf(f[j], c, -ref))) * scale;
         *reinterpret_cast<uint4*>(g + head + i * VEC) = pack16<T>(f);
       }
-      for (int i = tid; i < rest; i += kLongThreads) g[edge(i)] = from_f32<T>(empty ? 0.f : ex2(fmaf(to_f32(z[edge(i)]), by.c, -by.ref)) * scale);
+      for (int i = tid; i < rest; i += kLongThreads) {
+        const float f = to_f32(z[edge(i)]);
+        g[edge(i)] = from_f32<T>(empty ? 0.f : (far ? far_weight(f, m) : ex2(fmaf(f, c, -ref))) * scale);
+      }
       __syncthreads();
       for (int k = tid; k < a.K; k += kLongThreads) {
         const int i = __float_as_int(entries[k].y);
@@ -585,7 +612,8 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
             first = first && o >= k;
             p += ex2(entries[o].x);
           }
-        if (first) g[i] = from_f32<T>((ex2(fmaf(to_f32(z[i]), by.c, -by.ref)) / s - p) * w);
+        const float f = to_f32(z[i]);
+        if (first) g[i] = from_f32<T>(((far ? far_weight(f, m) : ex2(fmaf(f, c, -ref))) / s - p) * w);
       }
     }
     __syncthreads();
@@ -607,15 +635,22 @@ __global__ void __launch_bounds__(256) distill_loss_kernel(DistillArgs a, float*
     const float2* entries = a.entries + (long long)row * a.K;
     const float2 q = a.stats[row];
     constexpr float kLn2 = 0.6931471805599453f;
-    const Scale by = scale_of(q.x, a.c);
-    const float base = kLn2 * (log2f(q.y) - fmaf(q.x, by.c, -by.ref)), inv = 1.f / a.temperature;
+    const float ref = __fmul_rn(q.x, a.c);
+    const float base = kLn2 * (log2f(q.y) - (far_out(q.x, ref) ? 0.f : fmaf(q.x, a.c, -ref))), inv = 1.f / a.temperature;
     float part = 0.f;
-#pragma unroll 4
-    for (int k = lane; k < a.K; k += 32) {
-      const float2 e = entries[k];
-      const int i = __float_as_int(e.y);
-      const float x = i >= 0 ? to_f32(z[i]) : 0.f, p = ex2(e.x);
-      if (i >= 0 && !(p == 0.f)) part += p * (fmaf(kLn2, e.x, base) - (x - q.x) * inv);
+    constexpr int U = 4;                                      // entries of a lane at once: their logits come from anywhere
+    for (int k0 = lane; k0 < a.K; k0 += 32 * U) {
+      float2 e[U];
+      float x[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) e[j] = k0 + 32 * j < a.K ? entries[k0 + 32 * j] : make_float2(0.f, __int_as_float(-1));
+#pragma unroll
+      for (int j = 0; j < U; ++j) x[j] = __float_as_int(e[j].y) >= 0 ? to_f32(z[__float_as_int(e[j].y)]) : 0.f;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const float p = ex2(e[j].x);
+        if (__float_as_int(e[j].y) >= 0 && !(p == 0.f)) part += p * (fmaf(kLn2, e[j].x, base) - (x[j] - q.x) * inv);
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
@@ -629,7 +664,12 @@ __global__ void __launch_bounds__(256) distill_loss_kernel(DistillArgs a, float*
   if (!last) return;
   __threadfence();
   double v = 0.0;
-  for (int i = threadIdx.x; i < a.N; i += 256) v += __ldcg(a.loss + i);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < a.N / 4; i += 256) {
+    const float4 l = __ldcg(reinterpret_cast<const float4*>(a.loss) + i);
+    v += (double(l.x) + double(l.y)) + (double(l.z) + double(l.w));
+  }
+  if (threadIdx.x < a.N % 4) v += __ldcg(a.loss + a.N / 4 * 4 + threadIdx.x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (lane == 0) red[threadIdx.x >> 5] = v;
@@ -724,15 +764,15 @@ extern "C" {
 
 // Distillation of student logits z [N, V] (pitch ldz; fp32, bf16 or fp16: type 0, 1, 2) from teacher logits t [N, K] (type t_type) at classes idx [N, K].
 //   entries [N, K, 2] floats and one more: written from t and idx; read if t is null
-//   flags [N] bytes: the loss is a mean over the rows that have a teacher (written or read likewise); null: no mean
-//   loss [N] or null; out: their sum or mean, or null; stats [N, 2]: written, or read (have_stats: z is not searched for its maximum again)
+//   flags [N] bytes at 16 bytes: the loss is a mean over the rows that have a teacher (written or read likewise); null: no mean
+//   loss [N] (with out: at 16 bytes) or null; out: their sum or mean, or null; stats [N, 2]: written, or read (have_stats: z is not searched for its maximum again)
 //   grad [N, V] (pitch ldg; every row as far behind a multiple of 16 bytes as z's) or null: times up, which is null (1), one number, or (up_rows) one for every row; skip_one: nothing is done where up is one number and it is 1
 int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t, const long long* idx, float* entries, int N, int V, int K, float temperature,
                unsigned char* flags, const float* up, int up_rows, int skip_one, float* stats, int have_stats, float* loss, float* out, void* grad, long long ldg,
                void* stream) {
   using namespace lt;
   if (type < 0 || type > 2 || t_type < 0 || t_type > 2 || N < 0 || N >= 1 << 30 || V < 1 || V >= 1 << 30 || K < 1 || K > kDistillTop || !(temperature >= 0x1p-60f && temperature <= 0x1p60f) || (out && !loss) || (loss && (!stats || !t)) ||
-      (reinterpret_cast<uintptr_t>(entries) & 7) != 0)
+      (reinterpret_cast<uintptr_t>(entries) & 7) != 0 || (reinterpret_cast<uintptr_t>(flags) & 15) != 0 || (out && (reinterpret_cast<uintptr_t>(loss) & 15) != 0))
     return -int(kStatusBadArgument);
   if (N == 0) return 0;
   const int bytes = type == kElemF32 ? 4 : 2;

@@ -1678,6 +1678,14 @@ def _like_rows(z):
     return torch.empty(shift + N * ld, dtype=z.dtype, device=z.device).as_strided((N, V), (ld, 1), shift)
 
 
+def _distill_room(N: int, top: int):
+    """Where the parts of a workspace lie: ([N] losses that go into one number at 0,) [N] bytes, [N, K, 2] entries and a counter, [N, 2] maxima and sums; its size."""
+    flags = (N + 3) // 4 * 16
+    entries = flags + (N + 15) // 16 * 16
+    stats = entries + 8 * (N * top + 1)
+    return flags, entries, stats, stats + 8 * N
+
+
 def distill_loss(z, t, idx, temperature: float, reduction: str, with_grad: bool):
     """(loss, gradient for an upstream gradient of 1 or None, what `distill_grad` needs) of student logits z [N, V] (rows may be strided) against a teacher's top
     logits t [N, K] at classes idx [N, K] (`functional.distillation_loss` has the formulas)."""
@@ -1686,17 +1694,15 @@ def distill_loss(z, t, idx, temperature: float, reduction: str, with_grad: bool)
     z = z if z.stride(1) == 1 else z.contiguous()
     t, idx = t.contiguous(), (idx if idx.dtype == torch.int64 else idx.to(torch.int64)).contiguous()
     mean = reduction == "mean"
-    # [N, K, 2] entries and a counter, [N, 2] maxima and sums, [N] losses (those that go into one number), [N] bytes
-    room = z.new_empty(N * (2 * top + 3) + 2 + (N + 3) // 4, dtype=torch.float32)
+    flags, entries, stats, size = _distill_room(N, top)
+    room = torch.empty(size, dtype=torch.uint8, device=z.device)
     at = room.data_ptr()
-    stats = at + 8 * (N * top + 1)
-    loss, flags = stats + 8 * N, stats + 12 * N
     out = z.new_empty((N,) if reduction == "none" else (), dtype=torch.float32)
     rows = out.dim() > 0
     grad = _like_rows(z) if with_grad else None
     with _on(z):
-        _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), _ELEM[t.dtype], t.data_ptr(), idx.data_ptr(), at, N, V, top, temperature,
-                                 flags if mean else None, None, 0, 0, stats, 0, out.data_ptr() if rows else loss, None if rows else out.data_ptr(), _p(grad), 0 if grad is None else grad.stride(0), _stream()), "lt_distill")
+        _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), _ELEM[t.dtype], t.data_ptr(), idx.data_ptr(), at + entries, N, V, top, temperature,
+                                 at + flags if mean else None, None, 0, 0, at + stats, 0, out.data_ptr() if rows else at, None if rows else out.data_ptr(), _p(grad), 0 if grad is None else grad.stride(0), _stream()), "lt_distill")
     _launches[0] += 2
     return out, grad, room
 
@@ -1711,9 +1717,10 @@ def distill_grad(z, room, top: int, temperature: float, mean: bool, up, grad=Non
     if not there:
         grad = _like_rows(z)
     at = room.data_ptr()
+    flags, entries, stats, _ = _distill_room(N, top)
     with _on(z):
-        _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), 0, None, None, at, N, V, top, temperature, at + 4 * (N * (2 * top + 3) + 2) if mean else None,
-                                 up.data_ptr(), up.dim(), 1 if there else 0, at + 8 * (N * top + 1), 1, None, None, grad.data_ptr(), grad.stride(0),
+        _check(_fn("lt_distill")(_ELEM[z.dtype], z.data_ptr(), z.stride(0), 0, None, None, at + entries, N, V, top, temperature, at + flags if mean else None,
+                                 up.data_ptr(), up.dim(), 1 if there else 0, at + stats, 1, None, None, grad.data_ptr(), grad.stride(0),
                                  _stream()), "lt_distill")
     return grad
 

@@ -138,10 +138,10 @@ def test_the_native_calls_refuse_what_they_cannot_take():
         assert rc < 0
     assert embed(n=0) == embed(D=0) == grad(D=0) == 0
 
-    def distill(type=0, z=0, ldz=8, t_type=0, t=16, entries=0, N=2, V=8, K=1, T=1.0, stats=16, loss=16, out=None, grad=None, ldg=8):
-        return fn("lt_distill")(type, z, ldz, t_type, t, None, entries, N, V, K, T, None, None, 0, 0, stats, 0, loss, out, grad, ldg, None)
+    def distill(type=0, z=0, ldz=8, t_type=0, t=16, entries=0, N=2, V=8, K=1, T=1.0, stats=16, loss=16, out=None, grad=None, ldg=8, flags=None):
+        return fn("lt_distill")(type, z, ldz, t_type, t, None, entries, N, V, K, T, flags, None, 0, 0, stats, 0, loss, out, grad, ldg, None)
     for bad in (dict(type=3), dict(t_type=-1), dict(N=-1), dict(N=1 << 30), dict(V=0), dict(V=1 << 30), dict(K=0), dict(K=1025), dict(T=0.0), dict(T=-1.0), dict(T=math.nan),
-                dict(T=1e-30), dict(T=1e30), dict(entries=4), dict(stats=None), dict(t=None), dict(loss=None, out=16), dict(grad=4), dict(grad=16, ldg=9)):
+                dict(T=1e-30), dict(T=1e30), dict(entries=4), dict(flags=8), dict(out=16, loss=8), dict(stats=None), dict(t=None), dict(loss=None, out=16), dict(grad=4), dict(grad=16, ldg=9)):
         assert distill(**bad) < 0
     assert distill(N=0) == 0
     draw = lambda type=0, rows=2, V=8: fn("lt_sample_tokens")(type, None, 8, None, 0, None, None, None, None, 1.0, 0, 1.0, 0.0, rows, V, None, None, None)
