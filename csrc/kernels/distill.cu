@@ -230,7 +230,7 @@ struct DistillSmem {
   static __host__ __device__ int bytes(int nt, int vpt, int K) { return links(nt, vpt, K) + kChains * K * int(sizeof(LINK)); }
 };
 
-// A cluster of CTAs holds a row, every thread up to VPT vectors of 16 bytes: a row is read from global memory once.  The threads go over their vectors twice, first
+// A CTA, or for few rows a cluster of them, holds a row, every thread up to VPT vectors of 16 bytes: a row is read from global memory once.  The threads go over their vectors twice, first
 // for the warps' maxima and sums, which go to all warps of the cluster, and then for the gradient; between the two they do the first pass over the
 // next row, so that nobody waits for the exchange, and the rows after that are on their way into shared memory.  There is no barrier of all threads:
 // a thread reads the vectors that it fetched itself, and one mbarrier a row counts the pairs that arrive and this CTA's warps.  A warp that has passed the one of
@@ -530,47 +530,79 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
   if (clog) cluster_sync_all();                               // a CTA's shared memory is written until here
 }
 
-// Rows that no cluster holds: a CTA goes over a row twice.
+// Many long rows: a CTA goes over a row twice, the second time mostly out of L2 (of rows of 256 KB 296 are under way: 76 MB), and writes past it.  Nothing is
+// exchanged between CTAs, and two a SM with 63 registers a thread fill all 148; the clusters above find places for 132.  It moves the 2.1 GB of 4096 x 128256 bf16
+// logits and their gradient in 450 us with teacher and losses (cluster kernel: 506; the copy rate would allow 326), 1000 x 50257 fp32 in 97 us (127); losses
+// alone read 1.05 GB in 195 us (348).  What bounds it: two exponentials an element take the special function units 230 us, and a CTA's two passes do not
+// overlap with each other.  Three CTAs a SM of 40 registers spill (500 us), 1024 threads in one CTA wait for each other (509 us).
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs a) {
-  constexpr int VEC = kVec<T>;
+  constexpr int VEC = kVec<T>, U = 4;
   __shared__ float2 red[kLongWarps];
   __shared__ int isum[kLongWarps];
+  __shared__ int classes[kDistillTop];
   pdl_launch_dependents();
   pdl_wait();
   if (a.skip_one && a.up && a.up[0] == 1.f) return;
   float weight = a.temperature;
-  if (a.flags) weight /= float(max(1, count_flags(a.flags, a.N, isum)));
+  if (a.flags && a.grad) weight /= float(max(1, count_flags(a.flags, a.N, isum)));
   if (a.up && !a.up_rows) weight *= a.up[0];
   const float c = a.c;
+  const uint64_t c2 = pack_f32x2(c, c);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   for (int row = blockIdx.x; row < a.N; row += gridDim.x) {
     const T* z = static_cast<const T*>(a.z) + (long long)row * a.ldz;
     T* g = a.grad ? static_cast<T*>(a.grad) + (long long)row * a.ldg : nullptr;
-    const float2* entries = a.entries + (long long)row * a.K;
-    bool there = false;
-    for (int k = tid; k < a.K; k += kLongThreads) there = there || __float_as_int(entries[k].y) >= 0;
-    const bool empty = __syncthreads_or(there) == 0;
     const int head = min(a.V, int((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / int(sizeof(T)));
     const int vecs = (a.V - head) / VEC, tail = head + vecs * VEC, rest = head + (a.V - tail);
+    const uint4* from = reinterpret_cast<const uint4*>(z + head);
     auto edge = [&](int i) { return i < head ? i : tail + i - head; };
     float m = -INFINITY, s = 0.f;
     if (a.have_stats) {
       m = a.stats[row].x;
       s = a.stats[row].y;
     } else {
-      for (int i = tid; i < vecs; i += kLongThreads) {
-        float f[VEC];
-        unpack16<T>(*reinterpret_cast<const uint4*>(z + head + i * VEC), f);
+      for (int i0 = tid; i0 < vecs; i0 += U * kLongThreads) {
+        uint4 u[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+          u[k] = i0 + k * kLongThreads < vecs ? __ldcg(from + i0 + k * kLongThreads) : make_uint4(minus_inf<T>(), minus_inf<T>(), minus_inf<T>(), minus_inf<T>());
         float vm = m;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) vm = fmaxf(vm, f[j]);
-        const float ref = __fmul_rn(vm, c), from = vm == -INFINITY ? 0.f : -ref;
-        const bool far = far_out(vm, ref);
+        for (int k = 0; k < U; ++k) vm = fmaxf(vm, max16<T>(u[k]));
         s = moved(s, m, vm, c);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += far ? far_weight(f[j], vm) : ex2(fmaf(f[j], c, from));
         m = vm;
+        const float ref = __fmul_rn(m, c), below = m == -INFINITY ? 0.f : -ref;
+        if (!far_out(m, ref)) {
+          uint64_t sum[VEC / 2];
+#pragma unroll
+          for (int j = 0; j < VEC / 2; ++j) sum[j] = 0ull;
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            float f[VEC];
+            unpack16<T>(u[k], f);
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) {
+              float x, y;
+              unpack_f32x2(fma_f32x2(pack_f32x2(f[2 * j], f[2 * j + 1]), c2, pack_f32x2(below, below)), x, y);
+              sum[j] = add_f32x2(sum[j], pack_f32x2(ex2(x), ex2(y)));
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < VEC / 2; ++j) {
+            float x, y;
+            unpack_f32x2(sum[j], x, y);
+            s += x + y;
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < U; ++k) {
+            float f[VEC];
+            unpack16<T>(u[k], f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s += far_weight(f[j], m);
+          }
+        }
       }
       for (int i = tid; i < rest; i += kLongThreads) {
         const float f = to_f32(z[edge(i)]), vm = fmaxf(m, f), ref = __fmul_rn(vm, c);
@@ -586,30 +618,50 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
       if (a.stats && tid == 0) a.stats[row] = make_float2(m, s);
     }
     if (g) {
-      const float w = a.up_rows ? weight * a.up[row] : weight;
-      const float scale = w / s;
-      const float ref = __fmul_rn(m, c);
+      const float2* entries = a.entries + (long long)row * a.K;
+      for (int k = tid; k < a.K; k += kLongThreads) classes[k] = __float_as_int(entries[k].y);
+      const bool empty = __float_as_int(entries[0].y) == -2;
+      const float w = a.up_rows ? weight * a.up[row] : weight, scale = w / s, ref = __fmul_rn(m, c);
       const bool far = far_out(m, ref);
-      for (int i = tid; i < vecs; i += kLongThreads) {
-        float f[VEC];
-        unpack16<T>(*reinterpret_cast<const uint4*>(z + head + i * VEC), f);
+      uint4* to = reinterpret_cast<uint4*>(g + head);
+      for (int i0 = tid; i0 < vecs; i0 += U * kLongThreads) {
+        uint4 u[U];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f[j] = empty ? 0.f : (far ? far_weight(f[j], m) : ex2(fmaf(f[j], c, -ref))) * scale;
-        *reinterpret_cast<uint4*>(g + head + i * VEC) = pack16<T>(f);
+        for (int k = 0; k < U; ++k)
+          if (i0 + k * kLongThreads < vecs) u[k] = __ldcs(from + i0 + k * kLongThreads);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          if (i0 + k * kLongThreads >= vecs) break;
+          float f[VEC];
+          unpack16<T>(u[k], f);
+          if (!empty && !far) {
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) {
+              float x, y;
+              unpack_f32x2(fma_f32x2(pack_f32x2(f[2 * j], f[2 * j + 1]), c2, pack_f32x2(-ref, -ref)), x, y);
+              unpack_f32x2(mul_f32x2(pack_f32x2(ex2(x), ex2(y)), pack_f32x2(scale, scale)), f[2 * j], f[2 * j + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) f[j] = empty ? 0.f : far_weight(f[j], m) * scale;
+          }
+          __stcs(to + i0 + k * kLongThreads, pack16<T>(f));
+        }
       }
       for (int i = tid; i < rest; i += kLongThreads) {
         const float f = to_f32(z[edge(i)]);
         g[edge(i)] = from_f32<T>(empty ? 0.f : (far ? far_weight(f, m) : ex2(fmaf(f, c, -ref))) * scale);
       }
       __syncthreads();
+      // the classes of the teacher's entries once more, one that comes again by its first entry
       for (int k = tid; k < a.K; k += kLongThreads) {
-        const int i = __float_as_int(entries[k].y);
+        const int i = classes[k];
         if (i < 0) continue;
-        float p = 0.f;
+        float p = ex2(entries[k].x);
         bool first = true;
         for (int o = 0; o < a.K; ++o)
-          if (__float_as_int(entries[o].y) == i) {
-            first = first && o >= k;
+          if (classes[o] == i && o != k) {
+            first = first && o > k;
             p += ex2(entries[o].x);
           }
         const float f = to_f32(z[i]);
@@ -740,7 +792,8 @@ int distill(DistillArgs a, float* out, unsigned* finished, cudaStream_t st) {
   const int per = few ? 8 : 5;
   a.cluster_log = 0;
   while ((1 << a.cluster_log) < kDistillCluster && vecs > (per * kDistillThreads) << a.cluster_log) ++a.cluster_log;
-  if (vecs <= (per * kDistillThreads) << a.cluster_log) {
+  // rows that a CTA holds, with a gradient: read once (2048 x 32000 fp16, 128 entries: 82 us, twice 93); few rows: clusters, so that all SMs have work
+  if (vecs <= (per * kDistillThreads) << a.cluster_log && ((a.grad && a.cluster_log == 0) || a.N < 2 * sm_count())) {
     // few rows: more CTAs for each
     while ((1 << a.cluster_log) < kDistillCluster && (long long)a.N << (a.cluster_log + 1) <= sm_count() && vecs >> a.cluster_log >= 512) ++a.cluster_log;
     const int own = (vecs + (1 << a.cluster_log) - 1) >> a.cluster_log;

@@ -614,7 +614,7 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         has = there.any(1)
         below = lambda x: (x - x.detach().amax(1, keepdim=True)) / temperature         # (the largest is taken off first: the type's lowest value has a quotient then)
         log_p = torch.log_softmax(below(t.to(wide).masked_fill(~there, -math.inf).masked_fill(~has[:, None], 0.0)), -1)
-        log_q = torch.log_softmax(below(z.to(wide)), -1).gather(1, idx.to(torch.int64).clamp(0, V - 1))
+        log_q = torch.log_softmax(below(z.to(wide).masked_fill(~has[:, None], 0.0)), -1).gather(1, idx.to(torch.int64).clamp(0, V - 1))
         p = log_p.exp().masked_fill(~there, 0.0)
         counts = p != 0
         loss = (p * (torch.where(counts, log_p, 0.0) - torch.where(counts, log_q, 0.0))).sum(1) * temperature ** 2

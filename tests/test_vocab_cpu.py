@@ -64,6 +64,13 @@ def test_a_student_with_nothing_but_the_lowest_value_knows_nothing(dtype):
     assert abs(float(loss) - 2 * 0.25 * math.log(10)) < 1e-5 and abs(float(grad[0, 3]) + 0.45) < 2.0 ** -8 and abs(float(grad[1, 0]) - 0.05) < 2.0 ** -8
 
 
+def test_rows_without_a_teacher_have_no_gradient_whatever_the_student_says():
+    z = torch.tensor([[-math.inf] * 4, [math.nan] * 4, [1.0, 2.0, 3.0, 4.0]]).requires_grad_()
+    loss = Fn.distillation_loss(z, torch.zeros(3, 1), torch.tensor([[-1], [4], [0]]))
+    loss.backward()
+    assert bool(torch.isfinite(loss)) and not z.grad[:2].any() and bool(z.grad[2].all())
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_sampling(dtype):
     g = _gen(2)

@@ -492,6 +492,26 @@ def test_longer_rows_than_a_cluster_holds(dtype):
     _check_distill(z, t, cls, 1.3, "none", torch.rand(3, device="cuda", generator=g))
 
 
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 33001), (torch.float16, 33000), (torch.float32, 16601)])
+def test_many_long_rows(dtype, V):
+    """Rows that no CTA holds, more of them than there are places: of all kinds in turn."""
+    g = _gen(V)
+    N = 650
+    z = (torch.randn(N, V, device="cuda", generator=g) * 3).to(dtype)
+    t, cls = _teacher(N, V, 6, dtype, g, ragged=True)
+    cls[5] = torch.tensor([0, V - 1, 7, 0, V - 1, 9], device="cuda")
+    z[3] = torch.finfo(dtype).min
+    z[4, 100:] = torch.finfo(dtype).min
+    z[6, :V - 2] = -math.inf
+    cls[6] = -1
+    z[7, 11] = torch.finfo(dtype).max
+    cls[7] = torch.tensor([11, -1, -1, -1, -1, -1], device="cuda")
+    cls[4] = torch.tensor([1, 2, 3, -1, -1, -1], device="cuda")
+    _check_distill(z, t, cls, 1.3, "mean")
+    _check_distill(z, t, cls, 1.3, "none", torch.rand(N, device="cuda", generator=g))
+    _check_distill(z[:, 1:-2], t, cls.where(cls < V - 3, -1).where(torch.arange(N, device="cuda")[:, None] != 7, -1), 0.9, "sum", torch.tensor(2.0, device="cuda"))
+
+
 def test_two_streams_at_once():
     """Calls of the same kind on two streams have nothing in common."""
     from litetorch_b200.ops import functional as Fn

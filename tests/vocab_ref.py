@@ -71,6 +71,8 @@ def distillation(z, t, idx, temperature, reduction, up=None):
     finite = torch.where(used & torch.isfinite(terms), (log_p - lq).abs(), torch.zeros_like(p))
     near = torch.where(torch.isfinite(x.gather(1, j)), x.gather(1, j), torch.zeros_like(p))
     lost = temperature ** 2 * (p * (rel_p * finite + rel_p + near * u + rel_s + 8 * u * (1 + finite))).sum(1)
+    # (by definition, whatever the student's logits are there)
+    grad, bound = (torch.where(has[:, None], v, torch.zeros_like(v)) for v in (grad, bound))
     if reduction == "none":
         return rows, lost + rows.abs() * 2.0 ** -20, grad, bound
     return rows.sum() * share, lost.sum() * share + rows.abs().sum() * share * 2.0 ** -20, grad, bound
