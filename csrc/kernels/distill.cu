@@ -792,8 +792,8 @@ int distill(DistillArgs a, float* out, unsigned* finished, cudaStream_t st) {
   const int per = few ? 8 : 5;
   a.cluster_log = 0;
   while ((1 << a.cluster_log) < kDistillCluster && vecs > (per * kDistillThreads) << a.cluster_log) ++a.cluster_log;
-  // rows that a CTA holds, with a gradient: read once (2048 x 32000 fp16, 128 entries: 82 us, twice 93); few rows: clusters, so that all SMs have work
-  if (vecs <= (per * kDistillThreads) << a.cluster_log && ((a.grad && a.cluster_log == 0) || a.N < 2 * sm_count())) {
+  // rows that a CTA holds are read once (2048 x 32000 fp16, 128 entries: 82 us, twice 93; losses alone 47 and 43); few rows: clusters, so that all SMs have work
+  if (vecs <= (per * kDistillThreads) << a.cluster_log && (a.cluster_log == 0 || a.N < 2 * sm_count())) {
     // few rows: more CTAs for each
     while ((1 << a.cluster_log) < kDistillCluster && (long long)a.N << (a.cluster_log + 1) <= sm_count() && vecs >> a.cluster_log >= 512) ++a.cluster_log;
     const int own = (vecs + (1 << a.cluster_log) - 1) >> a.cluster_log;

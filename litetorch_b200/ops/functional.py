@@ -558,8 +558,9 @@ class _Distillation(torch.autograd.Function):
     recorded (whose backward may be replayed by itself), backward forms it from the logits and their kept maxima and sums."""
 
     @staticmethod
-    def forward(ctx, z, t, idx, temperature, reduction):
-        ahead = ctx.needs_input_grad[0] and reduction != "none" and not torch.cuda.is_current_stream_capturing()
+    def forward(ctx, z, t, idx, temperature, reduction, recorded):
+        # (needs_input_grad says nothing of grad mode)
+        ahead = recorded and ctx.needs_input_grad[0] and reduction != "none" and not torch.cuda.is_current_stream_capturing()
         loss, ctx.ahead, room = K.distill_loss(z, t, idx, temperature, reduction, ahead)
         ctx.save_for_backward(z, room)
         ctx.rest = t.shape[1], temperature, reduction == "mean"
@@ -572,7 +573,7 @@ class _Distillation(torch.autograd.Function):
         ahead, ctx.ahead = ctx.ahead, None                     # handed out once
         if ahead is not None and torch.cuda.is_current_stream_capturing():
             ahead = None
-        return K.distill_grad(z, room, *ctx.rest, up if up.is_contiguous() else up.contiguous(), ahead), None, None, None, None
+        return K.distill_grad(z, room, *ctx.rest, up if up.is_contiguous() else up.contiguous(), ahead), None, None, None, None, None
 
 
 def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_idx: torch.Tensor, temperature: float = 1.0,
@@ -606,7 +607,7 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     if logits.dim() != 2:
         z, t, idx = z.reshape(rows, V), t.reshape(rows, top), idx.reshape(rows, top)
     if z.is_cuda and z.dtype in _KERNEL_TYPES and rows > 0:
-        loss = _Distillation.apply(z, t if t.dtype in _KERNEL_TYPES else t.float(), idx, float(temperature), reduction)
+        loss = _Distillation.apply(z, t if t.dtype in _KERNEL_TYPES else t.float(), idx, float(temperature), reduction, torch.is_grad_enabled())
     else:
         wide = torch.promote_types(z.dtype, torch.float32)
         t = t.detach()

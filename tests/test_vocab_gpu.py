@@ -459,6 +459,20 @@ def test_a_row_of_its_own_for_every_loss():
     assert not z.grad[1::2].any() and bool(z.grad[::2].any(1).all())
 
 
+def test_no_gradient_is_formed_that_nobody_asks_for(monkeypatch):
+    from litetorch_b200.ops import functional as Fn
+    z = torch.randn(4, 900, device="cuda", requires_grad=True)
+    t, cls = _teacher(4, 900, 2, torch.float32, _gen(36))
+    asked, real = [], Fn.K.distill_loss
+    monkeypatch.setattr(Fn.K, "distill_loss", lambda *a: (asked.append(a[-1]), real(*a))[1])
+    with torch.no_grad():
+        Fn.distillation_loss(z, t, cls)
+    Fn.distillation_loss(z.detach(), t, cls)
+    Fn.distillation_loss(z, t, cls, reduction="none")
+    Fn.distillation_loss(z, t, cls)
+    assert asked == [False, False, False, True]
+
+
 def test_the_gradient_of_a_slice_is_of_the_slices_size():
     """The last positions of long answers: neighbouring rows lie far apart, those of their gradient do not."""
     from litetorch_b200.ops import functional as Fn
@@ -471,6 +485,15 @@ def test_the_gradient_of_a_slice_is_of_the_slices_size():
     before = torch.cuda.memory_allocated()
     grad, = torch.autograd.grad(loss, z)
     assert grad.untyped_storage().nbytes() < 3 * 1020 * 2 and torch.cuda.memory_allocated() - before < 1 << 16
+
+
+def test_differentiable_once():
+    from litetorch_b200.ops import functional as Fn
+    z = torch.randn(4, 90, device="cuda", requires_grad=True)
+    t, cls = _teacher(4, 90, 2, torch.float32, _gen(37))
+    for out in (Fn.distillation_loss(z, t, cls), Fn.token_embedding(cls[:, 0], z).sum()):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(out, z, create_graph=True)
 
 
 def test_more_rows_than_the_gpu_holds_clusters():
