@@ -317,7 +317,8 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
           mine[k * 32] = none;
         }
       }
-      for (int k = tid; k < a.K; k += nt) copy_async8(smem_u32(entry_buf + entry_turn * a.K + k), a.entries + (long long)to_fetch * a.K + k);
+      if (a.grad)
+        for (int k = tid; k < a.K; k += nt) copy_async8(smem_u32(entry_buf + entry_turn * a.K + k), a.entries + (long long)to_fetch * a.K + k);
     }
     to_fetch += stride;
     z_fetch += step;
@@ -540,7 +541,8 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
   constexpr int VEC = kVec<T>, U = 4;
   __shared__ float2 red[kLongWarps];
   __shared__ int isum[kLongWarps];
-  __shared__ int classes[kDistillTop];
+  // the teacher's entries by the low bits of their class: a bucket's last entry + 1, and an entry's next
+  __shared__ int classes[kDistillTop], bucket[kDistillTop], next[kDistillTop];
   pdl_launch_dependents();
   pdl_wait();
   if (a.skip_one && a.up && a.up[0] == 1.f) return;
@@ -558,9 +560,12 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
     const uint4* from = reinterpret_cast<const uint4*>(z + head);
     auto edge = [&](int i) { return i < head ? i : tail + i - head; };
     float m = -INFINITY, s = 0.f;
+    if (g)
+      for (int i = tid; i < kDistillTop; i += kLongThreads) bucket[i] = 0;
     if (a.have_stats) {
       m = a.stats[row].x;
       s = a.stats[row].y;
+      __syncthreads();
     } else {
       for (int i0 = tid; i0 < vecs; i0 += U * kLongThreads) {
         uint4 u[U];
@@ -619,7 +624,10 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
     }
     if (g) {
       const float2* entries = a.entries + (long long)row * a.K;
-      for (int k = tid; k < a.K; k += kLongThreads) classes[k] = __float_as_int(entries[k].y);
+      for (int k = tid; k < a.K; k += kLongThreads) {
+        const int i = classes[k] = __float_as_int(entries[k].y);
+        if (i >= 0) next[k] = atomicExch(&bucket[i & (kDistillTop - 1)], k + 1);
+      }
       const bool empty = __float_as_int(entries[0].y) == -2;
       const float w = a.up_rows ? weight * a.up[row] : weight, scale = w / s, ref = __fmul_rn(m, c);
       const bool far = far_out(m, ref);
@@ -657,13 +665,17 @@ __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs 
       for (int k = tid; k < a.K; k += kLongThreads) {
         const int i = classes[k];
         if (i < 0) continue;
+        // (the sum in whole numbers of 2^-62: it must not depend on the chain's order)
         float p = ex2(entries[k].x);
-        bool first = true;
-        for (int o = 0; o < a.K; ++o)
-          if (classes[o] == i && o != k) {
-            first = first && o > k;
-            p += ex2(entries[o].x);
+        unsigned long long sum = 0;
+        bool first = true, again = false;
+        for (int o = bucket[i & (kDistillTop - 1)]; o; o = next[o - 1])
+          if (classes[o - 1] == i) {
+            first = first && o - 1 >= k;
+            again = again || o - 1 != k;
+            sum += (unsigned long long)(ex2(entries[o - 1].x) * 4611686018427387904.f);
           }
+        if (again && p == p) p = float(double(sum) * (1.0 / 4611686018427387904.0));
         const float f = to_f32(z[i]);
         if (first) g[i] = from_f32<T>(((far ? far_weight(f, m) : ex2(fmaf(f, c, -ref))) / s - p) * w);
       }

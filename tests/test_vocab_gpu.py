@@ -535,6 +535,21 @@ def test_many_long_rows(dtype, V):
     _check_distill(z[:, 1:-2], t, cls.where(cls < V - 3, -1).where(torch.arange(N, device="cuda")[:, None] != 7, -1), 0.9, "sum", torch.tensor(2.0, device="cuda"))
 
 
+def test_many_entries_that_share_their_low_bits():
+    """The entries of long rows are found by the low ten bits of their class: all in one bucket, and classes that come again."""
+    g = _gen(38)
+    N, V, K = 300, 40000, 1024
+    z = torch.randn(N, V, device="cuda", generator=g).bfloat16()
+    t = torch.randn(N, K, device="cuda", generator=g)
+    idx = torch.randint(0, V, (N, K), device="cuda", generator=g)
+    idx[::3] = 5 + 1024 * torch.randint(0, 39, (K,), device="cuda", generator=g)
+    idx[1::3, 700:] = -1
+    _check_distill(z, t, idx, 1.0, "mean")
+    _check_distill(z, t, idx, 1.0, "none", torch.rand(N, device="cuda", generator=g))
+    a, b = (_check_distill(z, t, idx, 1.0, "sum")[1] for _ in range(2))
+    assert torch.equal(a, b)
+
+
 def test_two_streams_at_once():
     """Calls of the same kind on two streams have nothing in common."""
     from litetorch_b200.ops import functional as Fn
