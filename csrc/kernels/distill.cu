@@ -805,7 +805,9 @@ int distill(DistillArgs a, float* out, unsigned* finished, cudaStream_t st) {
   a.cluster_log = 0;
   while ((1 << a.cluster_log) < kDistillCluster && vecs > (per * kDistillThreads) << a.cluster_log) ++a.cluster_log;
   // rows that a CTA holds are read once (2048 x 32000 fp16, 128 entries: 82 us, twice 93; losses alone 47 and 43); few rows: clusters, so that all SMs have work
-  if (vecs <= (per * kDistillThreads) << a.cluster_log && (a.cluster_log == 0 || a.N < 2 * sm_count())) {
+  // Many entries in a short row make chains whose threads the others wait for (8192 x 4001 fp32, 256 entries: 370 us, 180 as a long row; 1003 bf16 411 and 116).
+  const bool dense = a.grad && !few && 8ll * a.K >= vecs;
+  if (vecs <= (per * kDistillThreads) << a.cluster_log && ((a.cluster_log == 0 && !dense) || a.N < 2 * sm_count())) {
     // few rows: more CTAs for each
     while ((1 << a.cluster_log) < kDistillCluster && (long long)a.N << (a.cluster_log + 1) <= sm_count() && vecs >> a.cluster_log >= 512) ++a.cluster_log;
     const int own = (vecs + (1 << a.cluster_log) - 1) >> a.cluster_log;

@@ -550,6 +550,17 @@ def test_many_entries_that_share_their_low_bits():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,K", [(515, 256), (4001, 1000)])
+def test_many_short_rows_with_many_entries(dtype, V, K):
+    g = _gen(V)
+    z = (torch.randn(400, V, device="cuda", generator=g) * 3).to(dtype)
+    t, cls = _teacher(400, V, K, dtype, g, ragged=True)
+    cls[7] = cls[7, :1]
+    _check_distill(z, t, cls, 1.5, "mean")
+    _check_distill(z, t, cls, 1.5, "none", torch.rand(400, device="cuda", generator=g))
+
+
 def test_two_streams_at_once():
     """Calls of the same kind on two streams have nothing in common."""
     from litetorch_b200.ops import functional as Fn
