@@ -222,10 +222,10 @@ template <typename LINK>
 struct DistillSmem {
   static constexpr int kTop = sizeof(LINK) == 1 ? 255 : kDistillTop;      // entries that a LINK numbers
   static constexpr int kVectors = 3, kEntries = 5, kChains = 4, kPeers = 4;           // rows in turn
-  // vpt: vectors of a thread
+  // vpt: vectors of a thread.  Chains begin at 16 bytes (a thread takes its eight at once), which an odd K does not see to by itself.
   static __host__ __device__ int entries(int nt, int vpt) { return kVectors * vpt * nt * 16; }
   static __host__ __device__ int peers(int nt, int vpt, int K) { return entries(nt, vpt) + kEntries * K * 8; }
-  static __host__ __device__ int heads(int nt, int vpt, int K) { return peers(nt, vpt, K) + kPeers * kDistillCluster * (nt / 32) * 8; }
+  static __host__ __device__ int heads(int nt, int vpt, int K) { return (peers(nt, vpt, K) + kPeers * kDistillCluster * (nt / 32) * 8 + 15) / 16 * 16; }
   static __host__ __device__ int links(int nt, int vpt, int K) { return heads(nt, vpt, K) + kChains * nt * 8 * int(sizeof(LINK)); }
   static __host__ __device__ int bytes(int nt, int vpt, int K) { return links(nt, vpt, K) + kChains * K * int(sizeof(LINK)); }
 };
@@ -855,6 +855,20 @@ int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t
   if (type == kElemF32) return distill<float>(a, out, finished, st);
   if (type == kElemBf16) return distill<__nv_bfloat16>(a, out, finished, st);
   return distill<__half>(a, out, finished, st);
+}
+
+// Where the parts of a CTA's shared memory lie for K entries, `threads` threads and `vectors` vectors a thread: entries, (maximum, sum) pairs, chains, links, the end.
+int lt_distill_places(int K, int threads, int vectors, int* places) {
+  using namespace lt;
+  if (K < 1 || K > kDistillTop || threads < 32 || threads > kDistillThreads || vectors < 1 || vectors > 8) return -int(kStatusBadArgument);
+  auto write = [&](auto s) {
+    typedef decltype(s) S;
+    const int at[5] = {S::entries(threads, vectors), S::peers(threads, vectors, K), S::heads(threads, vectors, K), S::links(threads, vectors, K), S::bytes(threads, vectors, K)};
+    std::copy(at, at + 5, places);
+  };
+  if (K <= DistillSmem<uint8_t>::kTop) write(DistillSmem<uint8_t>());
+  else write(DistillSmem<uint16_t>());
+  return 0;
 }
 
 }  // extern "C"

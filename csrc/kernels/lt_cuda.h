@@ -287,6 +287,7 @@ int lt_token_embedding_bwd(int type, const void* idx, int idx32, const void* dou
 int lt_distill(int type, const void* z, long long ldz, int t_type, const void* t, const long long* idx, float* entries, int N, int V, int K, float temperature,
                unsigned char* flags, const float* up, int up_rows, int skip_one, float* stats, int have_stats, float* loss, float* out, void* grad, long long ldg,
                void* stream);
+int lt_distill_places(int K, int threads, int vectors, int* places);
 
 // ---- sample.cu: tokens by temperature, top-k, top-p and min-p from given random numbers
 int lt_sample_tokens(int type, const void* z, long long ldz, const void* u, int u64bit, const float* tau, const int* top_k, const float* top_p, const float* min_p,

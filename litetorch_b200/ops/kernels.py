@@ -21,6 +21,7 @@ _SIGS = {
     "lt_token_embedding_fwd": [_i, _vp, _i, _vp, _vp, _ll, _i, _i, _f, _vp],
     "lt_token_embedding_bwd": [_i, _vp, _i, _vp, _ll, _vp, _ll, _i, _i, _f, _ll, _vp, _vp, _i, _vp],
     "lt_distill": [_i, _vp, _ll, _i, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _ll, _vp],
+    "lt_distill_places": [_i, _i, _i, _vp],
     "lt_sample_tokens": [_i, _vp, _ll, _vp, _i] + [_vp] * 4 + [_d, _i, _d, _d, _i, _i, _vp, _vp, _vp],
     "lt_residual_norm": [_i, _vp, _vp, _vp, _vp, _ll, _vp, _vp, _vp, _i, _vp, _f, _vp, _f, _vp, _vp, _i, _i, _i, _vp],
     "lt_latent_rope": [_i, _vp, _ll] + [_i] * 8 + [_vp, _f, _vp, _vp, _vp, _f, _vp, _i, _i, _vp, _vp, _vp],
@@ -146,7 +147,7 @@ class LlamaLayer(ctypes.Structure):
 _bound = {}
 
 # Kernels launched per native call; `launch_count()` is what bench.py reports as "gpu_launches".
-_LAUNCHES_PER_CALL = {"lt_gemm_num_tiles": 0, "lt_token_embedding_bwd": 4, "lt_gemm_skinny_set_target": 0, "lt_adam_q8": 3, "lt_set_wait_budget_cycles": 0, "lt_norm_bwd": 2, "lt_paged_decode": 2, "lt_paged_decode_window": 2, "lt_mlstm_prefill": 4, "lt_rglru_scan": 3, "lt_rglru_step": 2, "lt_flash_bwd": 3, "lt_flash_bwd_rope": 3, "lt_llama_layer_fwd": 8, "lt_llama_layer_bwd": 16, "lt_status_fetch": 0, "lt_sm_count": 0, "lt_gemm_set_tail_split": 0, "lt_reduce_parts": 0, "lt_reduce_all": 2, "lt_gemm_set_pair_mode": 0, "lt_flash_bwd_set_trace": 0, "lt_flash_fwd_set_trace": 0, "lt_norm_bwd_ctas": 0, "lt_paged_decode_places": 0,
+_LAUNCHES_PER_CALL = {"lt_gemm_num_tiles": 0, "lt_token_embedding_bwd": 4, "lt_distill_places": 0, "lt_gemm_skinny_set_target": 0, "lt_adam_q8": 3, "lt_set_wait_budget_cycles": 0, "lt_norm_bwd": 2, "lt_paged_decode": 2, "lt_paged_decode_window": 2, "lt_mlstm_prefill": 4, "lt_rglru_scan": 3, "lt_rglru_step": 2, "lt_flash_bwd": 3, "lt_flash_bwd_rope": 3, "lt_llama_layer_fwd": 8, "lt_llama_layer_bwd": 16, "lt_status_fetch": 0, "lt_sm_count": 0, "lt_gemm_set_tail_split": 0, "lt_reduce_parts": 0, "lt_reduce_all": 2, "lt_gemm_set_pair_mode": 0, "lt_flash_bwd_set_trace": 0, "lt_flash_fwd_set_trace": 0, "lt_norm_bwd_ctas": 0, "lt_paged_decode_places": 0,
                       "lt_adam_chunk_elems": 0}
 _launches = [0]
 

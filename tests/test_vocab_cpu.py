@@ -1,4 +1,5 @@
 """Embedding, distillation loss and token sampling on the CPU: the plain forms against 64-bit definitions, what is refused, and the calls that lead there."""
+import ctypes
 import math
 
 import pytest
@@ -153,6 +154,22 @@ def test_the_native_calls_refuse_what_they_cannot_take():
     assert distill(N=0) == 0
     draw = lambda type=0, rows=2, V=8: fn("lt_sample_tokens")(type, None, 8, None, 0, None, None, None, None, 1.0, 0, 1.0, 0.0, rows, V, None, None, None)
     assert draw(type=3) < 0 and draw(rows=-1) < 0 and draw(V=0) < 0 and draw(V=(1 << 19) + 1) < 0 and draw(rows=0) == 0
+
+
+def test_parts_of_the_distillation_kernels_shared_memory():
+    """Every part lies where its widest access may go, whatever the number of entries, none reaches into the next, and all of it is there."""
+    places = (ctypes.c_int * 5)()
+    for threads in (32, 64, 128, 256, 512):
+        for top in range(1, 1025):
+            link, most = (1, 8) if top <= 255 else (2, 5)
+            for vectors in range(1, most + 1):
+                assert K._fn("lt_distill_places")(top, threads, vectors, places) == 0
+                entries, pairs, chains, links, end = places
+                # 16-byte vectors, 8-byte entries and pairs, the chains of a thread's eight vectors at once, links
+                assert entries % 16 == 0 and pairs % 8 == 0 and chains % (8 * link) == 0 and links % link == 0, (top, threads, vectors)
+                assert entries >= 3 * threads * vectors * 16 and pairs >= entries + 5 * 8 * top and chains >= pairs + 4 * 8 * 8 * (threads // 32)
+                assert links >= chains + 4 * 8 * link * threads and end >= links + 4 * link * top and end <= 227 * 1024 - 1024
+    assert K._fn("lt_distill_places")(1025, 512, 5, places) < 0 and K._fn("lt_distill_places")(0, 512, 5, places) < 0
 
 
 # ---------------------------------------------------------------------------------------------- the calls that lead there

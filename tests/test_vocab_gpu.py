@@ -140,6 +140,22 @@ def test_rows_of_a_wider_tensor(dtype, offset, V, pitch):
     _check_distill(room[:1, offset:offset + V].expand(6, V), t, idx, 1.0, "sum")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,K", [(40, 4001, 257), (200, 2048, 301), (32, 32000, 301), (5, 50257, 256), (5, 50256, 257), (3, 40003, 1023), (290, 3001, 1023), (290, 9999, 511)])
+def test_few_rows_with_more_than_255_entries(dtype, N, V, K):
+    """Odd and even numbers of entries and classes, rows that one CTA or several hold, and classes that come again."""
+    g = _gen(K + V)
+    z = (torch.randn(N, V, device="cuda", generator=g) * 3).to(dtype)
+    t, cls = _teacher(N, V, K, dtype, g, ragged=True)
+    cls[1, K // 2:] = cls[1, :K - K // 2].clone()
+    cls[2] = V - 1
+    for reduction in ("mean", "sum"):
+        _check_distill(z, t, cls, 1.5, reduction)
+    up = torch.rand(N, device="cuda", generator=g)
+    a, b = (_check_distill(z, t, cls, 1.5, "none", up)[1] for _ in range(2))
+    assert torch.equal(a, b)
+
+
 def test_classes_that_come_again_and_entries_that_are_not_there():
     g = _gen(3)
     z = torch.randn(5, 40, device="cuda", generator=g)
