@@ -139,6 +139,16 @@ __device__ __noinline__ uint4 far_gradient(uint4 u, float m, float scale) {
   for (int j = 0; j < kVec<T>; ++j) f[j] = far_weight(f[j], m) * scale;
   return pack16<T>(f);
 }
+// A vector that begins with element i0 of a row of V, of which some lie outside.  (By elements from registers: warps are rows apart, and the last vector of
+// neighbouring rows may be another warp's, so that they can share no memory for it.)
+template <typename T>
+__device__ __noinline__ void store_cut(T* row, int i0, int V, uint4 u) {
+  float f[kVec<T>];
+  unpack16<T>(u, f);
+#pragma unroll
+  for (int j = 0; j < kVec<T>; ++j)
+    if (i0 + j >= 0 && i0 + j < V) row[i0 + j] = from_f32<T>(f[j]);
+}
 // (maximum, sum) over the warp.
 __device__ __forceinline__ void warp_max_sum(float& m, float& s, float c) {
   const float own = m;
@@ -243,7 +253,6 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
   typedef DistillSmem<LINK> S;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ __align__(8) uint64_t bars[S::kPeers];
-  __shared__ uint4 cut[2];                                    // the row's first and last vector, if they are cut
   __shared__ int isum[kDistillWarps];
   __shared__ int abort_flag;
   pdl_wait();
@@ -456,8 +465,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
         const bool cuts = !EVEN && (r.shift != 0 || r.vecs * VEC != a.V);
         const int head = cuts ? -r.lo - first : -1, last = cuts ? r.vecs - 1 - r.lo - first : -1;
         auto store = [&](int k, uint4 u) {
-          if (!EVEN && k * 32 == head) cut[0] = u;
-          else if (!EVEN && k * 32 == last) cut[1] = u;
+          if (!EVEN && (k * 32 == head || k * 32 == last)) store_cut<T>(g, (r.lo + first + k * 32) * VEC - r.shift, a.V, u);
           else *reinterpret_cast<uint4*>(to + k * 32 * VEC) = u;
         };
         auto gradient = [&](uint4 u) {
@@ -488,12 +496,6 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
 #pragma unroll 1
           for (int k = 0; k < vpt; ++k)
             if (k * 32 < end) store(k, empty ? make_uint4(0u, 0u, 0u, 0u) : far_gradient<T>(mine[k * 32], m, scale));
-        }
-        if (cuts) {                                           // cut vectors by their elements
-          if (head == 0 && end > 0)
-            for (int j = r.shift; j < min(VEC, a.V + r.shift); ++j) g[j - r.shift] = reinterpret_cast<const T*>(cut)[j];
-          if (r.vecs > 1 && r.vecs == r.end && last >= 0 && last < 32 * vpt && last % 32 == 0)
-            for (int j = 0; j < a.V + r.shift - (r.vecs - 1) * VEC; ++j) g[(r.vecs - 1) * VEC - r.shift + j] = reinterpret_cast<const T*>(cut + 1)[j];
         }
         // chains of this thread's vectors
         typedef typename Heads<LINK>::type heads_t;

@@ -156,6 +156,25 @@ def test_few_rows_with_more_than_255_entries(dtype, N, V, K):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype,N,V", [(torch.bfloat16, 400, 19197), (torch.float16, 400, 19197), (torch.bfloat16, 290, 40003), (torch.float32, 290, 20001),
+                                       (torch.float32, 250, 12289), (torch.bfloat16, 700, 4093), (torch.float16, 290, 131)])
+def test_rows_whose_last_vector_changes_its_owner(dtype, N, V):
+    """CTAs, and clusters of them, that take several rows, which begin and end at other places within 16 bytes."""
+    g = _gen(V)
+    z = (torch.randn(N, V, device="cuda", generator=g) * 3).to(dtype)
+    t, cls = _teacher(N, V, 5, dtype, g, ragged=True)
+    cls[1::2, 0], cls[1::2, 1] = V - 1, 0
+    up = torch.rand(N, device="cuda", generator=g)
+    _check_distill(z, t, cls, 1.0, "mean")
+    _, want = _check_distill(z, t, cls, 0.8, "none", up)
+    from litetorch_b200.ops import functional as Fn
+    leaf = z.detach().requires_grad_()
+    loss = Fn.distillation_loss(leaf, t, cls, 0.8, "none")
+    for _ in range(20):
+        grad, = torch.autograd.grad(loss, leaf, up, retain_graph=True)
+        assert torch.equal(grad, want)
+
+
 def test_classes_that_come_again_and_entries_that_are_not_there():
     g = _gen(3)
     z = torch.randn(5, 40, device="cuda", generator=g)
