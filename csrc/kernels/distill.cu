@@ -341,6 +341,7 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
   if (clog) cluster_sync_all();                               // every CTA is there to be written to
   int cur = 0, prev = 2;                                      // places of the first pass's vectors and of the second's
   int entry_cur = 0;                                          // place of the first pass's entries
+  bool ok = true;
   for (int it = 0; row - stride < a.N; row += stride, z += step, ++it) {
     if (row < a.N) {
       // ---- first pass over this row
@@ -422,7 +423,10 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
       const Row r = row_of(z - step);
       uint4* mine = vectors + prev * room;
       const float2* entries = entry_buf + (entry_cur == 0 ? S::kEntries - 1 : entry_cur - 1) * a.K;
-      mbar_wait(bar0 + 8 * turn, (was / S::kPeers) & 1, &abort_flag, a.status, kStatusTimeoutLocalFlag);
+      // (A warp whose wait runs out sends and arrives no more, since what belongs to a later row would be counted into a phase of which nobody has seen the end.
+      // It was there for this row and the next; the phase after them does not end, so that the waits of all other warps run out at that one at the latest.)
+      ok = __all_sync(0xffffffffu, mbar_wait(bar0 + 8 * turn, (was / S::kPeers) & 1, &abort_flag, a.status, kStatusTimeoutLocalFlag));
+      if (!ok) break;
       const bool empty = __float_as_int(entries[0].y) == -2;
       float m, s;
       if (a.have_stats) {
@@ -531,6 +535,9 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
   pdl_launch_dependents();
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (clog) cluster_sync_all();                               // a CTA's shared memory is written until here
+  if (!ok)                                                    // (and, where phases were not waited for, until what was sent has arrived)
+    for (const long long t0 = clock64(); clock64() - t0 < 1 << 15;) {
+    }
 }
 
 // Many long rows: a CTA goes over a row twice, the second time mostly out of L2 (of rows of 256 KB 296 are under way: 76 MB), and writes past it.  Nothing is

@@ -1,6 +1,7 @@
 """Embedding, distillation loss and token sampling on the CPU: the plain forms against 64-bit definitions, what is refused, and the calls that lead there."""
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -170,6 +171,68 @@ def test_parts_of_the_distillation_kernels_shared_memory():
                 assert entries >= 3 * threads * vectors * 16 and pairs >= entries + 5 * 8 * top and chains >= pairs + 4 * 8 * 8 * (threads // 32)
                 assert links >= chains + 4 * 8 * link * threads and end >= links + 4 * link * top and end <= 227 * 1024 - 1024
     assert K._fn("lt_distill_places")(1025, 512, 5, places) < 0 and K._fn("lt_distill_places")(0, 512, 5, places) < 0
+
+
+class _Overrun(Exception):
+    pass
+
+
+def _rows_by_phases(rng, ctas, warps, rows, slow, heeded):
+    """The warps of a cluster that go over rows as the distillation kernel's do, in any order of their steps: a warp sends its pair of a row to all CTAs and arrives at its
+    own one's barrier for the row (four in turn), then waits for the barrier of the row before.  Waits that are not over run out with the probability `slow`;
+    heeded: such a warp stops.  Returns whether a wait ran out; raises if something is counted into the phase of another row."""
+    pending = [[[row, warps, ctas * warps] for row in range(4)] for _ in range(ctas)]             # row of the phase, arrivals and pairs that are missing
+
+    def count(cta, row, what):
+        p = pending[cta][row % 4]
+        if p[0] != row:
+            raise _Overrun
+        p[what] -= 1
+        if p[1] == 0 and p[2] == 0:
+            p[0], p[1], p[2] = row + 4, warps, ctas * warps
+
+    def warp(cta):
+        for row in range(rows + 1):
+            if row < rows:
+                for to in rng.sample(range(ctas), ctas):
+                    count(to, row, 2)
+                    yield True
+                count(cta, row, 1)
+                yield True
+            if row > 0:
+                while pending[cta][(row - 1) % 4][0] == row - 1:
+                    if rng.random() < slow:
+                        out.append(row - 1)
+                        if heeded:
+                            return
+                        break
+                    yield True
+
+    out = []
+    running = [warp(c) for c in range(ctas) for _ in range(warps)]
+    weights = [rng.choice((1, 1, 30)) for _ in running]
+    for _ in range(200000):
+        if not running:
+            return bool(out)
+        i = rng.choices(range(len(running)), weights)[0]
+        if next(running[i], None) is None:
+            del running[i], weights[i]
+    assert heeded and out, "a wait that never ends"                # (here a wait without a limit, which others have left)
+    return True
+
+
+def test_no_row_is_counted_into_the_phase_of_another():
+    """The protocol of the kernel that holds rows: phases stay apart whatever the order, and, if a wait runs out, because that warp stops."""
+    assert not any(_rows_by_phases(random.Random(seed), 1 + seed % 3, 1 + seed % 4, 12, 0.0, True) for seed in range(60))
+    ran_out = [_rows_by_phases(random.Random(seed), 1 + seed % 3, 2 + seed % 3, 12, 0.02, True) for seed in range(200)]
+    assert sum(ran_out) > 100
+    overruns = 0
+    for seed in range(200):                                       # (what becomes of it otherwise)
+        try:
+            _rows_by_phases(random.Random(seed), 1 + seed % 3, 2 + seed % 3, 12, 0.02, False)
+        except _Overrun:
+            overruns += 1
+    assert overruns > 0
 
 
 # ---------------------------------------------------------------------------------------------- the calls that lead there
