@@ -6,7 +6,8 @@
 // once, so that results do not change from run to run (bf16 atomics, as in lt_embedding_bwd, round every addition and add in
 // any order).
 //
-// The gradient takes four launches:
+// The gradient of a small table by few tokens takes one launch (`embed_few_kernel`: 128 tokens, 8192 x 512 bf16 5.5 us, of which the write of 8 MB takes 1.3 at the copy rate), any
+// other four:
 //   sort   one cluster of CTAs sorts (token, place) by token with a stable counting sort of up to 9 bits a pass: within a token the places stay in order
 //   clear  the table becomes zero, beside the sort
 //   sum    a CTA takes `tile` neighbours of the sorted list and adds their rows.  A token with up to 64 places is summed where it begins; of one with more,
@@ -15,7 +16,7 @@
 //
 // What bounds it: the bytes of the table's gradient where they are many (8192 tokens, 128256 x 4096 bf16: rows and gradient 191 us, 96 % of the copy rate; the clear
 // alone writes 1.05 GB in 141 us and hides the sort), else launches one behind the other (2048 tokens, 32000 x 2048 bf16: 41 us replayed from a graph, of which the
-// sort takes 17 and the join 11; 128 tokens, 8192 x 512: 18 us).  Rows that do not begin at 16 bytes are moved element by element: 40001 x 1027 fp32
+// sort takes 17 and the join 11).  Rows that do not begin at 16 bytes are moved element by element: 40001 x 1027 fp32
 // 145 us, where the bytes take 82.
 #include "lt_cuda.h"
 
@@ -29,6 +30,7 @@ namespace lt {
 
 constexpr int kSortThreads = 1024, kSortBits = 9, kSortBins = 1 << kSortBits;
 constexpr int kMaxTile = 64, kShort = 64;                     // places of a token that are summed at once
+constexpr int kFewThreads = 256, kFewLog = 3, kFewTokens = 2048;        // of one launch: threads, the smallest group (power of two), the most tokens
 constexpr int kJoinTiles = 4;                                 // tiles that a CTA looks through
 
 // ---------------------------------------------------------------------------------------------- forward
@@ -209,8 +211,9 @@ __global__ void __launch_bounds__(512) embed_clear_kernel(unsigned char* grad, l
 // Columns of a thread: a vector of 16 bytes, or (where rows do not begin at 16 bytes) four that lie a CTA's width apart.
 template <typename T, bool WIDE> constexpr int kCols = WIDE ? kVec<T> : 4;
 
+// apart: how far the columns of a thread lie apart.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void store_row(T* row, int c, int D, const float (&acc)[kCols<T, WIDE>], float scale) {
+__device__ __forceinline__ void store_row(T* row, int c, int D, const float (&acc)[kCols<T, WIDE>], float scale, int apart) {
   if constexpr (WIDE) {
     float f[kCols<T, WIDE>];
 #pragma unroll
@@ -219,7 +222,7 @@ __device__ __forceinline__ void store_row(T* row, int c, int D, const float (&ac
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (c + j * int(blockDim.x) < D) row[c + j * blockDim.x] = from_f32<T>(acc[j] * scale);
+      if (c + j * apart < D) row[c + j * apart] = from_f32<T>(acc[j] * scale);
   }
 }
 
@@ -307,7 +310,7 @@ __global__ void __launch_bounds__(256) embed_sum_kernel(const uint2* order, cons
       }
       if (e == end - 1 || s[e + 1].x != key) {
         const bool from_before = head_long && key == head;
-        if (!from_before && !(tail_long && key == tail)) store_row<T, WIDE>(grad + (long long)key * D, c, D, acc, scale);
+        if (!from_before && !(tail_long && key == tail)) store_row<T, WIDE>(grad + (long long)key * D, c, D, acc, scale, blockDim.x);
         else {
           float* p = part + ((long long)t * 2 + (from_before ? 0 : 1)) * D + c;
           if constexpr (WIDE) {
@@ -383,7 +386,149 @@ __global__ void __launch_bounds__(256) embed_join_kernel(const uint2* order, con
           if (c + j * int(blockDim.x) < D) acc[j] += p[j * blockDim.x];
       }
     }
-    store_row<T, WIDE>(grad + (long long)order[min(n, t * tile + tile) - 1].x * D, c, D, acc, scale);
+    store_row<T, WIDE>(grad + (long long)order[min(n, t * tile + tile) - 1].x * D, c, D, acc, scale, blockDim.x);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- few tokens
+// One launch: a CTA takes 4 rows of the table a thread group, 16 KB of it, sets them to zero, looks through all tokens for those of its rows and adds theirs up.  Every CTA
+// reads all tokens (out of L2), which a program with few of them can afford for the three launches less.  A token's rows are added in fp32 in the order of their
+// places, by the group that has its row; those of a token with more than 64 places in as many pieces as there are groups, which are added in order.
+template <typename T, bool WIDE, typename IDX>
+__global__ void __launch_bounds__(kFewThreads) embed_few_kernel(const IDX* idx, const T* dout, long long ldd, T* grad, int n, int D, int V, float scale, long long pad, int log,
+                                                                int chunks) {
+  constexpr int NC = kCols<T, WIDE>, W = kFewThreads / 32, MAXR = kFewThreads / (1 << kFewLog) * 4, U = 8;
+  extern __shared__ uint16_t few_list[];                      // places of this CTA's tokens by row
+  __shared__ uint32_t cnt[W * MAXR], start[MAXR + 1], carry[W];
+  __shared__ float pieces[kFewThreads * NC];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int G = 1 << log, groups = kFewThreads >> log, R = groups * 4;
+  const int chunk = int(blockIdx.x) % chunks, v0 = int(blockIdx.x) / chunks * R, rows = min(R, V - v0);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, own = tid & (G - 1), g = tid >> log;
+  const int c = WIDE ? (chunk * G + own) * NC : chunk * G * NC + own;
+  float acc[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) acc[j] = 0.f;
+  if (c < D)
+    for (int r = g; r < rows; r += groups) store_row<T, WIDE>(grad + (long long)(v0 + r) * D, c, D, acc, 0.f, G);
+  for (int i = tid; i < W * R; i += kFewThreads) cnt[i] = 0u;
+  __syncthreads();
+  const int wpart = ((n + W - 1) / W + 31) / 32 * 32, wlo = min(n, warp * wpart), whi = min(n, wlo + wpart);
+  auto row_of = [&](int i) {                                  // -1: not this CTA's
+    const long long t = i < whi ? (long long)idx[i] : -1;
+    return t >= v0 && t < v0 + rows && t != pad ? int(t - v0) : -1;
+  };
+  bool any = false;
+#pragma unroll 8
+  for (int i = wlo + lane; i < whi; i += 32) {
+    const int r = row_of(i);
+    if (r >= 0) {
+      atomicAdd(&cnt[warp * R + r], 1u);
+      any = true;
+    }
+  }
+  any = __syncthreads_or(any);
+  if (!any) return;
+  // where the tokens of a row begin in the list, and those of a warp among them
+  {
+    uint32_t sum = 0;
+    if (tid < R)
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const uint32_t k = cnt[w * R + tid];
+        cnt[w * R + tid] = sum;
+        sum += k;
+      }
+    uint32_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t k = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += k;
+    }
+    if (lane == 31) carry[warp] = incl;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) incl += carry[w];
+    if (tid < R) {
+      start[tid + 1] = incl;
+      if (tid == 0) start[0] = 0u;
+#pragma unroll
+      for (int w = 0; w < W; ++w) cnt[w * R + tid] += incl - sum;
+    }
+    __syncthreads();
+  }
+  for (int i0 = wlo; i0 < whi; i0 += 32) {
+    const int r = row_of(i0 + lane);
+    const unsigned with = __ballot_sync(0xffffffffu, r >= 0);
+    if (r >= 0) {
+      const unsigned peers = __match_any_sync(with, r);
+      few_list[cnt[warp * R + r] + __popc(peers & ((1u << lane) - 1u))] = uint16_t(i0 + lane);
+      __syncwarp(with);
+      if ((peers >> lane) == 1u) cnt[warp * R + r] += __popc(peers);         // the last of its row
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  // acc = sum of the rows of the places [lo, hi) of the list
+  auto add = [&](uint32_t lo, uint32_t hi) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) acc[j] = 0.f;
+    for (uint32_t e0 = lo; e0 < hi; e0 += U) {
+      uint4 u[U];
+      T one[U][4];
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (e0 + k < hi) {
+          const T* p = dout + (long long)few_list[e0 + k] * ldd + c;
+          if constexpr (WIDE) u[k] = *reinterpret_cast<const uint4*>(p);
+          else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (c + j * G < D) one[k][j] = p[j * G];
+          }
+        }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (e0 + k >= hi) break;
+        if constexpr (WIDE) {
+          float f[NC];
+          unpack16<T>(u[k], f);
+#pragma unroll
+          for (int j = 0; j < NC; ++j) acc[j] += f[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + j * G < D) acc[j] += to_f32(one[k][j]);
+        }
+      }
+    }
+  };
+  bool many = false;
+  for (int r = g; r < rows; r += groups) {
+    const uint32_t lo = start[r], hi = start[r + 1];
+    many = many || hi - lo > uint32_t(kShort);
+    if (hi == lo || hi - lo > uint32_t(kShort) || c >= D) continue;
+    add(lo, hi);
+    store_row<T, WIDE>(grad + (long long)(v0 + r) * D, c, D, acc, scale, G);
+  }
+  if (!__syncthreads_or(many)) return;
+  for (int r = 0; r < rows; ++r) {
+    const uint32_t lo = start[r], m = start[r + 1] - lo;
+    if (m <= uint32_t(kShort)) continue;
+    const uint32_t part = (m + groups - 1) / groups, from = min(m, g * part);
+    if (c < D) {
+      add(lo + from, lo + min(m, from + part));
+#pragma unroll
+      for (int j = 0; j < NC; ++j) pieces[tid * NC + j] = acc[j];
+    }
+    __syncthreads();
+    if (g == 0 && c < D) {
+      for (int o = 1; o < groups; ++o)
+#pragma unroll
+        for (int j = 0; j < NC; ++j) acc[j] += pieces[((o << log) + own) * NC + j];
+      store_row<T, WIDE>(grad + (long long)(v0 + r) * D, c, D, acc, scale, G);
+    }
+    __syncthreads();
   }
 }
 
@@ -412,6 +557,17 @@ int embedding_bwd(const void* idx, const void* dout, long long ldd, void* grad, 
     LT_RETURN_IF_CUDA(cudaMemsetAsync(grad, 0, bytes, st));
     return 0;
   }
+  const bool vec = D % kVec<T> == 0 && ldd % kVec<T> == 0 && ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(part)) & 15) == 0;
+  if (order == nullptr) {
+    const int per = vec ? D / kVec<T> : (D + 3) / 4;
+    int log = kFewLog;
+    while (log < 6 && (1 << log) < per) ++log;
+    const long long rows = (kFewThreads >> log) * 4, chunks = (per + (1 << log) - 1) >> log, ctas = (V + rows - 1) / rows * chunks;
+    if (n > kFewTokens || ctas > 0x7fffffffll) return -int(kStatusBadArgument);
+    auto few = vec ? embed_few_kernel<T, true, IDX> : embed_few_kernel<T, false, IDX>;
+    LT_RETURN_IF_CUDA(launch_chained(few, unsigned(ctas), kFewThreads, n * 2, st, static_cast<const IDX*>(idx), static_cast<const T*>(dout), ldd, static_cast<T*>(grad), n, D, V, scale, pad, log, int(chunks)));
+    return 0;
+  }
   static OncePerDevice once;
   if (once.pending()) {
     LT_RETURN_IF_CUDA(cudaFuncSetAttribute(embed_sort_kernel<IDX>, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSortThreads / 32 + 2) * kSortBins * 4));
@@ -430,7 +586,6 @@ int embedding_bwd(const void* idx, const void* dout, long long ldd, void* grad, 
   LT_RETURN_IF_CUDA(launch_chained_clusters(embed_sort_kernel<IDX>, ctas, nt, smem, ctas, st, static_cast<const IDX*>(idx), n, V, pad, buf0, buf1, passes, bits, ctas));
   if (bytes > size_t(kClear) * 0x7fffffff) return -int(kStatusBadArgument);
   LT_RETURN_IF_CUDA(launch_chained(embed_clear_kernel, unsigned((bytes + kClear - 1) / kClear), 512, 0, st, static_cast<unsigned char*>(grad), (long long)bytes));
-  const bool vec = D % kVec<T> == 0 && ldd % kVec<T> == 0 && ((reinterpret_cast<uintptr_t>(dout) | reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(part)) & 15) == 0;
   const int per = vec ? D / kVec<T> : (D + 3) / 4;
   const int threads = per >= 256 ? 256 : (per + 31) / 32 * 32;
   const int chunks = (per + threads - 1) / threads, tiles = (n + tile - 1) / tile;
@@ -461,7 +616,7 @@ int lt_token_embedding_fwd(int type, const void* idx, int idx32, const void* tab
 }
 
 // grad[V, D] = scale * sums of dout's rows (pitch ldd) by token; tokens outside [0, V) and `pad` give nothing (pad < 0: there is none).  All of grad is written.
-// order: 2 n entries of 8 bytes; part: 2 ceil(n / tile) rows of D floats; tile: up to 64 sorted rows a CTA.
+// order: 2 n entries of 8 bytes, or null: all by one launch (up to 2048 tokens); part: 2 ceil(n / tile) rows of D floats; tile: up to 64 sorted rows a CTA.
 int lt_token_embedding_bwd(int type, const void* idx, int idx32, const void* dout, long long ldd, void* grad, long long n, int D, int V, float scale, long long pad,
                            void* order, float* part, int tile, void* stream) {
   using namespace lt;

@@ -147,7 +147,7 @@ class LlamaLayer(ctypes.Structure):
 _bound = {}
 
 # Kernels launched per native call; `launch_count()` is what bench.py reports as "gpu_launches".
-_LAUNCHES_PER_CALL = {"lt_gemm_num_tiles": 0, "lt_token_embedding_bwd": 4, "lt_distill_places": 0, "lt_gemm_skinny_set_target": 0, "lt_adam_q8": 3, "lt_set_wait_budget_cycles": 0, "lt_norm_bwd": 2, "lt_paged_decode": 2, "lt_paged_decode_window": 2, "lt_mlstm_prefill": 4, "lt_rglru_scan": 3, "lt_rglru_step": 2, "lt_flash_bwd": 3, "lt_flash_bwd_rope": 3, "lt_llama_layer_fwd": 8, "lt_llama_layer_bwd": 16, "lt_status_fetch": 0, "lt_sm_count": 0, "lt_gemm_set_tail_split": 0, "lt_reduce_parts": 0, "lt_reduce_all": 2, "lt_gemm_set_pair_mode": 0, "lt_flash_bwd_set_trace": 0, "lt_flash_fwd_set_trace": 0, "lt_norm_bwd_ctas": 0, "lt_paged_decode_places": 0,
+_LAUNCHES_PER_CALL = {"lt_gemm_num_tiles": 0, "lt_distill_places": 0, "lt_gemm_skinny_set_target": 0, "lt_adam_q8": 3, "lt_set_wait_budget_cycles": 0, "lt_norm_bwd": 2, "lt_paged_decode": 2, "lt_paged_decode_window": 2, "lt_mlstm_prefill": 4, "lt_rglru_scan": 3, "lt_rglru_step": 2, "lt_flash_bwd": 3, "lt_flash_bwd_rope": 3, "lt_llama_layer_fwd": 8, "lt_llama_layer_bwd": 16, "lt_status_fetch": 0, "lt_sm_count": 0, "lt_gemm_set_tail_split": 0, "lt_reduce_parts": 0, "lt_reduce_all": 2, "lt_gemm_set_pair_mode": 0, "lt_flash_bwd_set_trace": 0, "lt_flash_fwd_set_trace": 0, "lt_norm_bwd_ctas": 0, "lt_paged_decode_places": 0,
                       "lt_adam_chunk_elems": 0}
 _launches = [0]
 
@@ -1626,6 +1626,7 @@ def moe_expert_bwd(gu, dh_u, w, slot_src):
 
 # ------------------------------------------------------------------------------------------------ vocabulary: embedding, distillation, sampling
 _ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INDEX = (torch.int64, torch.int32)
 
 
 def _on(t: torch.Tensor):
@@ -1635,10 +1636,11 @@ def _on(t: torch.Tensor):
 
 def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """scale * table[idx] as [tokens, D] (fp32, bf16 or fp16, rounded once); a token outside the table gives zeros."""
-    assert table.dim() == 2 and table.is_contiguous() and table.dtype in _ELEM and idx.device == table.device
-    idx = _dense_index(idx, torch.int64, torch.int32)
     V, D = table.shape
-    out = torch.empty((idx.numel(), D), dtype=table.dtype, device=table.device)
+    assert table.is_contiguous() and table.dtype in _ELEM and idx.device == table.device
+    if idx.dim() != 1 or idx.dtype not in _INDEX or not idx.is_contiguous():
+        idx = _dense_index(idx, torch.int64, torch.int32)
+    out = table.new_empty((idx.numel(), D))
     with _on(table):
         _check(_fn("lt_token_embedding_fwd")(_ELEM[table.dtype], idx.data_ptr(), 1 if idx.dtype == torch.int32 else 0, table.data_ptr(), out.data_ptr(),
                                              idx.numel(), D, V, float(scale), _stream()), "lt_token_embedding_fwd")
@@ -1648,23 +1650,33 @@ def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0) 
 def token_embedding_grad(idx: torch.Tensor, dout: torch.Tensor, vocab: int, scale: float = 1.0, padding_idx: int = -1) -> torch.Tensor:
     """The gradient [vocab, D] of `token_embedding`'s table from dout [tokens, D]: sums in fp32 in the order of the tokens, rounded once, the same from run
     to run.  Tokens outside the table and `padding_idx` give nothing."""
-    assert dout.dim() == 2 and dout.dtype in _ELEM and idx.numel() == dout.shape[0] and idx.device == dout.device
-    idx = _dense_index(idx, torch.int64, torch.int32)
+    n, D = dout.shape
+    assert dout.dtype in _ELEM and idx.numel() == n and idx.device == dout.device
+    if idx.dim() != 1 or idx.dtype not in _INDEX or not idx.is_contiguous():
+        idx = _dense_index(idx, torch.int64, torch.int32)
     if dout.stride(1) != 1:
         dout = dout.contiguous()
-    n, D = dout.shape
-    grad = torch.empty((vocab, D), dtype=dout.dtype, device=dout.device)
-    # sorted rows that a CTA sums of 256 vectors of 16 bytes, or of 1024 columns: up to 32, so that there are eight CTAs an SM
     size = dout.element_size()
-    chunks = -(-D // (256 * 16 // size if D * size % 16 == 0 else 1024))
-    tile = 8
-    while tile < 32 and n * chunks >= 2 * tile * 8 * 148:
-        tile *= 2
-    # the sorted list twice, 8 bytes an entry, and two rows for the pieces of every tile
-    room = torch.empty(16 * n + (n + tile - 1) // tile * 8 * D, dtype=torch.uint8, device=dout.device)
+    grad = dout.new_empty((vocab, D))
+    # Few tokens and a small gradient: one launch, which reads all tokens for every 16 KB of it.  Replayed, one launch / sort and sums, us: 128 tokens, 8.4 MB 5.5 / 11.7;
+    # 1024, 8.4 MB 9.6 / 17.5; 2048, 8.4 MB 13.7 / 21.2; 2048, 64 KB 13.5 / 21.2; 256, 66 MB 15.7 / 15.8; but 4096, 64 KB 37 / 27; 512, 66 MB 17.8 / 16.4; 64, 263 MB 49 / 41.
+    if n <= 2048 and vocab * D * size <= 1 << 26 and n * vocab * D * size <= 1 << 34:
+        order = part = None
+        tile = 1
+    else:
+        # sorted rows that a CTA sums of 256 vectors of 16 bytes, or of 1024 columns: up to 32, so that there are eight CTAs an SM
+        chunks = -(-D // (256 * 16 // size if D * size % 16 == 0 else 1024))
+        tile = 8
+        while tile < 32 and n * chunks >= 2 * tile * 8 * 148:
+            tile *= 2
+        # the sorted list twice, 8 bytes an entry, and two rows for the pieces of every tile
+        room = torch.empty(16 * n + (n + tile - 1) // tile * 8 * D, dtype=torch.uint8, device=dout.device)
+        order = room.data_ptr()
+        part = order + 16 * n
+        _launches[0] += 3
     with _on(dout):
         _check(_fn("lt_token_embedding_bwd")(_ELEM[dout.dtype], idx.data_ptr(), 1 if idx.dtype == torch.int32 else 0, dout.data_ptr(), dout.stride(0), grad.data_ptr(),
-                                             n, D, int(vocab), float(scale), int(padding_idx), room.data_ptr(), room.data_ptr() + 16 * n, tile, _stream()),
+                                             n, D, int(vocab), float(scale), int(padding_idx), order, part, tile, _stream()),
                "lt_token_embedding_bwd")
     return grad
 

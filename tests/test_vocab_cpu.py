@@ -143,7 +143,8 @@ def test_the_native_calls_refuse_what_they_cannot_take():
     embed = lambda type=0, n=4, D=8, V=9: fn("lt_token_embedding_fwd")(type, None, 0, None, None, n, D, V, 1.0, None)
     grad = lambda type=0, n=4, D=8, V=9, tile=8: fn("lt_token_embedding_bwd")(type, None, 0, None, 8, None, n, D, V, 1.0, -1, None, None, tile, None)
     for rc in (embed(type=3), embed(type=-1), embed(n=-1), embed(n=1 << 31), embed(D=-1), embed(D=(1 << 30) + 1), embed(V=0), grad(type=3), grad(n=-1), grad(n=(1 << 31) - 4096),
-               grad(D=-1), grad(D=(1 << 30) + 1), grad(V=0), grad(V=(1 << 31) - 1), grad(tile=0), grad(tile=65)):
+               grad(D=-1), grad(D=(1 << 30) + 1), grad(V=0), grad(V=(1 << 31) - 1), grad(tile=0), grad(tile=65),
+               grad(n=2049)):                                        # (without a workspace: one launch, which takes up to 2048 tokens)
         assert rc < 0
     assert embed(n=0) == embed(D=0) == grad(D=0) == 0
 

@@ -62,6 +62,31 @@ def test_one_token_for_all_and_two_in_turn(n):
     _check_embed(torch.full((n,), 6, device="cuda"), 9, 48, torch.bfloat16, 0.5, 6, 3)                  # padding alone
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,D", [(1, 70000, 481), (33, 70000, 520), (700, 70000, 488), (2048, 40000, 856), (64, 17000, 2056)])
+def test_few_tokens_of_a_large_table(dtype, n, V, D):
+    """Gradients of more than 64 MB (of fp32 or 16-bit numbers): these are summed by sorted tokens however few there are."""
+    idx = torch.randint(0, V, (n,), device="cuda", generator=_gen(n))
+    idx[::3] = 7
+    _check_embed(idx, V, D, dtype, 1.5, 11, n + D)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,D", [(2048, 300, 64), (2049, 300, 64), (2048, 129, 1), (1500, 1000, 9), (2000, 17, 2048), (65, 3, 517), (2047, 128, 128), (256, 8192, 520)])
+def test_one_launch_for_few_tokens(dtype, n, V, D):
+    """Rows by a group of threads, and tokens with more than 64 places by all groups, beside tokens outside the table, padding, and none at all in most of it."""
+    g = _gen(n + D)
+    idx = torch.randint(-2, V + 2, (n,), device="cuda", generator=g)
+    _check_embed(idx, V, D, dtype, 0.75, V - 1, n)
+    idx[torch.rand(n, device="cuda", generator=g) < 0.6] = V // 2
+    idx[torch.rand(n, device="cuda", generator=g) < 0.1] = 0
+    _check_embed(idx.int(), V, D, dtype, 1.0, None, n + 1)
+    idx.fill_(V - 1)
+    idx[n // 2] = 0
+    _check_embed(idx, V, D, dtype, 1.0, None, n + 2)
+    _check_embed(idx, V, D, dtype, 1.0, V - 1, n + 3)
+
+
 def test_tokens_outside_the_table():
     idx = torch.tensor([[3, -1, 7], [8, 1 << 40, -(1 << 40)], [0, 7, 100]], device="cuda")
     _check_embed(idx, 8, 24, torch.float32, 2.0, None, 5)
