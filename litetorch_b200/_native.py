@@ -1,13 +1,16 @@
 """Build and load the native libraries.
 
-Two shared objects live in ``litetorch_b200/_lib``:
+Three shared objects live in ``litetorch_b200/_lib``:
 
 * ``liblt_cuda.so``  - every sm_100a kernel plus the CUDA-side runtime (allocator, graph capture,
   NVRTC JIT). Built with ``nvcc -gencode arch=compute_100a,code=sm_100a``.
 * ``liblt_host.so``  - the host runtime in C++17 with no CUDA dependency: checkpoint formats,
   data loader, serving scheduler, rendezvous store, JIT expression trees, thread pool.
 
-Both export plain C symbols and are called through ``ctypes``; nothing is JIT-compiled at import
+* ``liblt_torch_<torch's version>.so`` - nodes of torch's autograd graph in C++ for calls so short that a
+  node in Python would cost more than the kernels; built with ``g++`` against the installed torch.
+
+The first two export plain C symbols and are called through ``ctypes``; nothing is JIT-compiled at import
 time.  The reference ships one pybind11 module plus a dlopen'ed GPU library
 (src/backend/backend.cpp:61-341); here the split is host/CUDA so that CPU-only processes (gloo
 ranks, the data-loader workers, tests without a GPU) never touch the CUDA runtime.
@@ -19,6 +22,7 @@ import fcntl
 import glob
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -163,13 +167,47 @@ def build_host(force: bool = False, verbose: bool = False) -> str:
     return out
 
 
+def torch_sources():
+    return sorted(glob.glob(os.path.join(_CSRC, "torch_nodes", "*.cpp")))
+
+
+def _torch_library_path() -> str:
+    import torch
+    return os.path.join(_LIB, "liblt_torch_%s.so" % re.sub(r"[^0-9A-Za-z.]", "_", torch.__version__))
+
+
+def build_torch(force: bool = False, verbose: bool = False) -> str:
+    """Compile the autograd nodes against the installed torch (its C++ interface holds for one version only)."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    os.makedirs(_LIB, exist_ok=True)
+    out = _torch_library_path()
+    srcs = torch_sources()
+    if force or not os.path.exists(out) or os.path.getmtime(out) < _newest(srcs + [os.path.join(_CSRC, "kernels", "lt_cuda.h")]):
+        cuda_inc = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
+        cmd = ([shutil.which("g++") or "g++"] + CXX_FLAGS + ["-I" + p for p in include_paths("cuda")] + ["-I" + cuda_inc, "-I" + os.path.join(_CSRC, "kernels")] + srcs
+               + ["-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-shared", "-L" + os.path.join(os.path.dirname(torch.__file__), "lib"),
+                  "-ltorch_cpu", "-lc10", "-lc10_cuda", "-o", out + ".tmp"])
+        _compile_one(cmd, out)
+        os.replace(out + ".tmp", out)
+        if verbose:
+            print("compiled", out)
+    return out
+
+
 def build_all(force: bool = False, verbose: bool = False):
-    return build_host(force, verbose), build_cuda(force, verbose)
+    built = build_host(force, verbose), build_cuda(force, verbose)
+    try:
+        import torch
+    except ImportError:
+        return built                       # (an isolated build without torch: the nodes are built where they are first used)
+    return built + (build_torch(force, verbose),) if torch.version.cuda else built
 
 
 _lock = threading.Lock()
 _cuda = None
 _host = None
+_torch = None
 
 
 class NativeLibraryMissing(RuntimeError):
@@ -204,6 +242,27 @@ def host_lib() -> ctypes.CDLL:
                 build_host()
             _host = ctypes.CDLL(path, mode=ctypes.RTLD_GLOBAL)
     return _host
+
+
+def torch_lib() -> ctypes.CDLL:
+    """The autograd nodes (`torch.ops.litetorch_b200`), which call the kernels of `cuda_lib()`; built on first use if absent (g++ only, a quarter of a minute)."""
+    global _torch
+    if _torch is not None:
+        return _torch
+    cuda_lib()
+    with _lock:
+        if _torch is None:
+            path = _torch_library_path()
+            if not os.path.exists(path):
+                with open(os.path.join(_LIB, ".build.lock"), "w") as lock:
+                    fcntl.flock(lock, fcntl.LOCK_EX)
+                    build_torch()
+            try:
+                _torch = ctypes.CDLL(path)
+            except OSError as e:
+                raise NativeLibraryMissing("%s cannot be loaded (kernels that it calls are not in the native library that is loaded, or it is damaged): %s"
+                                           % (os.path.basename(path), e)) from None
+    return _torch
 
 
 def ensure_cuda(components=("all",)) -> ctypes.CDLL:

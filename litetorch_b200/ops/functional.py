@@ -492,25 +492,6 @@ def embedding(idx, table):
     return F.embedding(idx.to(torch.int64), table)
 
 
-def _once(name: str) -> None:
-    # (a second derivative would silently be that of a constant)
-    if torch.is_grad_enabled():
-        raise RuntimeError("%s is differentiable once" % name)
-
-
-class _TokenEmbedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, idx, table, scale, pad):
-        ctx.save_for_backward(idx)
-        ctx.rest = table.shape[0], scale, pad
-        return K.token_embedding(idx, table, scale)
-
-    @staticmethod
-    def backward(ctx, dout):
-        _once("token_embedding")
-        return None, K.token_embedding_grad(*ctx.saved_tensors, dout, *ctx.rest), None, None
-
-
 _KERNEL_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _INDEX_TYPES = (torch.int64, torch.int32)
 
@@ -541,7 +522,7 @@ def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0, 
         pad = int(padding_idx) % V
     flat = idx if idx.dim() == 1 and idx.is_contiguous() else idx.reshape(-1).contiguous()
     if table.is_cuda and table.dtype in _KERNEL_TYPES:
-        out = _TokenEmbedding.apply(flat, table if table.is_contiguous() else table.contiguous(), float(scale), pad)
+        out = K.token_embedding(flat, table if table.is_contiguous() else table.contiguous(), float(scale), pad)
         return out if flat is idx else out.view(*idx.shape, D)
     inside = ((flat >= 0) & (flat < V))[:, None]
     wide = table if table.dtype == torch.float64 else table.float()
@@ -568,7 +549,8 @@ class _Distillation(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, up):
-        _once("distillation_loss")
+        if torch.is_grad_enabled():                            # (a second derivative would silently be that of a constant)
+            raise RuntimeError("distillation_loss is differentiable once")
         z, room = ctx.saved_tensors
         ahead, ctx.ahead = ctx.ahead, None                     # handed out once
         if ahead is not None and torch.cuda.is_current_stream_capturing():

@@ -13,7 +13,7 @@ from ctypes import c_void_p, c_int, c_longlong, c_float
 
 import torch
 
-from .._native import cuda_lib
+from .._native import cuda_lib, torch_lib
 
 _vp, _i, _ll, _f, _d = c_void_p, c_int, c_longlong, c_float, ctypes.c_double
 
@@ -152,12 +152,26 @@ _LAUNCHES_PER_CALL = {"lt_gemm_num_tiles": 0, "lt_distill_places": 0, "lt_gemm_s
 _launches = [0]
 
 
+_node_ops = {}
+
+
+def _node(name):
+    """An operator of the library of autograd nodes."""
+    op = _node_ops.get(name)
+    if op is None:
+        torch_lib().lt_torch_launches.restype = c_longlong
+        op = _node_ops[name] = getattr(torch.ops.litetorch_b200, name).default
+    return op
+
+
 def launch_count() -> int:
-    return _launches[0]
+    return _launches[0] + (torch_lib().lt_torch_launches(0) if _node_ops else 0)
 
 
 def reset_launch_count():
     _launches[0] = 0
+    if _node_ops:
+        torch_lib().lt_torch_launches(1)
 
 
 class KernelError(RuntimeError):
@@ -1626,7 +1640,6 @@ def moe_expert_bwd(gu, dh_u, w, slot_src):
 
 # ------------------------------------------------------------------------------------------------ vocabulary: embedding, distillation, sampling
 _ELEM = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_INDEX = (torch.int64, torch.int32)
 
 
 def _on(t: torch.Tensor):
@@ -1634,51 +1647,11 @@ def _on(t: torch.Tensor):
     return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
-def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
-    """scale * table[idx] as [tokens, D] (fp32, bf16 or fp16, rounded once); a token outside the table gives zeros."""
-    V, D = table.shape
-    assert table.is_contiguous() and table.dtype in _ELEM and idx.device == table.device
-    if idx.dim() != 1 or idx.dtype not in _INDEX or not idx.is_contiguous():
-        idx = _dense_index(idx, torch.int64, torch.int32)
-    out = table.new_empty((idx.numel(), D))
-    with _on(table):
-        _check(_fn("lt_token_embedding_fwd")(_ELEM[table.dtype], idx.data_ptr(), 1 if idx.dtype == torch.int32 else 0, table.data_ptr(), out.data_ptr(),
-                                             idx.numel(), D, V, float(scale), _stream()), "lt_token_embedding_fwd")
-    return out
-
-
-def token_embedding_grad(idx: torch.Tensor, dout: torch.Tensor, vocab: int, scale: float = 1.0, padding_idx: int = -1) -> torch.Tensor:
-    """The gradient [vocab, D] of `token_embedding`'s table from dout [tokens, D]: sums in fp32 in the order of the tokens, rounded once, the same from run
-    to run.  Tokens outside the table and `padding_idx` give nothing."""
-    n, D = dout.shape
-    assert dout.dtype in _ELEM and idx.numel() == n and idx.device == dout.device
-    if idx.dim() != 1 or idx.dtype not in _INDEX or not idx.is_contiguous():
-        idx = _dense_index(idx, torch.int64, torch.int32)
-    if dout.stride(1) != 1:
-        dout = dout.contiguous()
-    size = dout.element_size()
-    grad = dout.new_empty((vocab, D))
-    # Few tokens and a small gradient: one launch, which reads all tokens for every 16 KB of it.  Replayed, one launch / sort and sums, us: 128 tokens, 8.4 MB 5.5 / 11.7;
-    # 1024, 8.4 MB 9.6 / 17.5; 2048, 8.4 MB 13.7 / 21.2; 2048, 64 KB 13.5 / 21.2; 256, 66 MB 15.7 / 15.8; but 4096, 64 KB 37 / 27; 512, 66 MB 17.8 / 16.4; 64, 263 MB 49 / 41.
-    if n <= 2048 and vocab * D * size <= 1 << 26 and n * vocab * D * size <= 1 << 34:
-        order = part = None
-        tile = 1
-    else:
-        # sorted rows that a CTA sums of 256 vectors of 16 bytes, or of 1024 columns: up to 32, so that there are eight CTAs an SM
-        chunks = -(-D // (256 * 16 // size if D * size % 16 == 0 else 1024))
-        tile = 8
-        while tile < 32 and n * chunks >= 2 * tile * 8 * 148:
-            tile *= 2
-        # the sorted list twice, 8 bytes an entry, and two rows for the pieces of every tile
-        room = torch.empty(16 * n + (n + tile - 1) // tile * 8 * D, dtype=torch.uint8, device=dout.device)
-        order = room.data_ptr()
-        part = order + 16 * n
-        _launches[0] += 3
-    with _on(dout):
-        _check(_fn("lt_token_embedding_bwd")(_ELEM[dout.dtype], idx.data_ptr(), 1 if idx.dtype == torch.int32 else 0, dout.data_ptr(), dout.stride(0), grad.data_ptr(),
-                                             n, D, int(vocab), float(scale), int(padding_idx), order, part, tile, _stream()),
-               "lt_token_embedding_bwd")
-    return grad
+def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: int = -1) -> torch.Tensor:
+    """scale * table[idx] as [tokens, D] (fp32, bf16 or fp16, rounded once) for dense tokens [n] and a dense table; a token outside the table gives zeros.  A
+    node of the autograd graph in C++ (csrc/torch_nodes): the gradient [V, D] is summed in fp32 in the order of the tokens and rounded once, the same from run
+    to run; tokens outside the table and `padding_idx` give nothing."""
+    return _node("token_embedding")(idx, table, scale, padding_idx)
 
 
 def _like_rows(z):

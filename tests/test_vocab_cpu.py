@@ -174,6 +174,15 @@ def test_parts_of_the_distillation_kernels_shared_memory():
     assert K._fn("lt_distill_places")(1025, 512, 5, places) < 0 and K._fn("lt_distill_places")(0, 512, 5, places) < 0
 
 
+def test_the_autograd_node_refuses_what_its_kernels_cannot_take():
+    """Checked before anything is launched; the public function makes dense tensors of what it is given."""
+    idx, table = torch.tensor([1, 2]), torch.randn(5, 4)
+    for args in ((idx, table), (idx, table.to("meta")), (idx, table.long()), (idx.float(), table), (idx, table[0])):
+        with pytest.raises(RuntimeError, match="dense tokens and a dense table"):
+            K.token_embedding(*args)
+    assert K.launch_count() >= 0
+
+
 class _Overrun(Exception):
     pass
 

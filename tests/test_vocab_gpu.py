@@ -105,6 +105,50 @@ def test_gradients_and_tokens_that_do_not_lie_side_by_side(dtype):
         _check_embed(idx, 11, 64, dtype, 1.5, 4, 10, dout)
 
 
+def test_the_embedding_in_an_autograd_graph():
+    """Both passes count as launches; the graph may be kept, checkpointed, hooked and run after what it read was freed, but not with tokens that changed since."""
+    from torch.utils.checkpoint import checkpoint
+    from litetorch_b200.ops import functional as Fn, kernels as K
+    g = _gen(40)
+    idx = torch.randint(0, 50, (6, 7), device="cuda", generator=g)
+    table = torch.randn(50, 24, device="cuda", generator=g, requires_grad=True)
+    dout = torch.randn(6, 7, 24, device="cuda", generator=g)
+    want, bound = ref.embedding_grad(idx, dout, 50, 2.0)
+    bound = bound + ref.rounding(want, torch.float32) + bound * 2.0 ** -23
+    Fn.token_embedding(idx, table)
+    K.reset_launch_count()
+    out = Fn.token_embedding(idx, table, 2.0)
+    seen = []
+    out.register_hook(lambda d: seen.append(d.shape))
+    first, = torch.autograd.grad(out, table, dout, retain_graph=True)
+    assert K.launch_count() == 2 and seen == [(6, 7, 24)]
+    keep = first.clone()
+    first.zero_()
+    again, = torch.autograd.grad(out, table, dout)
+    assert torch.equal(again, keep)
+    _within(again, want, bound)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out, table, dout)
+    checkpoint(lambda w: Fn.token_embedding(idx, w, 2.0), table, use_reentrant=False).backward(dout)
+    assert torch.equal(table.grad, keep)
+    (Fn.token_embedding(idx, table, 2.0) + Fn.token_embedding(idx, table, 2.0)).backward(dout)
+    _within(table.grad, 3 * want, 4 * bound)
+    out = Fn.token_embedding(idx, table, 2.0)
+    del table.grad
+    idx.copy_(49 - idx)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward(dout)
+    with torch.no_grad():
+        assert not Fn.token_embedding(idx, table).requires_grad
+    assert not Fn.token_embedding(idx, table.detach()).requires_grad
+    with torch.inference_mode():
+        assert torch.equal(Fn.token_embedding(idx, table), table.detach()[idx])
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            Fn.token_embedding(idx, fwd.make_dual(table.detach(), torch.ones_like(table)))
+
+
 def test_no_tokens_and_empty_rows():
     from litetorch_b200.ops import functional as Fn
     table = torch.randn(5, 8, device="cuda", requires_grad=True)
