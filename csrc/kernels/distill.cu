@@ -814,8 +814,10 @@ int distill(DistillArgs a, float* out, unsigned* finished, cudaStream_t st) {
   a.cluster_log = 0;
   while ((1 << a.cluster_log) < kDistillCluster && vecs > (per * kDistillThreads) << a.cluster_log) ++a.cluster_log;
   // rows that a CTA holds are read once (2048 x 32000 fp16, 128 entries: 82 us, twice 93; losses alone 47 and 43); few rows: clusters, so that all SMs have work
-  // Many entries in a short row make chains whose threads the others wait for (8192 x 4001 fp32, 256 entries: 370 us, 180 as a long row; 1003 bf16 411 and 116).
-  const bool dense = a.grad && !few && 8ll * a.K >= vecs;
+  // Many entries in a short row make chains whose threads the others wait for.  Loss and gradient / gradient alone, us, held and as a long row: 8192 x 1003 bf16 with 128
+  // entries 73 / 50 and 107 / 67, 224: 117 / 89 and 115 / 69, 255: 148 / 109 and 122 / 70, 256 (whose chains are twice as wide, of fewer vectors a thread): 372 / 314 and
+  // 117 / 70; 8192 x 4001 fp32 with 128: 126 / 81 and 147 / 95, 224: 147 / 98 and 156 / 101, 255: 165 / 106 and 161 / 100, 256: 270 / 179 and 157 / 100.
+  const bool dense = a.grad && a.K > 224 && 8ll * a.K >= vecs;
   if (vecs <= (per * kDistillThreads) << a.cluster_log && ((a.cluster_log == 0 && !dense) || a.N < 2 * sm_count())) {
     // few rows: more CTAs for each
     while ((1 << a.cluster_log) < kDistillCluster && (long long)a.N << (a.cluster_log + 1) <= sm_count() && vecs >> a.cluster_log >= 512) ++a.cluster_log;

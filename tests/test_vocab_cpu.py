@@ -143,8 +143,7 @@ def test_the_native_calls_refuse_what_they_cannot_take():
     embed = lambda type=0, n=4, D=8, V=9: fn("lt_token_embedding_fwd")(type, None, 0, None, None, n, D, V, 1.0, None)
     grad = lambda type=0, n=4, D=8, V=9, tile=8: fn("lt_token_embedding_bwd")(type, None, 0, None, 8, None, n, D, V, 1.0, -1, None, None, tile, None)
     for rc in (embed(type=3), embed(type=-1), embed(n=-1), embed(n=1 << 31), embed(D=-1), embed(D=(1 << 30) + 1), embed(V=0), grad(type=3), grad(n=-1), grad(n=(1 << 31) - 4096),
-               grad(D=-1), grad(D=(1 << 30) + 1), grad(V=0), grad(V=(1 << 31) - 1), grad(tile=0), grad(tile=65),
-               grad(n=2049)):                                        # (without a workspace: one launch, which takes up to 2048 tokens)
+               grad(D=-1), grad(D=(1 << 30) + 1), grad(V=0), grad(V=(1 << 31) - 1), grad(tile=0), grad(tile=65)):
         assert rc < 0
     assert embed(n=0) == embed(D=0) == grad(D=0) == 0
 
@@ -172,6 +171,11 @@ def test_parts_of_the_distillation_kernels_shared_memory():
                 assert entries >= 3 * threads * vectors * 16 and pairs >= entries + 5 * 8 * top and chains >= pairs + 4 * 8 * 8 * (threads // 32)
                 assert links >= chains + 4 * 8 * link * threads and end >= links + 4 * link * top and end <= 227 * 1024 - 1024
     assert K._fn("lt_distill_places")(1025, 512, 5, places) < 0 and K._fn("lt_distill_places")(0, 512, 5, places) < 0
+
+
+def test_a_gradient_without_a_workspace_is_one_of_few_tokens():
+    """One launch takes up to 2048 tokens; refused before anything is launched."""
+    assert K._fn("lt_token_embedding_bwd")(0, None, 0, None, 8, None, 2049, 8, 9, 1.0, -1, None, None, 1, None) < 0
 
 
 def test_the_autograd_node_refuses_what_its_kernels_cannot_take():

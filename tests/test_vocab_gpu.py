@@ -665,6 +665,18 @@ def test_many_short_rows_with_many_entries(dtype, V, K):
     _check_distill(z, t, cls, 1.5, "none", torch.rand(400, device="cuda", generator=g))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,K", [(515, 255), (515, 224), (4001, 225), (20000, 255), (20001, 224)])
+def test_many_rows_on_both_sides_of_many_entries(dtype, V, K):
+    """Rows that a CTA could hold, with so many entries that they are taken as long ones, and with a few less."""
+    g = _gen(V + K)
+    z = (torch.randn(400, V, device="cuda", generator=g) * 3).to(dtype)
+    t, cls = _teacher(400, V, K, dtype, g, ragged=True)
+    cls[7] = cls[7, :1]
+    _check_distill(z, t, cls, 1.5, "mean")
+    _check_distill(z, t, cls, 1.5, "none", torch.rand(400, device="cuda", generator=g))
+
+
 def test_two_streams_at_once():
     """Calls of the same kind on two streams have nothing in common."""
     from litetorch_b200.ops import functional as Fn
