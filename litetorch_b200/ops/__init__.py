@@ -271,7 +271,9 @@ class Ops:
     @staticmethod
     def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> Tuple[Tensor, Tensor]:
         """(tokens, log probabilities) of logits [..., V], drawn with the random numbers uniform [...] in [0, 1); every parameter is a number or a tensor with
-        one for every row (`functional.sample_tokens` says what they do)."""
+        one for every row (top_k: floats or integers; `functional.sample_tokens` says what they do)."""
+        if isinstance(top_k, Tensor) and _unwrap(top_k).is_floating_point():
+            top_k = _unwrap(top_k).to(torch.int64)
         tokens, logprobs = Fn.sample_tokens(_unwrap(logits), _unwrap(uniform), *(_unwrap(v) if isinstance(v, Tensor) else v for v in (temperature, top_k, top_p, min_p)))
         return _w(tokens), _w(logprobs)
 

@@ -295,6 +295,17 @@ def test_a_row_of_its_own_for_every_loss():
     assert not z.grad[1::2].any() and bool(z.grad[::2].any(1).all())
 
 
+def test_a_top_k_for_every_row_may_be_floats():
+    """As indices of the other operators on framework tensors may."""
+    g = _gen(8)
+    z, u, k = torch.randn(4, 30, generator=g), torch.rand(4, generator=g), torch.tensor([1.0, 3.0, 0.0, 30.0])
+    tokens, logs = lt.Ops.sample_tokens(lt.Tensor(z), lt.Tensor(u), 0.9, lt.Tensor(k))
+    want = Fn.sample_tokens(z, u, 0.9, k.long())
+    assert torch.equal(_unwrap(tokens), want[0]) and torch.equal(_unwrap(logs), want[1])
+    with pytest.raises(TypeError):                                # (a number that is none of a count stays refused)
+        lt.Ops.sample_tokens(lt.Tensor(z), lt.Tensor(u), 0.9, 2.5)
+
+
 def _model(vocab=64):
     from litetorch_b200.models.llama import LlamaConfig, LlamaEngine
     cfg = LlamaConfig(vocab_size=vocab, n_layers=1, d_model=32, n_heads=2, n_kv_heads=1, head_dim=16, ffn=48, max_seq=64)
