@@ -623,8 +623,8 @@ def _sample_plain(z, u, tau, k, p, low):
     first = (torch.arange(V, device=z.device) < k) | (k <= 0)
     ranked = e.gather(1, order) * first
     before = ranked.cumsum(1) - ranked
-    first &= (before < p * ranked.sum(1, keepdim=True)) | (p >= 1.0) | (torch.arange(V, device=z.device) == 0)
-    keep = torch.zeros_like(first).scatter_(1, order, first) & (e >= low.clamp(max=1.0))
+    first &= (before < p * ranked.sum(1, keepdim=True)) | ~(p < 1.0) | (torch.arange(V, device=z.device) == 0)
+    keep = torch.zeros_like(first).scatter_(1, order, first) & ~(e < low.clamp(max=1.0))
     e = e * keep
     total = e.sum(1, keepdim=True)
     cum = e.cumsum(1)
@@ -645,8 +645,8 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
         min_p > 0    those stay with w >= min_p
 
     and the token is the first, by index, at which the cumulated mass of what stays exceeds `uniform` times all of it; its log probability is that among what
-    stays.  temperature <= 0 takes the largest logit.  Every parameter is a number or a tensor with one for every row.  NaN counts as -inf; a row of nothing
-    else gives token -1.  The choice is that of exact sums: it does not change with the batch, the device or the run."""
+    stays.  temperature <= 0 takes the largest logit.  Every parameter is a number or a tensor with one for every row, where a
+    NaN is a temperature of 0, or a limit that is off.  A logit that is NaN counts as -inf; a row of nothing else gives token -1.  The choice is that of exact sums: it does not change with the batch, the device or the run."""
     if not logits.is_floating_point() or logits.dim() < 1:
         raise TypeError("sample_tokens: logits [..., V] of floating-point numbers are expected")
     lead, V = logits.shape[:-1], logits.shape[-1]

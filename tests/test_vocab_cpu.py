@@ -306,6 +306,20 @@ def test_a_top_k_for_every_row_may_be_floats():
         lt.Ops.sample_tokens(lt.Tensor(z), lt.Tensor(u), 0.9, 2.5)
 
 
+def test_nan_among_the_rows_parameters():
+    """A temperature that is NaN is one of 0, a limit that is NaN is off; the other rows are as they were."""
+    g = _gen(9)
+    z, u = torch.randn(3, 200, generator=g) * 3, torch.rand(3, generator=g)
+    nan = math.nan
+    for kw, off in ((dict(temperature=torch.tensor([0.7, nan, 1.5])), dict(temperature=torch.tensor([0.7, 0.0, 1.5]))),
+                    (dict(top_p=torch.tensor([0.5, nan, 0.9])), dict(top_p=torch.tensor([0.5, 1.0, 0.9]))),
+                    (dict(min_p=torch.tensor([0.1, nan, 0.9])), dict(min_p=torch.tensor([0.1, 0.0, 0.9]))),
+                    (dict(top_k=4, top_p=torch.tensor([0.5, nan, 0.9]), min_p=torch.tensor([nan, nan, 0.2])),
+                     dict(top_k=4, top_p=torch.tensor([0.5, 1.0, 0.9]), min_p=torch.tensor([0.0, 0.0, 0.2])))):
+        got, want = Fn.sample_tokens(z, u, **kw), Fn.sample_tokens(z, u, **off)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), kw
+
+
 def _model(vocab=64):
     from litetorch_b200.models.llama import LlamaConfig, LlamaEngine
     cfg = LlamaConfig(vocab_size=vocab, n_layers=1, d_model=32, n_heads=2, n_kv_heads=1, head_dim=16, ffn=48, max_seq=64)

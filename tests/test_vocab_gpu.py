@@ -406,6 +406,27 @@ def test_masks_infinities_and_nan(dtype):
         assert tokens[0] == tokens[1] == -1 and tokens[2] == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_parameters_of_rows_that_are_no_numbers(dtype):
+    """NaN is a temperature of 0 or a limit that is off; an infinite temperature makes all finite logits alike."""
+    g = _gen(41)
+    nan = math.nan
+    for V in (500, 50257):
+        z = _peaked(4, V, dtype, g)
+        z[3, ::3] = -math.inf
+        u = torch.rand(4, device="cuda", generator=g)
+        p, low = torch.tensor([0.5, nan, math.inf, -math.inf], device="cuda"), torch.tensor([nan, 0.1, -math.inf, math.inf], device="cuda")
+        tau = torch.tensor([0.7, math.inf, nan, math.inf], device="cuda")
+        p1, low1, tau1 = (torch.where(torch.isnan(a), b, a) for a, b in ((p, 1.0), (low, 0.0), (tau, 0.0)))
+        from litetorch_b200.ops import functional as Fn
+        for k in (0, 7, 400):
+            for args, same in (((tau, k, 1.0, 0.0), (tau1, k, 1.0, 0.0)), ((0.8, k, p, 0.0), (0.8, k, p1, 0.0)), ((0.8, k, 1.0, low), (0.8, k, 1.0, low1)), ((tau, k, p, low), (tau1, k, p1, low1))):
+                tokens, logs = Fn.sample_tokens(z, u, *args)
+                want, want_logs = ref.sample(z, u, *same)
+                assert torch.equal(tokens.cpu(), want)
+                _within(logs, want_logs, want_logs.abs() * 2.0 ** -23 + 1e-9)
+
+
 def test_random_numbers_at_and_outside_their_range():
     from litetorch_b200.ops import functional as Fn
     z = _peaked(7, 999, torch.float32, _gen(13))
