@@ -128,6 +128,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
 }
 
+// A thread's asynchronous copy of 16 bytes.
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+
 // ----------------------------------------------------------------------------------------------
 // TMA (tiled bulk tensor copies; no cluster multicast anywhere)
 // ----------------------------------------------------------------------------------------------

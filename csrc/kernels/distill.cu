@@ -157,7 +157,6 @@ __device__ __forceinline__ void warp_max_sum(float& m, float& s, float c) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
 }
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 // The first `bytes` of 16 (all that is read); the rest becomes zero.
 __device__ __forceinline__ void copy_async16_part(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -243,8 +242,10 @@ struct DistillSmem {
 // A CTA, or for few rows a cluster of them, holds a row, every thread up to VPT vectors of 16 bytes: a row is read from global memory once.  The threads go over their vectors twice, first
 // for the warps' maxima and sums, which go to all warps of the cluster, and then for the gradient; between the two they do the first pass over the
 // next row, so that nobody waits for the exchange, and the rows after that are on their way into shared memory.  There is no barrier of all threads:
-// a thread reads the vectors that it fetched itself, and one mbarrier a row counts the pairs that arrive and this CTA's warps.  A warp that has passed the one of
-// row i - 2 knows that all have begun row i - 1 and are through with row i - 4: what rows share lies in as many places as that takes.
+// a thread reads the vectors that it fetched itself, and one mbarrier a row counts the pairs that arrive and this CTA's warps.  A warp arrives there after its first pass
+// over the row, that is, after its second pass over the row two before.  One in its first pass over row i has passed the barrier of row i - 2, so that the slowest may be in its
+// second pass over row i - 3: pairs and chains lie in four places.  One that fetches row i + 2 has passed that of row i - 1, and the slowest may be in its second
+// pass over row i - 2: entries lie in five.
 // The teacher's classes are chained by the vector they lie in; the thread that writes the vector writes them again, from the 32-bit values.
 // EVEN: all rows begin and end with a vector.  LINK: the type that numbers entries.
 template <typename T, bool EVEN, typename LINK, int VPT>

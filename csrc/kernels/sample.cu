@@ -4,11 +4,12 @@
 //   top-k: the first k stay;  top-p: those stay whose predecessors' mass is below p times the mass of what stayed;  min-p: those stay with w_j >= min_p
 //   token = the first index at which the cumulated mass of what stays (in index order) exceeds u times all of it
 //
-// The result is a choice, so it must not depend on the order in which the GPU adds.  Weights are whole numbers of 2^-44 (from 64-bit exponentials):
-// their sums are exact in 64 bits for up to 2^19 tokens, in any order, and the masses next to a border are off by less than 2^-45 for each token before it.
+// The result is a choice, so it must not depend on the order in which the GPU adds.  Weights are whole numbers of 2^-44, so that their sums are exact in 64 bits for up
+// to 2^19 tokens, in any order.  Each is off by up to 2^-42.6 of itself (the series of its exponential, always too small) and by half of 2^-44: what weighs less than 2^-45 of
+// the largest weighs nothing, and a border lies within 2^-42.6 of the mass before it and 2^-45 for each token there of where exact weights would have it.
 //
-// A cluster of CTAs takes a row.  Limits in the order are found by radix selection on order-preserving keys of the logits: a histogram of counts
-// (top-k) or of masses (top-p) over the next 11 bits of the keys that share the bits found so far.
+// A cluster of CTAs takes a row.  Limits in the order are found by selection on order-preserving keys of the logits: a histogram of counts
+// (top-k) or of masses (top-p) over up to 1024 equal pieces of the interval of keys that is left, until pieces are single keys.
 #include "lt_cuda.h"
 
 #include "common/elem.cuh"
@@ -71,7 +72,7 @@ struct Weigh {
   double md, k;                 // the largest logit, log2(e) / tau
 };
 // 2^44 times the weight of a logit, to the nearest whole number: 2^y with y = 16ths + r, |r| <= 1/32, the 16ths from a table, 2^r by the exponential series up to the
-// fifth power (the next term is below 2^-42).  Adding 256 to the weight leaves the whole number in the low bits of the sum.  No branches: the compiler works at
+// fifth power (the next term is below 2^-42.6).  Adding 256 to the weight leaves the whole number in the low bits of the sum.  No branches: the compiler works at
 // several at once, each of which is a long chain.  Of an infinite largest logit only its equals weigh anything.
 __device__ __forceinline__ u64 mass_of(float z, const Weigh& q, const double* table) {
   const double y = (double(z) - q.md) * q.k;                  // (the difference first: it is exact, and 0 for the largest)
@@ -120,8 +121,6 @@ template <typename T> __device__ __forceinline__ uint4 no_nan(uint4 u) {
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
-
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 
 struct SampleShared {
   uint32_t hist[kSampleBins];

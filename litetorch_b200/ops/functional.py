@@ -565,7 +565,10 @@ def distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         T^2 sum_k p_k (log p_k - log q[idx_k]),   p = softmax(teacher_logits / T) over the K entries,   q = softmax(logits / T) over all V classes
 
     An entry whose class is outside [0, V) (-1 for padding) or whose logit is -inf is not there; a row without any has loss 0 and no gradient.
-    reduction: "mean" over the rows that have a teacher, "sum", or "none" (a loss for every row, fp32).  The teacher gets no gradient."""
+    reduction: "mean" over the rows that have a teacher, "sum", or "none" (a loss for every row, fp32).  The teacher gets no gradient.
+
+    Rows of logits have one distance from each other; logits of another layout (`logits[:, :-1]` of several sequences) are copied first, and their gradient is copied
+    back.  All positions with a teacher of -1 for the last need no copy."""
     if not logits.is_floating_point() or not teacher_logits.is_floating_point():
         raise TypeError("distillation_loss: logits are floating-point numbers")
     if teacher_idx.dtype not in _INDEX_TYPES:
@@ -645,8 +648,12 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, 
         min_p > 0    those stay with w >= min_p
 
     and the token is the first, by index, at which the cumulated mass of what stays exceeds `uniform` times all of it; its log probability is that among what
-    stays.  temperature <= 0 takes the largest logit.  Every parameter is a number or a tensor with one for every row, where a
-    NaN is a temperature of 0, or a limit that is off.  A logit that is NaN counts as -inf; a row of nothing else gives token -1.  The choice is that of exact sums: it does not change with the batch, the device or the run."""
+    stays.  temperature <= 0 takes the largest logit.  Every parameter is a number or a tensor with one for every row, where a NaN is a temperature of 0, or a
+    limit that is off.  A logit that is NaN counts as -inf; a row of nothing else gives token -1.
+
+    On a GPU the choice changes neither with the batch nor with the run: w is a whole number of 2^-44 (off by up to 2^-42.6 of itself, and nothing below 2^-45), and sums
+    of such numbers are exact.  The CPU's form adds 64-bit floats, so that the two may differ where `uniform` lies that close to a border.  Rows have one distance from
+    each other; logits of another layout (`logits[:, :-1]` of several sequences) are copied first."""
     if not logits.is_floating_point() or logits.dim() < 1:
         raise TypeError("sample_tokens: logits [..., V] of floating-point numbers are expected")
     lead, V = logits.shape[:-1], logits.shape[-1]
