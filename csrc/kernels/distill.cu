@@ -543,9 +543,9 @@ __global__ void __launch_bounds__(kDistillThreads, 1) distill_kernel(DistillArgs
 
 // Many long rows: a CTA goes over a row twice, the second time mostly out of L2 (of rows of 256 KB 296 are under way: 76 MB), and writes past it.  Nothing is
 // exchanged between CTAs, and two an SM with up to 63 registers a thread fill all 148; the clusters above find places for 132.  It moves the 2.1 GB of 4096 x 128256 bf16
-// logits and their gradient in 450 us with teacher and losses (cluster kernel: 506; the copy rate would allow 326), 1000 x 50257 fp32 in 97 us (127); losses
-// alone read 1.05 GB in 195 us (348).  What bounds it: two exponentials an element take the special function units 230 us, and a CTA's two passes do not
-// overlap with each other.  Three CTAs an SM of 40 registers spill (500 us), 1024 threads in one CTA wait for each other (509 us).
+// logits and their gradient in 450 to 470 us with teacher and losses (cluster kernel: 506; the copy rate would allow 326), 1000 x 50257 fp32 in 97 us (127); losses
+// alone read 1.05 GB in 195 us (348).  Nothing is full (DRAM 61 %, exponentials 55 %, issue 41 %): loads go to registers and stop at the end of each pass and row, and
+// a CTA's two passes do not overlap with each other.  Three CTAs an SM of 40 registers spill (500 us), 1024 threads in one CTA wait for each other (509 us).
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads) distill_long_kernel(DistillArgs a) {
   constexpr int VEC = kVec<T>, U = 4;

@@ -518,10 +518,10 @@ __constant__ double kSixteenths[16] = {1.0, 1.0442737824274138403, 1.09050773266
 //                          each is compared with each: its place in the order and the mass before it
 //   the general way        where that list would be long
 //
-// What bounds it: one row is a chain of exchanges (1 x 32000 bf16 with top-p: 16 us; read in 0.01).  A short list needs one pass over keys: 256 x 50257 bf16, top-k
-// and min-p, 25 us at 1.1 TB/s.  Masses of all tokens take eleven 64-bit operations and a table entry each: 512 x 128256 bf16 from the whole distribution
-// 197 us, the pipe for them 21 % busy and 37 % of issue slots taken; its chains of fixed latencies bound it, though CTAs of 256 threads, four an SM,
-// whose rows lie in L2 instead of shared memory take 197 as well (and 64 x 128256 fp32 160).
+// What it takes: one row is a chain of exchanges (1 x 32000 bf16 with top-p: 12 us replayed; read in 0.01).  A short list needs one pass over keys: 256 x 50257 bf16, top-k
+// and min-p, 25 us at 1.1 TB/s, in two waves of CTAs.  Masses of all tokens take eleven 64-bit operations and a table entry each: 512 x 128256 bf16 from the whole
+// distribution 189 to 198 us, where nothing is full (with 16 warps an SM the pipe for them 21 % busy and 37 % of issue slots taken): too little is under way at once.  CTAs
+// of 256 threads, four an SM, whose rows lie in L2 instead of shared memory take 197 as well (and 64 x 128256 fp32 160).
 template <typename T, int THREADS>                            // up to so many
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_kernel(SampleArgs a) {
   constexpr int VEC = kVec<T>;
@@ -828,7 +828,7 @@ int lt_sample_tokens(int type, const void* z, long long ldz, const void* u, int 
   while (ctas < kSampleCluster && (long long)rows * ctas * 2 <= 2 * sm_count() && V / ctas >= 8192) ctas *= 2;
   if ((long long)rows * ctas > 0x7fffffffll) return -int(kStatusBadArgument);
   const bool many = (long long)rows * ctas > 2 * sm_count();
-  // (rows whose part takes so much memory that few CTAs share an SM: 512 threads; 64 x 128256 fp32 106 us, with 256 threads 121, 512 x 128256 bf16 197 and 205)
+  // (rows whose part takes so much memory that few CTAs share an SM: 512 threads; 64 x 128256 fp32 106 us, with 256 threads 121, 512 x 128256 bf16 197 and 205, in one run)
   while (threads > (many && bytes(ctas) > 48 * 1024 ? 512 : 128) && (many || vecs / ctas + 1 <= threads / 2)) threads /= 2;
   const bool held = (vecs / ctas + 1) * 16 <= kSampleHold;
   const int smem = held ? (vecs / ctas + 1) * 16 : 0;

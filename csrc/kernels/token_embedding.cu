@@ -15,7 +15,7 @@
 //   join   adds the pieces, in order
 //
 // What bounds it: the bytes of the table's gradient where they are many (8192 tokens, 128256 x 4096 bf16: rows and gradient 191 us, 96 % of the copy rate; the clear
-// alone writes 1.05 GB in 141 us and hides the sort), else launches one behind the other (2048 tokens, 32000 x 2048 bf16: 41 us replayed from a graph, of which the
+// alone writes 1.05 GB in 141 us and hides the sort), else launches one behind the other (2048 tokens, 32000 x 2048 bf16: 37 us replayed from a graph, of which the
 // sort takes 17 and the join 11).  Rows that do not begin at 16 bytes are moved element by element: 40001 x 1027 fp32
 // 145 us, where the bytes take 82.
 #include "lt_cuda.h"

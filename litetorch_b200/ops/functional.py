@@ -503,8 +503,8 @@ def _whole(name: str, t: torch.Tensor) -> None:
 
 def token_embedding(idx: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """scale * table[idx] for tokens idx [...] and a table [V, D]: [..., D], rounded once from fp32.  A token outside [0, V) gives a row of zeros and no
-    gradient; `padding_idx` (negative: from the end) gives its row and no gradient.  The table's gradient is summed over the sorted tokens in fp32 and in their
-    order, then rounded once, where `embedding` adds bf16 numbers with atomics: it is the same from run to run."""
+    gradient; `padding_idx` (negative: from the end) gives its row and no gradient.  The table's gradient is summed in fp32 in the order of the tokens, then
+    rounded once, where `embedding` adds bf16 numbers with atomics: it is the same from run to run.  It is differentiable once."""
     if table.dim() != 2 or not table.is_floating_point():
         raise TypeError("token_embedding: the table is a matrix of floating-point numbers")
     V, D = table.shape
